@@ -30,6 +30,22 @@ std::vector<at::Tensor> router_topk_forward(const at::Tensor& logits, int64_t to
 at::Tensor router_topk_backward(const at::Tensor& scores, const at::Tensor& weights, const at::Tensor& experts,
                                 const at::Tensor& dscores, const at::Tensor& dweights, double norm_p);
 
+// model_glue.cpp: expert selection and distillation
+std::vector<at::Tensor> select_experts_forward(const at::Tensor& logits, int64_t top_k, bool use_sigmoid,
+                                               const c10::optional<at::Tensor>& bias, int64_t groups,
+                                               int64_t top_groups, int64_t norm_p, double scale);
+at::Tensor select_experts_backward(const at::Tensor& logits, const at::Tensor& experts,
+                                   const c10::optional<at::Tensor>& dscores,
+                                   const c10::optional<at::Tensor>& dweights, bool use_sigmoid, int64_t norm_p,
+                                   double scale);
+std::vector<at::Tensor> distill_forward(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& ids,
+                                        const c10::optional<at::Tensor>& targets, double temperature,
+                                        double hard_weight, double scale, bool want_grad, bool in_place);
+at::Tensor distill_backward(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& ids,
+                            const c10::optional<at::Tensor>& targets, const at::Tensor& stats,
+                            const at::Tensor& grad_out, double temperature, double hard_weight, double scale);
+void scale_unless_one_op(at::Tensor x, const at::Tensor& factor);
+
 // torch_glue.cpp: grouped GEMM
 bool grouped_gemm_supported(const at::Tensor& a, const at::Tensor& b, bool trans_a, bool trans_b,
                             int64_t num_groups);
@@ -56,7 +72,6 @@ std::vector<at::Tensor> expert_rows_backward(
     int64_t capacity, int64_t pair);
 int64_t read_status(bool clear);
 int64_t launch_count();
-void count_launches(int64_t n);
 at::Tensor gemm_role_timers(const at::Tensor& like);
 at::Tensor bsmm_op(int64_t mode, const at::Tensor& a, bool a_mn, const at::Tensor& b, bool b_mn,
                    const at::Tensor& idx0, const c10::optional<at::Tensor>& idx1,
@@ -140,6 +155,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("binned_scatter_wgrad", &mb::binned_scatter_wgrad);
   m.def("router_topk_forward", &mb::router_topk_forward);
   m.def("router_topk_backward", &mb::router_topk_backward);
+  m.def("select_experts_forward", &mb::select_experts_forward);
+  m.def("select_experts_backward", &mb::select_experts_backward);
+  m.def("distill_forward", &mb::distill_forward, "Per-row loss, row statistics and, if wanted, the gradient");
+  m.def("distill_backward", &mb::distill_backward);
+  m.def("scale_unless_one_", &mb::scale_unless_one_op);
   m.def("grouped_gemm_supported", &mb::grouped_gemm_supported);
   m.def("grouped_gemm", &mb::grouped_gemm);
   m.def("combine_rows", &mb::combine_rows_op);

@@ -73,6 +73,50 @@ cudaError_t router_topk_bwd(DType type, const void* scores, const int64_t* exper
                             const void* dweights, int64_t tokens, int num_experts, int top_k, float norm_p,
                             void* dlogits, cudaStream_t stream);
 
+// ---- select_experts.cu ----------------------------------------------------------
+constexpr int kSelectMaxTopK = 32;     // a lane of the warp that owns a token holds one choice
+constexpr int kSelectMaxGroups = 32;
+struct SelectArgs {
+  int64_t tokens;
+  int experts, top_k, groups, top_groups;
+  int norm_p;                          // 0 (weights are not divided), 1 or 2
+  bool use_sigmoid;
+  float scale;
+  const float* bias;                   // [experts], nullable
+  int group_lanes, shared_stride;      // filled by the launchers
+};
+cudaError_t select_experts_fwd(DType type, const void* logits, SelectArgs args, void* scores, void* weights,
+                               int64_t* ids, cudaStream_t stream);
+// `dscores` (nullable) has rows `dscores_stride` elements apart (0: one row for all tokens); `dweights` nullable.
+cudaError_t select_experts_bwd(DType type, const void* logits, SelectArgs args, const int64_t* ids,
+                               const void* dscores, int64_t dscores_stride, const void* dweights, void* dlogits,
+                               cudaStream_t stream);
+
+// ---- distill.cu -----------------------------------------------------------------
+constexpr int kDistillMaxTop = 1024;
+constexpr int kDistillTimeout = 9;
+struct DistillArgs {
+  const void* logits;                  // [rows, vocab]
+  int64_t rows;
+  int vocab, top;
+  const void* values;                  // [rows, top] teacher logits of type `value_type`
+  DType value_type;
+  const void* ids;                     // [rows, top], int64 (`ids64`) or int32; outside [0, vocab): unused
+  bool ids64;
+  const int64_t* targets;              // [rows], nullable; outside [0, vocab): none
+  float temperature, hard_weight;
+  float scale;                         // of the gradient (1 / rows)
+  int* status;                         // receives kDistillTimeout when a copy never completes
+};
+// Per-row loss and `stats` [rows, 3]: the largest logit and the sums of e^((z - max) / T) and e^(z - max);
+// with `grad` (may be the logits themselves) also the gradient of scale * sum(loss).
+cudaError_t distill_fwd(DType type, const DistillArgs& args, float* loss, float* stats, void* grad, cudaStream_t stream);
+// The gradient alone, from the statistics of a forward pass, times *grad_out.
+cudaError_t distill_bwd(DType type, const DistillArgs& args, const float* stats, const float* grad_out, void* grad,
+                        cudaStream_t stream);
+// x *= *factor; returns without touching x where the factor is one.
+cudaError_t scale_unless_one(DType type, void* x, int64_t numel, const float* factor, int sms, cudaStream_t stream);
+
 // ---- optim.cu -----------------------------------------------------------------
 struct AdamTensor {
   void* param;        // 16-bit (or fp32) shadow weights the model computes with

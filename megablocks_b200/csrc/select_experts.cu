@@ -1,0 +1,455 @@
+// Expert selection with a balancing bias and expert groups, forward and backward.
+//
+//   s_e = softmax(x)_e or sigmoid(x_e),   c_e = s_e + bias_e   (the bias takes part in the choice only)
+//   a group's value is the sum of its two largest c; the best `top_groups` groups stay
+//   the top_k largest c of those groups are chosen, w_i = scale * s_i / ||s_chosen||_p  (p = 0: not divided)
+//   scores_e = s_e / sum_e s_e   (for the softmax that is s_e itself)
+//
+// One warp owns a token and holds its experts in registers, PL a lane, fetched V at a time.  The order of
+// the experts is exact: equal values go to the lowest id, and values that 32 bits cannot tell apart are
+// ordered by their 64-bit ones.  Without a bias the scores have the order of the logits, which are compared
+// as they are.  With one, each comparison that decides (neighbours in the chosen order, the last chosen one
+// and the next, the last group that stays and the next) is checked against a bound of the arithmetic's
+// error; a token with a closer pair, a few in a thousand, is chosen again from scores in 64 bits.
+#include "common.cuh"
+
+namespace mb {
+
+namespace {
+
+constexpr int kWarps = 4;
+
+__device__ __forceinline__ float warp_sum_f(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// Unsigned key in the order of the floats; NaN counts as +infinity, -0 as 0.  0 is below every key.
+__device__ __forceinline__ unsigned ordered(float v) {
+  unsigned u = __float_as_uint(v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) u = 0x7f800000u;
+  if (u == 0x80000000u) u = 0u;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(unsigned k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// Expert of slot j of a lane; ascending in j.
+template <int V>
+__device__ __forceinline__ int expert_of(int j, int lane) {
+  return (j / V) * (32 * V) + lane * V + j % V;
+}
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Slots {
+  T v[V];
+};
+
+template <typename T, int PL, int V>
+__device__ __forceinline__ void load_slots(const T* row, int lane, int experts, float fill, float (&x)[PL]) {
+#pragma unroll
+  for (int j = 0; j < PL; j += V) {
+    const int e = expert_of<V>(j, lane);
+    if (e < experts) {          // experts % V == 0
+      const Slots<T, V> p = *reinterpret_cast<const Slots<T, V>*>(row + e);
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[j + k] = to_float(p.v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[j + k] = fill;
+    }
+  }
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+// Scores of a lane's slots; returns what a single score needs to be taken again (maximum and inverse sum
+// of the softmax) and the sum of all scores.
+struct RowStat {
+  float top, inv, total;
+};
+
+template <int PL, int V>
+__device__ __forceinline__ RowStat scores_of(const float (&x)[PL], int lane, int experts, bool use_sigmoid,
+                                             float (&s)[PL]) {
+  RowStat r{0.f, 1.f, 0.f};
+  float sum = 0.f;
+  if (use_sigmoid) {
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      s[j] = expert_of<V>(j, lane) < experts ? sigmoid(x[j]) : 0.f;
+      sum += s[j];
+    }
+    r.total = warp_sum_f(sum);
+  } else {
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) top = fmaxf(top, x[j]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    r.top = top == -INFINITY ? 0.f : top;         // nothing but -inf: every score is zero
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      s[j] = expert_of<V>(j, lane) < experts ? __expf(x[j] - r.top) : 0.f;
+      sum += s[j];
+    }
+    sum = warp_sum_f(sum);
+    r.inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) s[j] *= r.inv;
+    r.total = sum == 0.f ? 0.f : 1.f;
+  }
+  return r;
+}
+
+__device__ __forceinline__ float score_at(float x, const RowStat& r, bool use_sigmoid) {
+  return use_sigmoid ? sigmoid(x) : __expf(x - r.top) * r.inv;
+}
+
+// ---- the choice in 64 bits: lane i returns the i-th expert ---------------------------------------------
+__device__ __forceinline__ double key64(double v) { return v != v ? INFINITY : v; }
+
+template <typename T>
+__device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, double* c, int lane) {
+  const int E = a.experts;
+  double top = -INFINITY, sum = 0.;
+  if (!a.use_sigmoid) {
+    for (int e = lane; e < E; e += 32) top = fmax(top, double(to_float(row[e])));
+    for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (top == -INFINITY) top = 0.;
+  }
+  for (int e = lane; e < E; e += 32) {
+    const double x = to_float(row[e]);
+    c[e] = a.use_sigmoid ? 1. / (1. + exp(-x)) : exp(x - top);
+    sum += c[e];
+  }
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  for (int e = lane; e < E; e += 32) {
+    const double s = a.use_sigmoid ? c[e] : (sum == 0. ? 0. : c[e] / sum);
+    c[e] = key64(a.bias != nullptr ? s + double(a.bias[e]) : s);
+  }
+  __syncwarp();
+  unsigned kept = 0xffffffffu;
+  const int size = E / a.groups;
+  if (a.top_groups < a.groups) {
+    double value = -INFINITY;
+    if (lane < a.groups) {
+      double b1 = -INFINITY, b2 = -INFINITY;
+      for (int i = 0; i < size; ++i) {
+        const double v = c[lane * size + i];
+        if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) { b2 = v; }
+      }
+      value = size > 1 ? b1 + b2 : b1;
+    }
+    int rank = 0;
+    for (int h = 0; h < a.groups; ++h) {
+      const double o = __shfl_sync(0xffffffffu, value, h);
+      rank += o > value || (o == value && h < lane);
+    }
+    kept = __ballot_sync(0xffffffffu, lane < a.groups && rank < a.top_groups);
+    __syncwarp();
+  }
+  // Lane's experts are lane, lane + 32, ...: at most 32 of them, the taken ones a bit each.
+  unsigned gone = 0u;
+  int mine = 0;
+  for (int i = 0; i < a.top_k; ++i) {
+    double best = -INFINITY;
+    int at = 0x7fffffff;
+    for (int e = lane, n = 0; e < E; e += 32, ++n) {
+      if ((gone >> n & 1u) || !(kept >> (e / size) & 1u)) continue;
+      const double v = a.bias != nullptr ? c[e] : key64(double(to_float(row[e])));
+      if (at == 0x7fffffff || v > best) { best = v; at = e; }
+    }
+    for (int d = 16; d > 0; d >>= 1) {
+      const double ov = __shfl_xor_sync(0xffffffffu, best, d);
+      const int oe = __shfl_xor_sync(0xffffffffu, at, d);
+      if (oe != 0x7fffffff && (at == 0x7fffffff || ov > best || (ov == best && oe < at))) { best = ov; at = oe; }
+    }
+    if ((at & 31) == lane) gone |= 1u << (at >> 5);
+    if (lane == i) mine = at;
+  }
+  return mine;
+}
+
+__host__ __device__ constexpr int padded_slot(int e) { return e + (e >> 5) * 4; }
+
+// Groups that stay, as lane bits: bit (g * lanes per group).  `c` are the choice values (NaN as +inf).
+// Sets `doubt` when the last group that stays and the next are closer than the arithmetic tells apart.
+template <int PL, int V>
+__device__ __forceinline__ unsigned choose_groups(const float (&c)[PL], const SelectArgs& a, float* shared, int lane,
+                                                  float margin, bool& doubt) {
+  const int size = a.experts / a.groups;
+#pragma unroll
+  for (int j = 0; j < PL; ++j) {
+    const int e = expert_of<V>(j, lane);
+    if (e < a.experts) shared[padded_slot(e)] = c[j];
+  }
+  __syncwarp();
+  const int lanes = a.group_lanes, g = lane / lanes;
+  float b1 = -INFINITY, b2 = -INFINITY;
+  if (g < a.groups) {
+    for (int i = lane % lanes; i < size; i += lanes) {
+      const float v = shared[padded_slot(g * size + i)];
+      b2 = fmaxf(b2, fminf(b1, v));
+      b1 = fmaxf(b1, v);
+    }
+  }
+  for (int d = lanes / 2; d > 0; d >>= 1) {
+    const float o1 = __shfl_xor_sync(0xffffffffu, b1, d), o2 = __shfl_xor_sync(0xffffffffu, b2, d);
+    b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+    b1 = fmaxf(b1, o1);
+  }
+  const unsigned value = g < a.groups ? ordered(size > 1 ? b1 + b2 : b1) : 0u;
+  int rank = 0;
+  for (int h = 0; h < a.groups; ++h) {
+    const unsigned o = __shfl_sync(0xffffffffu, value, h * lanes);
+    rank += o > value || (o == value && h < g);
+  }
+  const bool stays = g < a.groups && rank < a.top_groups;
+  const float last = from_ordered(__reduce_min_sync(0xffffffffu, stays ? value : 0xffffffffu));
+  const float next = from_ordered(__reduce_max_sync(0xffffffffu, stays ? 0u : value));
+  doubt = !(last - next > 2.f * margin + 0x1p-21f * fmaxf(fabsf(last), fabsf(next)));
+  return __ballot_sync(0xffffffffu, stays);
+}
+
+template <typename T, int PL, int V>
+__global__ void __launch_bounds__(kWarps * 32)
+select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restrict__ scores, T* __restrict__ weights,
+                  int64_t* __restrict__ ids) {
+  extern __shared__ double shared[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = a.experts;
+  const int64_t t = int64_t(blockIdx.x) * kWarps + warp;
+  if (t >= a.tokens) return;
+  const T* row = logits + t * E;
+  float x[PL], s[PL];
+  load_slots<T, PL, V>(row, lane, E, -INFINITY, x);
+  const RowStat r = scores_of<PL, V>(x, lane, E, a.use_sigmoid, s);
+  const float inv_total = a.use_sigmoid && r.total != 0.f ? 1.f / r.total : 1.f;
+#pragma unroll
+  for (int j = 0; j < PL; j += V) {
+    const int e = expert_of<V>(j, lane);
+    if (e < E) {
+      Slots<T, V> p;
+#pragma unroll
+      for (int k = 0; k < V; ++k) p.v[k] = from_float<T>(s[j + k] * inv_total);
+      *reinterpret_cast<Slots<T, V>*>(scores + t * E + e) = p;
+    }
+  }
+
+  // Twice the error of a score: exponent's rounding and unit, division, sum (see the bound's terms: 1.6 x
+  // 2^-22 for the sigmoid, 1.6 x 2^-20 of the largest for the softmax); the sum with the bias adds its own
+  // rounding where two values are compared.
+  const float margin = a.use_sigmoid ? 0x1p-20f : 0x1p-18f * r.inv;
+  const bool biased = a.bias != nullptr;
+  bool doubt = false;
+  unsigned key[PL];
+  {
+    float c[PL];
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      const int e = expert_of<V>(j, lane);
+      c[j] = biased && e < E ? s[j] + __ldg(a.bias + e) : s[j];
+      key[j] = e < E ? ordered(biased ? c[j] : x[j]) : 0u;
+    }
+    if (a.top_groups < a.groups) {
+#pragma unroll
+      for (int j = 0; j < PL; ++j) c[j] = c[j] != c[j] ? INFINITY : c[j];
+      const unsigned stays = choose_groups<PL, V>(c, a, reinterpret_cast<float*>(shared + warp * a.shared_stride),
+                                                  lane, margin, doubt);
+      const float inv_size = float(a.groups) / float(E);
+#pragma unroll
+      for (int j = 0; j < PL; ++j) {
+        const int g = int((expert_of<V>(j, lane) + 0.5f) * inv_size);       // exact: at most 1024 experts
+        if (!(stays >> (g * a.group_lanes) & 1u)) key[j] = 0u;
+      }
+    }
+  }
+
+  int mine = 0, before = 0;
+  float before_c = 0.f;
+  // With a bias one expert more than is chosen: the last one has to be told from the next.
+  const int rounds = a.top_k + (biased ? 1 : 0);
+  for (int i = 0; i < rounds && !doubt; ++i) {
+    unsigned best = 0u;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < PL; ++j)
+      if (key[j] > best) { best = key[j]; at = expert_of<V>(j, lane); }
+    const unsigned top = __reduce_max_sync(0xffffffffu, best);
+    if (top == 0u) break;                         // all experts are chosen
+    const int e = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
+    if (biased) {
+      const float c = from_ordered(top);
+      if (i > 0 && !(before_c - c > margin + 0x1p-22f * fmaxf(fabsf(before_c), fabsf(c))))
+        doubt = !(ordered(to_float(row[before])) == ordered(to_float(row[e])) && a.bias[before] == a.bias[e]);
+      before_c = c;
+      before = e;
+    }
+    if (lane == i) mine = e;
+    if (at == e) {
+#pragma unroll
+      for (int j = 0; j < PL; ++j)
+        if (expert_of<V>(j, lane) == e) key[j] = 0u;
+    }
+  }
+  if (doubt) {
+    __syncwarp();
+    mine = choose_wide<T>(row, a, shared + warp * a.shared_stride, lane);
+  }
+
+  const bool live = lane < a.top_k;
+  const float w = live ? score_at(to_float(row[mine]), r, a.use_sigmoid) : 0.f;
+  float factor = a.scale;
+  if (a.norm_p != 0) {
+    const float acc = warp_sum_f(a.norm_p == 1 ? w : w * w);
+    // Chosen scores that are all zero have zero weights.
+    factor = acc == 0.f ? 0.f : a.scale / (a.norm_p == 1 ? acc : sqrtf(acc));
+  }
+  if (live) {
+    weights[t * a.top_k + lane] = from_float<T>(w * factor);
+    ids[t * a.top_k + lane] = mine;
+  }
+}
+
+// dlogits from the gradients of the weights and (optionally) of the scores.  The scores are taken again
+// from the logits, which costs the bytes that stored scores would and keeps their 32 bits.
+template <typename T, int PL, int V>
+__global__ void __launch_bounds__(kWarps * 32)
+select_bwd_kernel(const T* __restrict__ logits, const SelectArgs a, const int64_t* __restrict__ ids,
+                  const T* __restrict__ dscores, int64_t dscores_stride, const T* __restrict__ dweights,
+                  T* __restrict__ dlogits) {
+  const int lane = threadIdx.x & 31, E = a.experts;
+  const int64_t t = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (t >= a.tokens) return;
+  const T* row = logits + t * E;
+  const bool live = lane < a.top_k;
+  const int mine = live ? int(ids[t * a.top_k + lane]) : 0;
+  const float dw = live && dweights != nullptr ? to_float(dweights[t * a.top_k + lane]) * a.scale : 0.f;
+  const float mine_x = to_float(row[mine]);
+  float x[PL], s[PL];
+  RowStat r{0.f, 1.f, 0.f};
+  const bool whole = !a.use_sigmoid || dscores != nullptr;      // more than the chosen experts' own logits
+  if (whole) {
+    load_slots<T, PL, V>(row, lane, E, -INFINITY, x);
+    r = scores_of<PL, V>(x, lane, E, a.use_sigmoid, s);
+  }
+  const float w = live ? score_at(mine_x, r, a.use_sigmoid) : 0.f;
+  float dsel = dw;
+  if (a.norm_p != 0) {
+    const float acc = warp_sum_f(a.norm_p == 1 ? w : w * w);
+    const float dot = warp_sum_f(dw * w);
+    const float inv = acc == 0.f ? 0.f : 1.f / (a.norm_p == 1 ? acc : sqrtf(acc));
+    dsel = (dw - dot * inv * (a.norm_p == 1 ? 1.f : w * inv)) * inv;
+  }
+  if (!live) dsel = 0.f;
+  float g[PL];
+  float inner = 0.f, inv_total = 1.f;
+  if (dscores != nullptr) {
+    load_slots<T, PL, V>(dscores + t * dscores_stride, lane, E, 0.f, g);
+#pragma unroll
+    for (int j = 0; j < PL; ++j) inner += g[j] * s[j];
+    if (a.use_sigmoid && r.total != 0.f) inv_total = 1.f / r.total;
+  }
+  // softmax: inner = <ds, s> with both gradients; sigmoid: <g, scores> of the scores' gradient alone.
+  inner = a.use_sigmoid ? (dscores != nullptr ? warp_sum_f(inner) * inv_total : 0.f) : warp_sum_f(inner + dsel * w);
+  T* out = dlogits + t * E;
+#pragma unroll
+  for (int j = 0; j < PL; j += V) {
+    const int e = expert_of<V>(j, lane);
+    if (e < E) {
+      Slots<T, V> p;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float d = 0.f;
+        if (whole) {
+          const float gs = dscores != nullptr ? g[j + k] : 0.f;
+          d = a.use_sigmoid ? (gs - inner) * inv_total * s[j + k] * sigmoid(-x[j + k]) : s[j + k] * (gs - inner);
+        }
+        p.v[k] = from_float<T>(d);
+      }
+      *reinterpret_cast<Slots<T, V>*>(out + e) = p;
+    }
+  }
+  __syncwarp();               // the chosen experts' values over the ones just stored
+  if (live) {
+    const float gs = dscores != nullptr ? to_float(dscores[t * dscores_stride + mine]) : 0.f;
+    float d;
+    if (a.use_sigmoid) d = ((dscores != nullptr ? (gs - inner) * inv_total : 0.f) + dsel) * w * sigmoid(-mine_x);
+    else d = w * (gs + dsel - inner);
+    out[mine] = from_float<T>(d);
+  }
+}
+
+template <typename T, int V>
+bool row_vectors(int experts, const void* p) {
+  return experts % V == 0 && reinterpret_cast<uintptr_t>(p) % (V * sizeof(T)) == 0;
+}
+
+// PL slots a lane, fetched min(PL, 16 bytes) at a time where the rows allow it, else one by one.
+#define MB_SELECT_SWITCH(T, experts, aligned, CALL)                       \
+  if (experts <= 32) { CALL(1, 1); }                                      \
+  else if (experts <= 64) { if (aligned(2)) { CALL(2, 2); } else { CALL(2, 1); } } \
+  else if (experts <= 128) { if (aligned(4)) { CALL(4, 4); } else { CALL(4, 1); } } \
+  else if (experts <= 256) {                                              \
+    constexpr int W = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;            \
+    if (aligned(W)) { CALL(8, W); } else { CALL(8, 1); }                  \
+  } else if (experts <= 512) {                                            \
+    constexpr int W = 16 / sizeof(T);                                     \
+    if (aligned(W)) { CALL(16, W); } else { CALL(16, 1); }                \
+  } else {                                                                \
+    constexpr int W = 16 / sizeof(T);                                     \
+    if (aligned(W)) { CALL(32, W); } else { CALL(32, 1); }                \
+  }
+
+bool complete(SelectArgs& a) {
+  if (a.experts < 1 || a.experts > kRouterMaxExperts || a.top_k < 1 || a.top_k > kSelectMaxTopK) return false;
+  if (a.groups < 1 || a.groups > kSelectMaxGroups || a.experts % a.groups != 0 || a.top_groups < 1 ||
+      a.top_groups > a.groups || a.top_k > a.top_groups * (a.experts / a.groups) || a.norm_p < 0 || a.norm_p > 2)
+    return false;
+  a.group_lanes = 1;
+  while (a.group_lanes * 2 * a.groups <= 32) a.group_lanes *= 2;
+  a.shared_stride = a.bias != nullptr || a.top_groups < a.groups ? (a.experts > 16 ? a.experts : 16) : 0;
+  return true;
+}
+
+}  // namespace
+
+cudaError_t select_experts_fwd(DType type, const void* logits, SelectArgs a, void* scores, void* weights,
+                               int64_t* ids, cudaStream_t stream) {
+  if (!complete(a)) return cudaErrorInvalidValue;
+  if (a.tokens == 0) return cudaSuccess;
+  const size_t shared = size_t(a.shared_stride) * kWarps * sizeof(double);      // at most 32 KB
+  MB_SWITCH_FLOAT(type, T, {
+#define MB_SELECT_ALIGNED(v) (row_vectors<T, v>(a.experts, logits) && row_vectors<T, v>(a.experts, scores))
+#define MB_SELECT_FWD(PL, V)                                                                                     \
+  select_fwd_kernel<T, PL, V><<<ceil_div(a.tokens, kWarps), kWarps * 32, shared, stream>>>(                      \
+      static_cast<const T*>(logits), a, static_cast<T*>(scores), static_cast<T*>(weights), ids)
+    MB_SELECT_SWITCH(T, a.experts, MB_SELECT_ALIGNED, MB_SELECT_FWD)
+  })
+#undef MB_SELECT_FWD
+#undef MB_SELECT_ALIGNED
+  return cudaGetLastError();
+}
+
+cudaError_t select_experts_bwd(DType type, const void* logits, SelectArgs a, const int64_t* ids, const void* dscores,
+                               int64_t dscores_stride, const void* dweights, void* dlogits, cudaStream_t stream) {
+  if (!complete(a)) return cudaErrorInvalidValue;
+  if (a.tokens == 0) return cudaSuccess;
+  MB_SWITCH_FLOAT(type, T, {
+#define MB_SELECT_ALIGNED(v)                                                              \
+  (row_vectors<T, v>(a.experts, logits) && row_vectors<T, v>(a.experts, dlogits) &&        \
+   (dscores == nullptr || row_vectors<T, v>(a.experts, dscores)))
+#define MB_SELECT_BWD(PL, V)                                                                                     \
+  select_bwd_kernel<T, PL, V><<<ceil_div(a.tokens, kWarps), kWarps * 32, 0, stream>>>(                           \
+      static_cast<const T*>(logits), a, ids, static_cast<const T*>(dscores), dscores_stride,                     \
+      static_cast<const T*>(dweights), static_cast<T*>(dlogits))
+    MB_SELECT_SWITCH(T, a.experts, MB_SELECT_ALIGNED, MB_SELECT_BWD)
+  })
+#undef MB_SELECT_BWD
+#undef MB_SELECT_ALIGNED
+  return cudaGetLastError();
+}
+
+}  // namespace mb

@@ -595,6 +595,8 @@ at::Tensor& timing_words(const at::Device& device) {
 
 }  // namespace
 
+int* device_status(const at::Device& device) { return status_word(device).data_ptr<int>(); }
+
 at::Tensor gemm_role_timers(const at::Tensor& like) { return timing_words(like.device()); }
 
 // True when the tcgen05 kernel can run this problem; the Python caller falls back

@@ -28,6 +28,9 @@ at::Tensor scatter_wgrad_op(const at::Tensor& x, const at::Tensor& grad, const a
 at::Tensor binned_scatter_wgrad(const at::Tensor& x, const at::Tensor& grad, const at::Tensor& indices,
                                 const at::Tensor& bins, int64_t top_k);
 at::Tensor column_sum_op(const at::Tensor& x);
+// The device's status word, which kernels that give up a wait write, and the count of launched kernels.
+int* device_status(const at::Device& device);
+void count_launches(int64_t n);
 // `only_out2`: the activation epilogues (kEpiAct, kEpiGluDual) store nothing but the activation; c and out3
 // come back undefined.
 std::vector<at::Tensor> grouped_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& bins, bool trans_a,

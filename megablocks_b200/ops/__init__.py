@@ -6,6 +6,7 @@ from megablocks_b200.ops.metadata import (exclusive_cumsum, histogram, inclusive
 from megablocks_b200.ops.permute import (binned_gather, binned_scatter, gather, padded_gather, padded_scatter,
                                          scatter)
 from megablocks_b200.ops.route import route_plan
+from megablocks_b200.ops.select import select_experts, update_expert_bias
 from megablocks_b200.ops.sparse import Matrix, dds, dsd, sdd
 
 __all__ = [
@@ -29,6 +30,8 @@ __all__ = [
     'gmm_bins',
     'grouped_gemm',
     'route_plan',
+    'select_experts',
+    'update_expert_bias',
     'Matrix',
     'sdd',
     'dsd',

@@ -6,6 +6,8 @@
   costs three passes instead of the dozen of the eager float() / log_softmax /
   nll_loss chain.  The logits tensor must not be used after the loss (it is the
   gradient afterwards).
+* :func:`distillation_loss` / :func:`linear_distillation_loss` - distillation from a teacher's top logits
+  (optionally mixed with the targets' cross entropy), loss and gradient in one pass over the student's logits.
 * :func:`layer_norm` - LayerNorm whose backward reduces the weight and bias
   gradients through shared memory in the same pass that produces ``dx``.
 
@@ -22,6 +24,7 @@
 All fall back to the PyTorch ops on CPU tensors.
 """
 
+import math
 import os
 from typing import Any
 
@@ -88,6 +91,149 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float16, torch.float32) and logits.is_contiguous():
         return _CrossEntropy.apply(logits, targets.contiguous())
     return F.cross_entropy(logits.float(), targets)
+
+
+def _mean_rows(loss: torch.Tensor) -> torch.Tensor:
+    return loss.sum() / max(loss.shape[0], 1)
+
+
+class _Distillation(torch.autograd.Function):
+    """The forward pass takes the gradient of the loss while it has the row, into a tensor of its own; the
+    backward pass multiplies it by the incoming scalar where that is not one.  fp16 logits take it in the
+    backward pass instead: unscaled it underflows, and the loss scale is only known there."""
+
+    @staticmethod
+    def forward(ctx: Any, logits, values, ids, targets, temperature, hard_weight):
+        ctx.how = temperature, hard_weight, 1.0 / max(logits.shape[0], 1)
+        loss, stats, ctx.grad = ext().distill_forward(logits, values, ids, targets, *ctx.how,
+                                                      logits.dtype != torch.float16, False)
+        ctx.save_for_backward(logits, values, ids, targets, stats)
+        return _mean_rows(loss)
+
+    @staticmethod
+    def backward(ctx: Any, grad_out: torch.Tensor):
+        grad, ctx.grad = ctx.grad, None         # a second backward pass takes it again from the logits
+        scale = grad_out.detach().float().reshape(1)
+        if grad is not None:
+            ext().scale_unless_one_(grad, scale)
+        else:
+            logits, values, ids, targets, stats = ctx.saved_tensors
+            grad = ext().distill_backward(logits, values, ids, targets, stats, scale, *ctx.how)
+        return grad, None, None, None, None, None
+
+
+class _LinearDistillation(torch.autograd.Function):
+    """The language-model head and the loss: the gradient of the logits over the logits, as in
+    :class:`_LinearCrossEntropy`."""
+
+    @staticmethod
+    def forward(ctx: Any, hidden, weight, values, ids, targets, temperature, hard_weight):
+        logits = hidden @ weight.t()
+        loss, _, dlogits = ext().distill_forward(logits, values, ids, targets, temperature, hard_weight,
+                                                 1.0 / max(logits.shape[0], 1), True, True)
+        ctx.save_for_backward(hidden, weight, dlogits)
+        return _mean_rows(loss)
+
+    @staticmethod
+    def backward(ctx: Any, grad_out: torch.Tensor):
+        hidden, weight, dlogits = ctx.saved_tensors
+        scale = grad_out.detach().float()
+        dh = (dlogits @ weight).mul_(scale) if ctx.needs_input_grad[0] else None
+        dw = (dlogits.t() @ hidden).mul_(scale) if ctx.needs_input_grad[1] else None
+        return dh, dw, None, None, None, None, None
+
+
+MAX_TEACHER_TOP = 1024
+
+
+def _check_distillation(rows, device, teacher_logits, teacher_ids, temperature, targets, hard_weight):
+    if teacher_logits.dim() != 2 or teacher_logits.shape != teacher_ids.shape or teacher_logits.shape[0] != rows:
+        raise ValueError('distillation expects the teacher\'s logits and ids as [rows, top], one row per row of logits')
+    if not 1 <= teacher_logits.shape[1] <= MAX_TEACHER_TOP:
+        raise ValueError(f'distillation takes 1 to {MAX_TEACHER_TOP} teacher logits a row')
+    if teacher_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError('the teacher\'s ids must be int32 or int64')
+    if teacher_logits.dtype not in (torch.float16, torch.bfloat16, torch.float32, torch.float64):
+        raise ValueError('the teacher\'s logits must be floating-point')
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise ValueError(f'the temperature must be positive, got {temperature}')
+    if not (math.isfinite(hard_weight) and hard_weight >= 0):
+        raise ValueError(f'hard_weight must not be negative, got {hard_weight}')
+    if hard_weight and targets is None:
+        raise ValueError('hard_weight needs targets')
+    if targets is not None and (targets.shape != (rows,) or targets.dtype != torch.int64):
+        raise ValueError('targets must be int64 with one entry per row')
+    if any(t is not None and t.device != device for t in (teacher_logits, teacher_ids, targets)):
+        raise ValueError('the teacher\'s logits, its ids and the targets must be on the device of the logits')
+
+
+def _teacher(teacher_logits, teacher_ids, targets, hard_weight):
+    return (teacher_logits.detach().contiguous(), teacher_ids.contiguous(),
+            targets.contiguous() if targets is not None and hard_weight else None)
+
+
+def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                      temperature: float = 1.0, targets=None, hard_weight: float = 0.0) -> torch.Tensor:
+    """Mean over the rows of ``T^2 KL(p || q) + hard_weight * cross_entropy(logits, targets)``.
+
+    ``q = softmax(logits[rows, vocab] / T)`` and ``p`` is the softmax of a row's ``teacher_logits[rows, top] / T``
+    over the columns that ``teacher_ids[rows, top]`` (int32 or int64) names: the teacher's kept logits, taken as
+    its whole distribution.  Ids outside the vocabulary mark unused slots, a column named twice counts twice;
+    a row without a used slot has no such term, one whose target lies outside the vocabulary no cross
+    entropy, and a row with neither has a gradient of zero, whatever its logits.  Every row counts in the mean.
+    The teacher gets no gradient; the logits stay as they are."""
+    if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] < 1:
+        raise ValueError('distillation expects floating-point logits[rows, vocab]')
+    _check_distillation(logits.shape[0], logits.device, teacher_logits, teacher_ids, temperature, targets, hard_weight)
+    if (logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float16, torch.float32)
+            and teacher_logits.dtype != torch.float64):
+        logits = logits.contiguous()
+        args = (*_teacher(teacher_logits, teacher_ids, targets, hard_weight), float(temperature), float(hard_weight))
+        if torch.is_grad_enabled() and logits.requires_grad:
+            return _Distillation.apply(logits, *args)
+        return _mean_rows(ext().distill_forward(logits, *args, 1.0, False, False)[0])
+    return _composed_distillation(logits, teacher_logits, teacher_ids, temperature, targets, hard_weight)
+
+
+def _composed_distillation(logits, teacher_logits, teacher_ids, temperature, targets, hard_weight):
+    """The same from PyTorch ops."""
+    rows, vocab = logits.shape
+    z = logits if logits.dtype == torch.float64 else logits.float()
+    ids = teacher_ids.long()
+    used = (ids >= 0) & (ids < vocab)
+    values = (teacher_logits.detach().to(z.dtype) / temperature).masked_fill(~used, -math.inf)
+    used = used & (values != -math.inf)
+    live = used.any(dim=-1)
+    logp = values.masked_fill(~live.unsqueeze(1), 0.0).log_softmax(dim=-1).masked_fill(~used, 0.0)
+    p = logp.exp() * used
+    # Rows that teach nothing take no part at all, so that nothing of their logits reaches a gradient.
+    hard = torch.zeros_like(live)
+    if targets is not None and hard_weight:
+        hard = (targets >= 0) & (targets < vocab)
+    z = z.masked_fill(~(live | hard).unsqueeze(1), 0.0)
+    logq = (z / temperature).log_softmax(dim=-1).gather(1, ids.masked_fill(~used, 0))
+    loss = temperature**2 * torch.where(used & live.unsqueeze(1), p * (logp - logq), 0.0).sum()
+    if targets is not None and hard_weight:
+        ce = -z.log_softmax(dim=-1).gather(1, targets.masked_fill(~hard, 0).unsqueeze(1)).squeeze(1)
+        loss = loss + hard_weight * torch.where(hard, ce, 0.0).sum()
+    return loss / max(rows, 1)
+
+
+def linear_distillation_loss(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor,
+                             teacher_ids: torch.Tensor, temperature: float = 1.0, targets=None,
+                             hard_weight: float = 0.0) -> torch.Tensor:
+    """:func:`distillation_loss` of ``hidden[rows, h] @ weight[vocab, h]^T``: the language-model head and its loss.
+    On CUDA the logits are written once, and once overwritten with their gradient."""
+    if (hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float32) and hidden.dim() == 2
+            and weight.dtype == hidden.dtype and teacher_logits.dtype != torch.float64
+            and not torch.is_autocast_enabled() and os.environ.get('MB200_FUSED_LM_LOSS', '1') != '0'):
+        _check_distillation(hidden.shape[0], hidden.device, teacher_logits, teacher_ids, temperature, targets,
+                            hard_weight)
+        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+            args = _teacher(teacher_logits, teacher_ids, targets, hard_weight)
+            return _LinearDistillation.apply(hidden.contiguous(), weight, *args, float(temperature),
+                                             float(hard_weight))
+    return distillation_loss(F.linear(hidden, weight), teacher_logits, teacher_ids, temperature, targets, hard_weight)
 
 
 class _LayerNorm(torch.autograd.Function):

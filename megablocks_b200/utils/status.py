@@ -15,6 +15,7 @@ _MESSAGES = {
     2: 'grouped GEMM: MMA warp timed out waiting for a TMA tile',
     3: 'grouped GEMM: MMA warp timed out waiting for a free accumulator',
     4: 'grouped GEMM: epilogue timed out waiting for an accumulator',
+    9: 'distillation loss: a row of logits never arrived in shared memory',
     16: 'expert-parallel count exchange: a peer never published its counts',
     17: 'expert-parallel receive buffer overflow: more rows were routed to this rank than the buffer holds',
     18: 'grouped GEMM: rows of an expert never arrived from a peer (dispatch flag not released)',
