@@ -1,0 +1,198 @@
+// PyTorch-facing host code of the windowed attention: argument checks, output allocation, tensor maps.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "kernels.h"
+#include "torch_ops.h"
+
+namespace mb {
+
+namespace {
+
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+int sm_count() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
+
+// [batch, seq, heads, dim] 16-bit tensor that the kernels read in place: rows of whole 16 bytes on 16-byte
+// boundaries, and no dimension that is broadcast.
+bool in_place(const at::Tensor& t) {
+  if (!t.is_cuda() || t.dim() != 4 || !(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf)) return false;
+  const int64_t dim = t.size(3);
+  if (dim < 8 || dim > 128 || dim % 8 != 0 || t.stride(3) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0)
+    return false;
+  for (int d = 0; d < 3; ++d)
+    if (t.size(d) > 1 && (t.stride(d) <= 0 || t.stride(d) % 8 != 0 || t.stride(d) >= (int64_t(1) << 38))) return false;
+  return true;
+}
+
+// (dim, seq, heads, batch) map with boxes of 64 x rows, 128-byte swizzle.
+CUtensorMap make_map(const at::Tensor& t, int box_rows) {
+  const int order[3] = {1, 2, 0};
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(t.size(3)), 1, 1, 1};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(t.size(order[i]));
+    // The stride of a dimension of one is never used, but has to be valid.
+    strides[i] = static_cast<cuuint64_t>(t.size(order[i]) > 1 ? t.stride(order[i]) * 2 : 256);
+  }
+  const cuuint32_t box[4] = {64u, static_cast<cuuint32_t>(box_rows), 1u, 1u};
+  CUtensorMap map;
+  const CUresult rc = encode_tensor_map(&map, t.scalar_type() == at::kBFloat16, 4, t.data_ptr(), dims, strides, box);
+  TORCH_CHECK(rc == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", int(rc));
+  return map;
+}
+
+attn::Params make_params(const at::Tensor& q, const at::Tensor& k, int64_t window, int64_t sinks,
+                         const OptTensor& lengths, double scale) {
+  TORCH_CHECK(in_place(q) && in_place(k), "window_attention expects 16-bit CUDA tensors [batch, seq, heads, dim] with "
+              "aligned rows");
+  TORCH_CHECK(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3) && k.size(2) >= 1 &&
+                  q.size(2) % k.size(2) == 0 && q.size(1) >= 1 && q.size(1) < (int64_t(1) << 22) &&
+                  q.size(0) * q.size(2) < (int64_t(1) << 16) && q.size(0) >= 1 && q.size(2) >= 1,
+              "window_attention: sizes do not match or are too large");
+  TORCH_CHECK(window >= 1 && sinks >= 0 && scale > 0, "window_attention: bad window, sinks or scale");
+  if (lengths.has_value())
+    TORCH_CHECK(lengths->device() == q.device() && lengths->is_contiguous() && lengths->scalar_type() == at::kInt &&
+                    lengths->dim() == 1 && lengths->size(0) == q.size(0),
+                "window_attention: lengths must be int32 [batch]");
+  attn::Params p{};
+  p.batch = int(q.size(0));
+  p.seq = int(q.size(1));
+  p.heads = int(q.size(2));
+  p.kv_heads = int(k.size(2));
+  p.dim = int(q.size(3));
+  p.window = int(std::min<int64_t>(window, p.seq));
+  p.sinks = int(std::min<int64_t>(sinks, p.seq));
+  p.lengths = lengths.has_value() ? lengths->data_ptr<int>() : nullptr;
+  p.scale = float(scale);
+  p.seq_pad = (p.seq + attn::kPadRows - 1) / attn::kPadRows * attn::kPadRows;
+  p.status = device_status(q.device());
+  return p;
+}
+
+void check_like(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  TORCH_CHECK(in_place(t) && t.device() == like.device() && t.scalar_type() == like.scalar_type() &&
+                  t.sizes() == like.sizes(), "window_attention: ", name, " does not match");
+}
+
+}  // namespace
+
+bool window_attention_in_place(const at::Tensor& t) { return in_place(t); }
+
+// {out, log-sum-exp [batch, heads, padded seq] (undefined unless wanted)}
+std::vector<at::Tensor> window_attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                 int64_t window, int64_t sinks, const OptTensor& lengths, double scale,
+                                                 bool want_lse) {
+  c10::cuda::CUDAGuard guard(q.device());
+  attn::Params p = make_params(q, k, window, sinks, lengths, scale);
+  TORCH_CHECK(k.device() == q.device() && k.scalar_type() == q.scalar_type(), "window_attention: k does not match q");
+  check_like(v, k, "v");
+  at::Tensor out = at::empty({p.batch, p.seq, p.heads, p.dim}, q.options()), lse;
+  if (want_lse) {
+    lse = at::empty({p.batch, p.heads, p.seq_pad}, q.options().dtype(at::kFloat));
+    p.lse = lse.data_ptr<float>();
+  }
+  C10_CUDA_CHECK(attn::forward(q.scalar_type() == at::kBFloat16, make_map(q, attn::kTile), make_map(k, attn::kTile),
+                               make_map(v, attn::kTile), make_map(out, attn::kTile), p, stream()));
+  count_launches(1);
+  return {out, lse};
+}
+
+std::vector<at::Tensor> window_attention_backward(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+                                                  const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse,
+                                                  int64_t window, int64_t sinks, const OptTensor& lengths, double scale,
+                                                  bool want_q, bool want_kv) {
+  c10::cuda::CUDAGuard guard(q.device());
+  attn::Params p = make_params(q, k, window, sinks, lengths, scale);
+  TORCH_CHECK(k.device() == q.device() && k.scalar_type() == q.scalar_type(), "window_attention: k does not match q");
+  check_like(v, k, "v");
+  check_like(dout, q, "the gradient");
+  check_like(out, q, "the output");
+  TORCH_CHECK(out.is_contiguous() && dout.is_contiguous(), "window_attention: output and gradient must be contiguous");
+  TORCH_CHECK(lse.device() == q.device() && lse.is_contiguous() && lse.scalar_type() == at::kFloat &&
+                  lse.numel() == int64_t(p.batch) * p.heads * p.seq_pad, "window_attention: bad log-sum-exp");
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  at::Tensor dq, dk, dv, far;
+  at::Tensor delta = at::empty_like(lse);
+  p.lse = lse.data_ptr<float>();
+  p.delta = delta.data_ptr<float>();
+  C10_CUDA_CHECK(attn::row_sums(bf16, out.data_ptr(), dout.data_ptr(), p, stream()));
+  count_launches(1);
+  if (want_kv) {
+    dk = at::empty({p.batch, p.seq, p.kv_heads, p.dim}, q.options());
+    dv = at::empty({p.batch, p.seq, p.kv_heads, p.dim}, q.options());
+    if (p.sinks > 0) {
+      // Every query sees the first tokens: their tile's stream is as long as the sequence, the others' a
+      // window.  What exceeds that is split into parts of a window's length.
+      const int half = attn::kHalfTile;
+      const int usual = (p.window + attn::kTile + half - 1) / half;
+      const int far_tiles = std::max(0, (p.seq + half - 1) / half - usual);
+      if (far_tiles > usual / 2) {
+        p.far_tiles = std::max({usual, 16, (far_tiles + 63) / 64});
+        p.far_splits = (far_tiles + p.far_tiles - 1) / p.far_tiles;
+        far = at::empty({p.far_splits + 1, p.batch, p.kv_heads, 2, p.sinks, p.dim}, lse.options());
+        p.far = far.data_ptr<float>();
+      }
+    }
+    C10_CUDA_CHECK(attn::backward_keys(bf16, make_map(k, attn::kTile), make_map(v, attn::kTile),
+                                       make_map(q, attn::kHalfTile), make_map(dout, attn::kHalfTile),
+                                       make_map(dk, attn::kTile), make_map(dv, attn::kTile), p, stream()));
+    count_launches(1);
+    if (p.far_splits > 0) {
+      C10_CUDA_CHECK(attn::sum_far(bf16, dk.data_ptr(), dv.data_ptr(), p, stream()));
+      count_launches(1);
+    }
+  }
+  if (want_q) {
+    dq = at::empty({p.batch, p.seq, p.heads, p.dim}, q.options());
+    C10_CUDA_CHECK(attn::backward_queries(bf16, make_map(q, attn::kTile), make_map(dout, attn::kTile),
+                                          make_map(k, attn::kHalfTile), make_map(v, attn::kHalfTile),
+                                          make_map(dq, attn::kTile), p, stream()));
+    count_launches(1);
+  }
+  return {dq, dk, dv};
+}
+
+at::Tensor window_attention_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                   const at::Tensor& lengths, int64_t window, int64_t sinks, double scale) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.is_contiguous() && reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 == 0 &&
+                  in_place(k) && in_place(v) && q.device() == k.device() && k.device() == v.device() &&
+                  q.scalar_type() == k.scalar_type() && k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() &&
+                  q.size(0) == k.size(0) && q.size(2) == k.size(3) && q.size(1) % k.size(2) == 0 &&
+                  k.size(1) < (int64_t(1) << 30) && q.size(0) < (int64_t(1) << 16) && q.size(1) < (int64_t(1) << 16),
+              "window_attention_decode expects 16-bit CUDA q[batch, heads, dim] and caches [batch, capacity, kv_heads, "
+              "dim] with aligned rows");
+  TORCH_CHECK(lengths.device() == q.device() && lengths.is_contiguous() && lengths.scalar_type() == at::kInt &&
+                  lengths.dim() == 1 && lengths.size(0) == q.size(0),
+              "window_attention_decode: lengths must be int32 [batch]");
+  TORCH_CHECK(window >= 1 && sinks >= 0 && scale > 0, "window_attention_decode: bad window, sinks or scale");
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty_like(q);
+  if (q.size(0) == 0) return out;
+  attn::DecodeParams p{};
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.out = out.data_ptr();
+  p.k_batch = k.stride(0), p.k_row = k.stride(1), p.k_head = k.stride(2);
+  p.v_batch = v.stride(0), p.v_row = v.stride(1), p.v_head = v.stride(2);
+  p.lengths = lengths.data_ptr<int>();
+  p.batch = int(q.size(0));
+  p.capacity = int(k.size(1));
+  p.heads = int(q.size(1));
+  p.kv_heads = int(k.size(2));
+  p.dim = int(q.size(2));
+  p.window = int(std::min<int64_t>(window, p.capacity));
+  p.sinks = int(std::min<int64_t>(sinks, p.capacity));
+  p.scale = float(scale);
+  C10_CUDA_CHECK(attn::decode(q.scalar_type() == at::kBFloat16, p, sm_count(), stream()));
+  count_launches(1);
+  return out;
+}
+
+}  // namespace mb

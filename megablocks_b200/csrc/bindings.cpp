@@ -46,6 +46,19 @@ at::Tensor distill_backward(const at::Tensor& logits, const at::Tensor& values, 
                             const at::Tensor& grad_out, double temperature, double hard_weight, double scale);
 void scale_unless_one_op(at::Tensor x, const at::Tensor& factor);
 
+// attention_glue.cpp
+bool window_attention_in_place(const at::Tensor& t);
+std::vector<at::Tensor> window_attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                 int64_t window, int64_t sinks,
+                                                 const c10::optional<at::Tensor>& lengths, double scale, bool want_lse);
+std::vector<at::Tensor> window_attention_backward(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+                                                  const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse,
+                                                  int64_t window, int64_t sinks,
+                                                  const c10::optional<at::Tensor>& lengths, double scale, bool want_q,
+                                                  bool want_kv);
+at::Tensor window_attention_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                   const at::Tensor& lengths, int64_t window, int64_t sinks, double scale);
+
 // torch_glue.cpp: grouped GEMM
 bool grouped_gemm_supported(const at::Tensor& a, const at::Tensor& b, bool trans_a, bool trans_b,
                             int64_t num_groups);
@@ -160,6 +173,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_forward", &mb::distill_forward, "Per-row loss, row statistics and, if wanted, the gradient");
   m.def("distill_backward", &mb::distill_backward);
   m.def("scale_unless_one_", &mb::scale_unless_one_op);
+  m.def("window_attention_in_place", &mb::window_attention_in_place);
+  m.def("window_attention_forward", &mb::window_attention_forward);
+  m.def("window_attention_backward", &mb::window_attention_backward);
+  m.def("window_attention_decode", &mb::window_attention_decode);
   m.def("grouped_gemm_supported", &mb::grouped_gemm_supported);
   m.def("grouped_gemm", &mb::grouped_gemm);
   m.def("combine_rows", &mb::combine_rows_op);

@@ -117,6 +117,63 @@ cudaError_t distill_bwd(DType type, const DistillArgs& args, const float* stats,
 // x *= *factor; returns without touching x where the factor is one.
 cudaError_t scale_unless_one(DType type, void* x, int64_t numel, const float* factor, int sms, cudaStream_t stream);
 
+// ---- window_attention*.cu ----------------------------------------------------------
+// Causal attention inside a sliding window with first tokens that stay visible: query i sees key j when
+// j <= i and (i - j < window or j < sinks).  16-bit tensors of `dim` <= 128, a multiple of 8.  The tensor
+// maps describe [batch, seq, heads, dim] as (dim, seq, heads, batch) with boxes of 64 x rows and 128-byte
+// swizzle.
+namespace attn {
+
+constexpr int kTile = 128;             // rows of a resident tile, keys of a streamed one in the forward pass
+constexpr int kHalfTile = 64;          // rows of a streamed tile in the backward pass
+constexpr int kPadRows = 256;          // per-row statistics are padded to a multiple of this
+constexpr int kErrLoad = 48, kErrMma = 49, kErrRows = 50;
+
+struct Params {
+  int batch, seq, heads, kv_heads, dim;
+  int window, sinks;                   // 1 <= window <= seq, 0 <= sinks <= seq
+  const int* lengths;                  // [batch] valid tokens, nullable (all of them)
+  float scale;                         // of the scores
+  float* lse;                          // [batch, heads, seq_pad] base-2 log-sum-exp of the scaled scores
+  float* delta;                        // [batch, heads, seq_pad] sum over dim of dout * out
+  int seq_pad;
+  // Backward pass over the keys: queries a window away from the first tokens are split into `far_splits`
+  // parts of `far_tiles` tiles, whose shares of the first tokens' gradients are summed afterwards.
+  int far_splits, far_tiles;
+  float* far;                          // [far_splits + 1][batch, kv_heads][2][sinks][dim]
+  int* status;
+};
+
+cudaError_t forward(bool bf16, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                    const CUtensorMap& out, const Params& params, cudaStream_t stream);
+// delta, and zeros behind the sequences' ends.
+cudaError_t row_sums(bool bf16, const void* out, const void* dout, const Params& params, cudaStream_t stream);
+// Maps with 128-row boxes (`q`, `k`, ...: resident tiles and results) and 64-row boxes (`q_half`, ...: streamed).
+cudaError_t backward_keys(bool bf16, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q_half,
+                          const CUtensorMap& dout_half, const CUtensorMap& dk, const CUtensorMap& dv,
+                          const Params& params, cudaStream_t stream);
+cudaError_t backward_queries(bool bf16, const CUtensorMap& q, const CUtensorMap& dout, const CUtensorMap& k_half,
+                             const CUtensorMap& v_half, const CUtensorMap& dq, const Params& params,
+                             cudaStream_t stream);
+// The first tokens' gradients from the parts of `far`.
+cudaError_t sum_far(bool bf16, void* dk, void* dv, const Params& params, cudaStream_t stream);
+
+// One new token per sequence over a cache [batch, capacity, kv_heads, dim] with the given strides (elements,
+// multiples of 8) and unit stride in dim; the token is the last of the `lengths[b]` valid ones.
+struct DecodeParams {
+  const void* q;                       // [batch, heads, dim]
+  const void* k;
+  const void* v;
+  void* out;                           // [batch, heads, dim]
+  int64_t k_batch, k_row, k_head, v_batch, v_row, v_head;
+  const int* lengths;
+  int batch, capacity, heads, kv_heads, dim, window, sinks;
+  float scale;
+};
+cudaError_t decode(bool bf16, const DecodeParams& params, int sms, cudaStream_t stream);
+
+}  // namespace attn
+
 // ---- optim.cu -----------------------------------------------------------------
 struct AdamTensor {
   void* param;        // 16-bit (or fp32) shadow weights the model computes with

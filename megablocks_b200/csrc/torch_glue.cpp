@@ -528,24 +528,31 @@ EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
-// Two-dimensional map of a row-major [rows, cols] 16-bit tensor.  The driver call needs a current context,
-// which a thread whose first CUDA call this is does not have yet (autograd's worker, when the gradient's
-// storage came from the allocator's cache): the runtime makes it current, and the call is made again.
-CUresult encode_2d(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, cuuint32_t box_rows,
-                   cuuint32_t box_cols, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
-  const cuuint32_t box[2] = {box_cols, box_rows};
-  const cuuint32_t elem_strides[2] = {1u, 1u};
+// The driver call needs a current context, which a thread whose first CUDA call this is does not have yet
+// (autograd's worker, when the gradient's storage came from the allocator's cache): the runtime makes it
+// current, and the call is made again.
+CUresult encode_map(CUtensorMap* map, bool bf16, int rank, const void* base, const cuuint64_t* dims,
+                    const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle,
+                    CUtensorMapL2promotion promotion) {
+  const cuuint32_t elem_strides[4] = {1u, 1u, 1u, 1u};
   auto encode = [&] {
-    return encode_tiled_fn()(
-        map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
-        strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return encode_tiled_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                             cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, elem_strides,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   const CUresult rc = encode();
   if (rc != CUDA_ERROR_INVALID_CONTEXT && rc != CUDA_ERROR_NOT_INITIALIZED) return rc;
   C10_CUDA_CHECK(cudaSetDevice(at::cuda::current_device()));
   return encode();
+}
+
+// Two-dimensional map of a row-major [rows, cols] 16-bit tensor.
+CUresult encode_2d(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, cuuint32_t box_rows,
+                   cuuint32_t box_cols, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  return encode_map(map, bf16, 2, base, dims, strides, box, swizzle, promotion);
 }
 
 // Row-major [rows, cols] 16-bit tensor, box = box_rows x 64 columns, 128-byte swizzle.
@@ -594,6 +601,13 @@ at::Tensor& timing_words(const at::Device& device) {
 }
 
 }  // namespace
+
+CUresult encode_tensor_map(CUtensorMap* map, bool bf16, int rank, const void* base, const cuuint64_t* dims,
+                           const cuuint64_t* strides, const cuuint32_t* box) {
+  TORCH_CHECK(rank >= 2 && rank <= 4, "tensor maps have 2 to 4 dimensions");
+  return encode_map(map, bf16, rank, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
 
 int* device_status(const at::Device& device) { return status_word(device).data_ptr<int>(); }
 

@@ -2,6 +2,7 @@
 // the module (bindings.cpp) also exposes one by one.
 #pragma once
 
+#include <cuda.h>
 #include <torch/extension.h>
 
 #include <vector>
@@ -31,6 +32,9 @@ at::Tensor column_sum_op(const at::Tensor& x);
 // The device's status word, which kernels that give up a wait write, and the count of launched kernels.
 int* device_status(const at::Device& device);
 void count_launches(int64_t n);
+// Tensor map of a 16-bit tensor (innermost dimension dense, `strides` in bytes of the others), 128-byte swizzle.
+CUresult encode_tensor_map(CUtensorMap* map, bool bf16, int rank, const void* base, const cuuint64_t* dims,
+                           const cuuint64_t* strides, const cuuint32_t* box);
 // `only_out2`: the activation epilogues (kEpiAct, kEpiGluDual) store nothing but the activation; c and out3
 // come back undefined.
 std::vector<at::Tensor> grouped_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& bins, bool trans_a,

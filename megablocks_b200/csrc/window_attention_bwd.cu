@@ -1,0 +1,460 @@
+// Windowed causal attention, backward, on the 5th-generation tensor cores.
+//
+//   P_ij  = exp(scale q_i k_j - lse_i)             dS_ij = P_ij (dO_i v_j - delta_i),  delta_i = dO_i O_i
+//   dV_j  = sum_i P_ij dO_i     dK_j = scale sum_i dS_ij q_i     dQ_i = scale sum_j dS_ij k_j
+//
+// Two kernels of one shape.  A CTA holds two resident tiles of 128 rows and streams pairs of 64-row tiles
+// past them: the keys' kernel holds K and V and streams Q and dO of every query head that shares them (so
+// the heads' gradients are summed where they are made, in a fixed order), the queries' kernel holds Q and dO
+// and streams K and V.  Each pair gives two products in tensor memory (scores and dO V^T, with the resident
+// rows on the lanes), which a group of 128 threads turns into P and dS in place; those are A operands of
+// the sums, which stay in tensor memory.  Nothing is transposed and nothing is added atomically: the scores
+// are computed once for either kernel, 7 products of a tile where one pass with atomic sums for dQ would
+// take 5, and gradients come out the same in every run.  Two groups of row threads take alternate pairs.
+#include "window_attention.cuh"
+
+namespace mb {
+namespace attn {
+
+namespace {
+
+constexpr int kThreads = 384;          // warp 0 loads, warp 1 issues MMAs, warps 4-7 and 8-11 own the rows
+
+template <int D>
+struct Layout {
+  static constexpr int kResidentBytes = kTile * D * 2;
+  static constexpr int kStreamBytes = kHalfTile * D * 2;
+  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kStatBytes = 2 * kHalfTile * 4;             // lse and delta of a streamed tile's rows
+  static constexpr int kBytes = 2 * kResidentBytes + kStages * (2 * kStreamBytes + kStatBytes) + 1024 + 256;
+};
+
+// The streamed tiles of a CTA.  Keys' kernel: query tiles [lo, lo + per_head) of each of `heads` heads;
+// queries' kernel: key tiles, the first tokens' before the window's.
+struct Stream {
+  int count, per_head, lo, head_tiles;
+  __device__ __forceinline__ int tile(int t, bool keys) const {
+    if (keys) return lo + t % per_head;
+    return t < head_tiles ? t : lo + t - head_tiles;
+  }
+};
+
+template <typename T, int D, bool KEYS>
+__global__ void __launch_bounds__(kThreads, 1)
+window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_constant__ CUtensorMap map_x1,
+                  const __grid_constant__ CUtensorMap map_y0, const __grid_constant__ CUtensorMap map_y1,
+                  const __grid_constant__ CUtensorMap map_out0, const __grid_constant__ CUtensorMap map_out1,
+                  const __grid_constant__ Params p) {
+  using L = Layout<D>;
+  constexpr int kStages = L::kStages, kStream = L::kStreamBytes, kResident = L::kResidentBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* tile_x = smem;                                          // x0, x1
+  uint8_t* ring = smem + 2 * kResident;                            // [stage]: y0, y1
+  float* stats = reinterpret_cast<float*>(ring + kStages * 2 * kStream);       // [stage]: lse, delta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + kStages * 2 * kHalfTile);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + kStages;
+  uint64_t* x_full = bars + 2 * kStages;
+  uint64_t* s_full = x_full + 1;                   // [2] both products of a group's pair are in tensor memory
+  uint64_t* d_full = s_full + 2;                   // [2] P and dS are
+  uint64_t* acc_full = d_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Keys' kernel: heads fastest, so that the tiles of the first tokens, which have the longest streams, start
+  // first.  `part` > 0: queries far from the first tokens.
+  const int ratio = p.heads / p.kv_heads;
+  const int heads_here = KEYS ? p.kv_heads : p.heads;
+  const int own_head = blockIdx.x % heads_here, b = blockIdx.x / heads_here;
+  const int far_blocks = KEYS ? p.far_splits * ((p.sinks + kTile - 1) / kTile) : 0;
+  const int part = KEYS && int(blockIdx.y) < far_blocks ? 1 + int(blockIdx.y) % p.far_splits : 0;
+  const int x_tile = part > 0 ? int(blockIdx.y) / p.far_splits : int(blockIdx.y) - far_blocks;
+  const int x_row = x_tile * kTile;
+  const int len = length_of(p, b);
+
+  Stream st{0, 1, 0, 0};
+  if (x_row < len) {
+    const int tiles = (len + kHalfTile - 1) / kHalfTile;
+    if constexpr (KEYS) {
+      // Queries from the tile's own on; up to a window behind its last key, or all for first tokens.
+      const int near = int(min(int64_t(tiles), (int64_t(x_row) + kTile + p.window - 2) / kHalfTile + 1));
+      st.lo = x_row / kHalfTile;
+      int hi = near;
+      if (x_row < p.sinks) {
+        if (p.far_splits == 0) hi = tiles;
+        if (part > 0) {
+          st.lo = near + (part - 1) * p.far_tiles;
+          hi = min(tiles, st.lo + p.far_tiles);
+        }
+      }
+      st.per_head = max(0, hi - st.lo);
+      st.count = st.per_head * ratio;
+    } else {
+      st.lo = max(0, x_row - p.window + 1) / kHalfTile;
+      st.head_tiles = min((p.sinks + kHalfTile - 1) / kHalfTile, st.lo);
+      st.count = st.head_tiles + (min(x_row + kTile, len) - 1) / kHalfTile - st.lo + 1;
+    }
+  }
+  auto stream_head = [&](int t) { return KEYS ? own_head * ratio + t / st.per_head : own_head / ratio; };
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(x_full), 1);
+    mbar_init(smem_u32(acc_full), 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(smem_u32(&s_full[g]), 1);
+      mbar_init(smem_u32(&d_full[g]), 4);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // Group g: scores at g * 128, the other product at g * 128 + 64.  Sums: at 256 (dV, or dQ) and 256 + D (dK).
+  const uint32_t tmem_acc = tmem + 256;
+
+  if (warp == 0) {
+    // ---- loader ----------------------------------------------------------------------------------
+    if (lane == 0 && st.count > 0) {
+      const uint32_t x_bar = smem_u32(x_full);
+      mbar_arrive_expect_tx(x_bar, 2 * kResident);
+      for (int box = 0; box < D / 64; ++box) {
+        tma_load_4d(smem_u32(tile_x + box * (kTile * 128)), &map_x0, x_bar, box * 64, x_row, own_head, b);
+        tma_load_4d(smem_u32(tile_x + kResident + box * (kTile * 128)), &map_x1, x_bar, box * 64, x_row, own_head, b);
+      }
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int t = 0; t < st.count; ++t) {
+        if (!mbar_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.status, kErrLoad, kWaitNs)) break;
+        const uint32_t bar = smem_u32(&full[stage]);
+        const int row = st.tile(t, KEYS) * kHalfTile, h = stream_head(t);
+        uint8_t* y = ring + stage * 2 * kStream;
+        mbar_arrive_expect_tx(bar, 2 * kStream + (KEYS ? L::kStatBytes : 0));
+        for (int box = 0; box < D / 64; ++box) {
+          tma_load_4d(smem_u32(y + box * (kHalfTile * 128)), &map_y0, bar, box * 64, row, h, b);
+          tma_load_4d(smem_u32(y + kStream + box * (kHalfTile * 128)), &map_y1, bar, box * 64, row, h, b);
+        }
+        if constexpr (KEYS) {
+          const int64_t at = (int64_t(b) * p.heads + h) * p.seq_pad + row;
+          float* s = stats + stage * 2 * kHalfTile;
+          bulk_load(smem_u32(s), p.lse + at, kHalfTile * 4, bar);
+          bulk_load(smem_u32(s + kHalfTile), p.delta + at, kHalfTile * 4, bar);
+        }
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---- MMA issuer ------------------------------------------------------------------------------
+    constexpr uint32_t idesc_s = instr_desc_f16(kIsBf16<T>, false, false, kTile, kHalfTile);
+    constexpr uint32_t idesc_a = instr_desc_f16(kIsBf16<T>, false, true, kTile, D);
+    const uint32_t x0 = smem_u32(tile_x), x1 = smem_u32(tile_x + kResident);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && mbar_wait(smem_u32(bar), parity, abort_flag, p.status, kErrMma, kWaitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      tcgen05_fence_after();
+    };
+    int stage = 0, old = 0;            // stage of pair t and of pair t - 1
+    uint32_t phase = 0;
+    if (st.count > 0) wait(x_full, 0);
+    for (int t = 0; t <= st.count && ok; ++t) {
+      if (t < st.count) {
+        const int g = t & 1;
+        wait(&full[stage], phase);
+        if (!ok) break;
+        uint8_t* y = ring + stage * 2 * kStream;
+        const int left = len - st.tile(t, KEYS) * kHalfTile;
+        if (left < kHalfTile) {
+          zero_rows<kHalfTile, D>(y, left, lane);
+          zero_rows<kHalfTile, D>(y + kStream, left, lane);
+        }
+        if (lane == 0) {
+          const uint32_t y0 = smem_u32(y), y1 = smem_u32(y + kStream);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            umma_f16(tmem + g * 128, desc_along_dim<kTile>(x0, i), desc_along_dim<kHalfTile>(y0, i), idesc_s, i != 0);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            umma_f16(tmem + g * 128 + 64, desc_along_dim<kTile>(x1, i), desc_along_dim<kHalfTile>(y1, i), idesc_s,
+                     i != 0);
+          umma_commit(smem_u32(&s_full[g]));
+        }
+        __syncwarp();
+      }
+      if (t > 0) {
+        const int g = (t - 1) & 1;
+        wait(&d_full[g], ((t - 1) >> 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t y0 = smem_u32(ring + old * 2 * kStream), y1 = y0 + kStream;
+          if constexpr (KEYS) {
+#pragma unroll
+            for (int i = 0; i < kHalfTile / 16; ++i)
+              umma_f16_ta(tmem_acc, tmem + g * 128 + i * 8, desc_along_rows<kHalfTile>(y1, i), idesc_a, t > 1 || i != 0);
+          }
+#pragma unroll
+          for (int i = 0; i < kHalfTile / 16; ++i)
+            umma_f16_ta(tmem_acc + (KEYS ? D : 0), tmem + g * 128 + 64 + i * 8, desc_along_rows<kHalfTile>(y0, i),
+                        idesc_a, t > 1 || i != 0);
+          umma_commit(smem_u32(&empty[old]));
+          if (t == st.count) umma_commit(smem_u32(acc_full));
+        }
+        __syncwarp();
+      }
+      old = stage;
+      if (t < st.count && ++stage == kStages) { stage = 0; phase ^= 1u; }
+    }
+  } else if (warp >= 4) {
+    // ---- rows ------------------------------------------------------------------------------------
+    const int g = (warp - 4) >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane, mine = x_row + r;          // this thread's key (or query)
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const uint32_t ts = tmem + g * 128 + lanes, td = ts + 64;
+    const float scale = p.scale * kLog2e;
+    float row_lse = 0.f, row_delta = 0.f;
+    if constexpr (!KEYS) {
+      if (mine < p.seq_pad) {
+        const int64_t at = (int64_t(b) * p.heads + own_head) * p.seq_pad + mine;
+        row_lse = p.lse[at];
+        row_delta = p.delta[at];
+      }
+    }
+    bool ok = true;
+    int stage = g;
+    for (int t = g; t < st.count && ok; t += 2) {
+      while (stage >= kStages) stage -= kStages;
+      ok = mbar_wait(smem_u32(&s_full[g]), (t >> 1) & 1, abort_flag, p.status, kErrRows, kWaitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const int y_row = st.tile(t, KEYS) * kHalfTile;
+      // Columns whose pair is visible.  Keys' kernel: queries i = y_row + column see this key when
+      // key <= i < key + window, or from the key on for a first token; rows behind the end have an infinite
+      // lse.  Queries' kernel: keys of the window, and first tokens.
+      int from, to, keep;              // [from, to), and in the queries' kernel also [0, keep) where it is below `to`
+      bool edge;
+      if constexpr (KEYS) {
+        from = mine - y_row;
+        to = mine < p.sinks ? kHalfTile : int(min(int64_t(kHalfTile), int64_t(mine) + p.window - y_row));
+        // Far queries belong to the first tokens only, and are another CTA's where they are split.
+        keep = 0;
+        edge = x_row + kTile - 1 > y_row || (y_row + kHalfTile - 1) - x_row >= p.window ||
+               y_row + kHalfTile > len || x_row + kTile > len;
+        to = min(to, len - y_row);
+      } else {
+        from = mine - p.window + 1 - y_row;
+        to = min(kHalfTile, mine + 1 - y_row);
+        keep = p.sinks - y_row;
+        edge = y_row + kHalfTile - 1 > x_row || (x_row + kTile - 1) - y_row >= p.window || x_row + kTile > len;
+      }
+      const float* col_lse = stats + stage * 2 * kHalfTile;
+      const float* col_delta = col_lse + kHalfTile;
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], d[32];
+        tmem_ld_32x32(ts + c * 32, s);
+        tmem_ld_32x32(td + c * 32, d);
+        tmem_ld_wait();
+        uint32_t pp[16], dd[16];
+#pragma unroll
+        for (int x = 0; x < 32; x += 2) {
+          float pr[2], ds[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int k = c * 32 + x + u;
+            const float lse = KEYS ? col_lse[k] : row_lse, delta = KEYS ? col_delta[k] : row_delta;
+            pr[u] = exp2_approx(fmaf(__uint_as_float(s[x + u]), scale, -lse));
+            ds[u] = pr[u] * (__uint_as_float(d[x + u]) - delta);
+            if (edge && !(k < to && (k >= from || (!KEYS && k < keep)))) pr[u] = ds[u] = 0.f;
+          }
+          if constexpr (KEYS) pp[x / 2] = pack2<T>(pr[0], pr[1]);
+          dd[x / 2] = pack2<T>(ds[0], ds[1]);
+        }
+        if constexpr (KEYS) tmem_st_32x16(ts + c * 16, pp);
+        tmem_st_32x16(td + c * 16, dd);
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&d_full[g]));
+      stage += 2;
+    }
+    if (st.count > 0 && ok) {
+      ok = mbar_wait(smem_u32(acc_full), 0, abort_flag, p.status, kErrRows, kWaitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      tcgen05_fence_after();
+    }
+    // Group 0: dV, or the first half of dQ; group 1: dK, or the other half.
+    constexpr int kChunks = KEYS ? D / 32 : D / 64;
+    const uint32_t acc = tmem_acc + lanes + (KEYS ? g * D : g * (D / 2));
+    const float factor = KEYS && g == 0 ? 1.f : p.scale;
+    const bool some = st.count > 0 && ok;
+    const bool live = some && mine < len;
+    uint8_t* staged = KEYS ? tile_x + (1 - g) * kResident : tile_x;    // all products have been taken
+    // A first token whose far queries are other CTAs': this CTA's share goes to the workspace.
+    const bool shared_sum = KEYS && p.far_splits > 0 && mine < p.sinks && mine < p.seq;
+    float* far = nullptr;
+    if (shared_sum)
+      far = p.far + ((((int64_t(part) * p.batch + b) * p.kv_heads + own_head) * 2 + (1 - g)) * p.sinks + mine) * p.dim;
+#pragma unroll 1
+    for (int c = 0; c < kChunks; ++c) {
+      uint32_t raw[32];
+      if (some) {
+        tmem_ld_32x32(acc + c * 32, raw);
+        tmem_ld_wait();
+      }
+      if (!live) {
+#pragma unroll
+        for (int x = 0; x < 32; ++x) raw[x] = 0u;
+      }
+      if (far != nullptr) {
+#pragma unroll
+        for (int x = 0; x < 32; x += 4)
+          if (c * 32 + x < p.dim)
+            *reinterpret_cast<float4*>(far + c * 32 + x) =
+                make_float4(__uint_as_float(raw[x]) * factor, __uint_as_float(raw[x + 1]) * factor,
+                            __uint_as_float(raw[x + 2]) * factor, __uint_as_float(raw[x + 3]) * factor);
+      }
+      if (part == 0) stage_row<T>(staged, r, KEYS ? c : g * kChunks + c, raw, factor);
+    }
+    fence_proxy_async_smem();
+    if (KEYS) {
+      group_barrier(1 + g);
+      if (part == 0 && quarter == 0 && lane == 0 && x_row < p.seq) {
+        for (int box = 0; box < D / 64; ++box)
+          if (box * 64 < p.dim)
+            tma_store_4d(g == 0 ? &map_out1 : &map_out0, smem_u32(staged + box * (kTile * 128)), box * 64, x_row,
+                         own_head, b);
+        bulk_commit_group();
+        bulk_wait_read_all();
+      }
+    } else {
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (g == 0 && quarter == 0 && lane == 0 && x_row < p.seq) {
+        for (int box = 0; box < D / 64; ++box)
+          if (box * 64 < p.dim)
+            tma_store_4d(&map_out0, smem_u32(staged + box * (kTile * 128)), box * 64, x_row, own_head, b);
+        bulk_commit_group();
+        bulk_wait_read_all();
+      }
+    }
+    __syncwarp();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    settle(abort_flag);
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// delta_i = dO_i O_i, 16 lanes a row of one head; zero behind a sequence's end, whatever lies there.
+template <typename T>
+__global__ void __launch_bounds__(256)
+row_sums_kernel(const T* __restrict__ out, const T* __restrict__ dout, const Params p) {
+  const int lane = threadIdx.x & 15, h = blockIdx.y, b = blockIdx.z;
+  const int i = blockIdx.x * 16 + (threadIdx.x >> 4);
+  float sum = 0.f;
+  if (i < length_of(p, b) && lane * 8 < p.dim) {
+    const int64_t at = ((int64_t(b) * p.seq + i) * p.heads + h) * p.dim + lane * 8;
+    const uint4 x = *reinterpret_cast<const uint4*>(out + at), y = *reinterpret_cast<const uint4*>(dout + at);
+    const T* xs = reinterpret_cast<const T*>(&x);
+    const T* ys = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = fmaf(to_float(xs[k]), to_float(ys[k]), sum);
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) p.delta[(int64_t(b) * p.heads + h) * p.seq_pad + i] = sum;
+}
+
+// One warp a first token of a key head: its parts in order, rounded once.
+template <typename T>
+__global__ void __launch_bounds__(128)
+sum_far_kernel(T* __restrict__ dk, T* __restrict__ dv, const Params p) {
+  const int64_t n = int64_t(p.batch) * p.kv_heads * p.sinks * p.dim;
+  const int64_t x = int64_t(blockIdx.x) * 128 + threadIdx.x;
+  if (x >= 2 * n) return;
+  // x runs over [batch][kv_heads][2][sinks][dim], the layout of a part.
+  const int d = int(x % p.dim);
+  int64_t rest = x / p.dim;
+  const int row = int(rest % p.sinks);
+  rest /= p.sinks;
+  const int which = int(rest % 2);
+  rest /= 2;
+  const int h = int(rest % p.kv_heads), b = int(rest / p.kv_heads);
+  if (row >= p.seq) return;
+  float sum = 0.f;
+  for (int s = 0; s <= p.far_splits; ++s) sum += p.far[s * 2 * n + x];
+  T* out = which == 0 ? dk : dv;
+  out[((int64_t(b) * p.seq + row) * p.kv_heads + h) * p.dim + d] = from_float<T>(sum);
+}
+
+template <typename T, int D, bool KEYS>
+cudaError_t launch_backward(const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& y0, const CUtensorMap& y1,
+                            const CUtensorMap& o0, const CUtensorMap& o1, const Params& p, cudaStream_t stream) {
+  auto kernel = window_bwd_kernel<T, D, KEYS>;
+  const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes);
+  if (rc != cudaSuccess) return rc;
+  const int far = KEYS ? p.far_splits * ((p.sinks + kTile - 1) / kTile) : 0;
+  const dim3 grid((KEYS ? p.kv_heads : p.heads) * p.batch, far + (p.seq + kTile - 1) / kTile);
+  kernel<<<grid, kThreads, Layout<D>::kBytes, stream>>>(x0, x1, y0, y1, o0, o1, p);
+  return cudaGetLastError();
+}
+
+template <bool KEYS>
+cudaError_t backward(bool bf16, const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& y0,
+                     const CUtensorMap& y1, const CUtensorMap& o0, const CUtensorMap& o1, const Params& p,
+                     cudaStream_t stream) {
+  if (p.dim <= 64)
+    return bf16 ? launch_backward<__nv_bfloat16, 64, KEYS>(x0, x1, y0, y1, o0, o1, p, stream)
+                : launch_backward<__half, 64, KEYS>(x0, x1, y0, y1, o0, o1, p, stream);
+  return bf16 ? launch_backward<__nv_bfloat16, 128, KEYS>(x0, x1, y0, y1, o0, o1, p, stream)
+              : launch_backward<__half, 128, KEYS>(x0, x1, y0, y1, o0, o1, p, stream);
+}
+
+}  // namespace
+
+cudaError_t row_sums(bool bf16, const void* out, const void* dout, const Params& p, cudaStream_t stream) {
+  const dim3 grid(p.seq_pad / 16, p.heads, p.batch);
+  if (bf16)
+    row_sums_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(out),
+                                              static_cast<const __nv_bfloat16*>(dout), p);
+  else
+    row_sums_kernel<<<grid, 256, 0, stream>>>(static_cast<const __half*>(out), static_cast<const __half*>(dout), p);
+  return cudaGetLastError();
+}
+
+cudaError_t backward_keys(bool bf16, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q_half,
+                          const CUtensorMap& dout_half, const CUtensorMap& dk, const CUtensorMap& dv, const Params& p,
+                          cudaStream_t stream) {
+  return backward<true>(bf16, k, v, q_half, dout_half, dk, dv, p, stream);
+}
+
+cudaError_t backward_queries(bool bf16, const CUtensorMap& q, const CUtensorMap& dout, const CUtensorMap& k_half,
+                             const CUtensorMap& v_half, const CUtensorMap& dq, const Params& p, cudaStream_t stream) {
+  return backward<false>(bf16, q, dout, k_half, v_half, dq, dq, p, stream);
+}
+
+cudaError_t sum_far(bool bf16, void* dk, void* dv, const Params& p, cudaStream_t stream) {
+  const int64_t n = int64_t(2) * p.batch * p.kv_heads * p.sinks * p.dim;
+  const unsigned grid = static_cast<unsigned>((n + 127) / 128);
+  if (bf16)
+    sum_far_kernel<<<grid, 128, 0, stream>>>(static_cast<__nv_bfloat16*>(dk), static_cast<__nv_bfloat16*>(dv), p);
+  else
+    sum_far_kernel<<<grid, 128, 0, stream>>>(static_cast<__half*>(dk), static_cast<__half*>(dv), p);
+  return cudaGetLastError();
+}
+
+}  // namespace attn
+}  // namespace mb

@@ -1,5 +1,6 @@
 """Public ops namespace (same names as ``megablocks.ops``) plus this library's additions."""
 
+from megablocks_b200.ops.attention import window_attention, window_attention_decode
 from megablocks_b200.ops.gg import gmm, gmm_bins, grouped_gemm
 from megablocks_b200.ops.metadata import (exclusive_cumsum, histogram, inclusive_cumsum, repeat, replicate,
                                           round_up, sort, sum, topology)
@@ -32,6 +33,8 @@ __all__ = [
     'route_plan',
     'select_experts',
     'update_expert_bias',
+    'window_attention',
+    'window_attention_decode',
     'Matrix',
     'sdd',
     'dsd',

@@ -23,6 +23,9 @@ _MESSAGES = {
     20: 'expert-parallel dispatch: a peer never released its receive buffer',
     32: 'data-parallel gradient reduction: a peer never announced its bucket',
     33: 'data-parallel gradient reduction: a peer never finished reading or writing a bucket',
+    48: 'window attention: the loader timed out waiting for a free shared-memory stage',
+    49: 'window attention: the MMA warp timed out waiting for a tile or for probabilities',
+    50: 'window attention: the row warps timed out waiting for scores or for the result',
 }
 
 
