@@ -84,29 +84,35 @@ void check_like(const at::Tensor& t, const at::Tensor& like, const char* name) {
 
 bool window_attention_in_place(const at::Tensor& t) { return in_place(t); }
 
-// {out, log-sum-exp [batch, heads, padded seq] (undefined unless wanted)}
-std::vector<at::Tensor> window_attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                 int64_t window, int64_t sinks, const OptTensor& lengths, double scale,
-                                                 bool want_lse) {
+namespace {
+
+// {out} and, where they are wanted for a backward pass, the log-sum-exp [batch, heads, padded seq] and what
+// the rounding of `out` left.
+std::vector<at::Tensor> window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
+                                       int64_t sinks, const OptTensor& lengths, double scale, bool train) {
   c10::cuda::CUDAGuard guard(q.device());
   attn::Params p = make_params(q, k, window, sinks, lengths, scale);
   TORCH_CHECK(k.device() == q.device() && k.scalar_type() == q.scalar_type(), "window_attention: k does not match q");
   check_like(v, k, "v");
-  at::Tensor out = at::empty({p.batch, p.seq, p.heads, p.dim}, q.options()), lse;
-  if (want_lse) {
+  at::Tensor out = at::empty({p.batch, p.seq, p.heads, p.dim}, q.options()), lse, low;
+  if (train) {
+    low = at::empty_like(out);
+    p.out_low = low.data_ptr();
     lse = at::empty({p.batch, p.heads, p.seq_pad}, q.options().dtype(at::kFloat));
     p.lse = lse.data_ptr<float>();
   }
+  const CUtensorMap map_out = make_map(out, attn::kTile);
   C10_CUDA_CHECK(attn::forward(q.scalar_type() == at::kBFloat16, make_map(q, attn::kTile), make_map(k, attn::kTile),
-                               make_map(v, attn::kTile), make_map(out, attn::kTile), p, stream()));
+                               make_map(v, attn::kTile), map_out, train ? make_map(low, attn::kTile) : map_out, p,
+                               stream()));
   count_launches(1);
-  return {out, lse};
+  return {out, lse, low};
 }
 
-std::vector<at::Tensor> window_attention_backward(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
-                                                  const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse,
-                                                  int64_t window, int64_t sinks, const OptTensor& lengths, double scale,
-                                                  bool want_q, bool want_kv) {
+std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+                                        const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse,
+                                        const at::Tensor& low, int64_t window, int64_t sinks, const OptTensor& lengths,
+                                        double scale, bool want_q, bool want_kv) {
   c10::cuda::CUDAGuard guard(q.device());
   attn::Params p = make_params(q, k, window, sinks, lengths, scale);
   TORCH_CHECK(k.device() == q.device() && k.scalar_type() == q.scalar_type(), "window_attention: k does not match q");
@@ -120,6 +126,7 @@ std::vector<at::Tensor> window_attention_backward(const at::Tensor& dout, const 
   at::Tensor dq, dk, dv, far;
   at::Tensor delta = at::empty_like(lse);
   p.lse = lse.data_ptr<float>();
+  p.out_low = low.data_ptr();
   p.delta = delta.data_ptr<float>();
   C10_CUDA_CHECK(attn::row_sums(bf16, out.data_ptr(), dout.data_ptr(), p, stream()));
   count_launches(1);
@@ -158,8 +165,54 @@ std::vector<at::Tensor> window_attention_backward(const at::Tensor& dout, const 
   return {dq, dk, dv};
 }
 
+struct Window : torch::autograd::Function<Window> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                            const at::Tensor& v, int64_t window, int64_t sinks, const OptTensor& lengths, double scale) {
+    const auto out = window_forward(q, k, v, window, sinks, lengths, scale, true);
+    ctx->save_for_backward({q, k, v, out[0], out[1], out[2], lengths.has_value() ? *lengths : at::Tensor()});
+    ctx->saved_data["how"] = std::vector<int64_t>{window, sinks};
+    ctx->saved_data["scale"] = scale;
+    return out[0];
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(7);
+    const auto s = ctx->get_saved_variables();
+    const auto how = ctx->saved_data["how"].toIntVector();
+    at::Tensor dout = grads[0].contiguous();
+    if (reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 != 0) dout = dout.clone();
+    const bool need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2);
+    const auto g = window_backward(dout, s[0], s[1], s[2], s[3], s[4], s[5], how[0], how[1],
+                                   s[6].defined() ? OptTensor(s[6]) : OptTensor(), ctx->saved_data["scale"].toDouble(),
+                                   ctx->needs_input_grad(0), need_k || need_v);
+    out[0] = g[0];
+    if (need_k) out[1] = g[1];
+    if (need_v) out[2] = g[2];
+    return out;
+  }
+};
+
+OptTensor int32(const OptTensor& t) {
+  return t.has_value() ? OptTensor(t->to(at::kInt).contiguous()) : OptTensor();
+}
+
+}  // namespace
+
+// Tensors that the kernels cannot read in place are copied.  Behind a C++ node: the host passes it in a few
+// microseconds each way, a Python one in some 20.
+at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
+                            int64_t sinks, const OptTensor& lengths, double scale) {
+  auto ready = [](const at::Tensor& t) { return in_place(t) ? t : t.clone(at::MemoryFormat::Contiguous); };
+  const at::Tensor qr = ready(q), kr = ready(k), vr = ready(v);
+  if (at::GradMode::is_enabled() && (qr.requires_grad() || kr.requires_grad() || vr.requires_grad()))
+    return Window::apply(qr, kr, vr, window, sinks, int32(lengths), scale);
+  return window_forward(qr, kr, vr, window, sinks, int32(lengths), scale, false)[0];
+}
+
 at::Tensor window_attention_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                   const at::Tensor& lengths, int64_t window, int64_t sinks, double scale) {
+                                   const at::Tensor& lengths_in, int64_t window, int64_t sinks, double scale) {
+  const at::Tensor lengths = lengths_in.to(at::kInt).contiguous();
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.is_contiguous() && reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 == 0 &&
                   in_place(k) && in_place(v) && q.device() == k.device() && k.device() == v.device() &&
                   q.scalar_type() == k.scalar_type() && k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() &&

@@ -31,31 +31,19 @@ at::Tensor router_topk_backward(const at::Tensor& scores, const at::Tensor& weig
                                 const at::Tensor& dscores, const at::Tensor& dweights, double norm_p);
 
 // model_glue.cpp: expert selection and distillation
-std::vector<at::Tensor> select_experts_forward(const at::Tensor& logits, int64_t top_k, bool use_sigmoid,
-                                               const c10::optional<at::Tensor>& bias, int64_t groups,
-                                               int64_t top_groups, int64_t norm_p, double scale);
-at::Tensor select_experts_backward(const at::Tensor& logits, const at::Tensor& experts,
-                                   const c10::optional<at::Tensor>& dscores,
-                                   const c10::optional<at::Tensor>& dweights, bool use_sigmoid, int64_t norm_p,
-                                   double scale);
-std::vector<at::Tensor> distill_forward(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& ids,
-                                        const c10::optional<at::Tensor>& targets, double temperature,
-                                        double hard_weight, double scale, bool want_grad, bool in_place);
-at::Tensor distill_backward(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& ids,
-                            const c10::optional<at::Tensor>& targets, const at::Tensor& stats,
-                            const at::Tensor& grad_out, double temperature, double hard_weight, double scale);
-void scale_unless_one_op(at::Tensor x, const at::Tensor& factor);
+std::vector<at::Tensor> select_experts(const at::Tensor& logits, int64_t top_k, bool use_sigmoid,
+                                       const c10::optional<at::Tensor>& bias, int64_t groups, int64_t top_groups,
+                                       int64_t norm_p, double scale);
+at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& ids,
+                             const c10::optional<at::Tensor>& targets, double temperature, double hard_weight);
+std::vector<at::Tensor> distill_in_place(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& ids,
+                                         const c10::optional<at::Tensor>& targets, double temperature,
+                                         double hard_weight);
 
 // attention_glue.cpp
 bool window_attention_in_place(const at::Tensor& t);
-std::vector<at::Tensor> window_attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                 int64_t window, int64_t sinks,
-                                                 const c10::optional<at::Tensor>& lengths, double scale, bool want_lse);
-std::vector<at::Tensor> window_attention_backward(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
-                                                  const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse,
-                                                  int64_t window, int64_t sinks,
-                                                  const c10::optional<at::Tensor>& lengths, double scale, bool want_q,
-                                                  bool want_kv);
+at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
+                            int64_t sinks, const c10::optional<at::Tensor>& lengths, double scale);
 at::Tensor window_attention_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                    const at::Tensor& lengths, int64_t window, int64_t sinks, double scale);
 
@@ -168,14 +156,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("binned_scatter_wgrad", &mb::binned_scatter_wgrad);
   m.def("router_topk_forward", &mb::router_topk_forward);
   m.def("router_topk_backward", &mb::router_topk_backward);
-  m.def("select_experts_forward", &mb::select_experts_forward);
-  m.def("select_experts_backward", &mb::select_experts_backward);
-  m.def("distill_forward", &mb::distill_forward, "Per-row loss, row statistics and, if wanted, the gradient");
-  m.def("distill_backward", &mb::distill_backward);
-  m.def("scale_unless_one_", &mb::scale_unless_one_op);
+  m.def("select_experts", &mb::select_experts, "Scores, weights and ids of the chosen experts; differentiable");
+  m.def("distillation_loss", &mb::distillation_loss, "Mean loss against a teacher's top logits; differentiable");
+  m.def("distill_in_place", &mb::distill_in_place, "The same loss, its gradient written over the logits");
   m.def("window_attention_in_place", &mb::window_attention_in_place);
-  m.def("window_attention_forward", &mb::window_attention_forward);
-  m.def("window_attention_backward", &mb::window_attention_backward);
+  m.def("window_attention", &mb::window_attention, "Windowed causal attention; differentiable");
   m.def("window_attention_decode", &mb::window_attention_decode);
   m.def("grouped_gemm_supported", &mb::grouped_gemm_supported);
   m.def("grouped_gemm", &mb::grouped_gemm);

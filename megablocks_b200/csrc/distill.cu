@@ -269,7 +269,7 @@ __device__ __forceinline__ Powers powers(const DistillArgs& a) {
 
 template <typename T, bool CACHED>
 __global__ void __launch_bounds__(kMaxThreads)
-distill_fwd_kernel(const DistillArgs a, float* __restrict__ loss, float* __restrict__ stats, T* grad) {
+distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ float red[3 * kMaxThreads / 32];
@@ -335,7 +335,7 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ loss, float* __restr
       const uint32_t bar = ptx::smem_u32(&bars[c]);
       if (!ptx::mbar_wait(bar, 0, &abort_flag, a.status, kDistillTimeout, kWaitNs)) {
         // The row never came: no result, and no way out before the copies have ended or the limit is reached.
-        if (threadIdx.x == 0) loss[row] = NAN;
+        if (threadIdx.x == 0) stats[4 * row] = NAN;
         for (; c * chunk_packs < cut.packs; ++c) {
           const uint64_t t0 = ptx::globaltimer_ns();
           while (!ptx::mbar_try_wait(ptx::smem_u32(&bars[c]), 0) && ptx::globaltimer_ns() - t0 < kWaitNs) {}
@@ -374,10 +374,7 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ loss, float* __restr
     for (int w = 0; w < int(blockDim.x >> 5); ++w) sum += red[w];
     float l = live ? a.temperature * a.temperature * (entropy_s - kLn2 * sum) : 0.f;
     if (target >= 0) l += a.hard_weight * (kLn2 * __log2f(sums.hard) + (sums.m - z_target));
-    loss[row] = l;
-    stats[3 * row] = sums.m;
-    stats[3 * row + 1] = sums.soft;
-    stats[3 * row + 2] = sums.hard;
+    *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(l, sums.m, sums.soft, sums.hard);
   }
   if (grad == nullptr) return;
   T* out = grad + row * a.vocab;
@@ -411,12 +408,26 @@ distill_bwd_kernel(const DistillArgs a, const float* __restrict__ stats, const f
     if (column[i] >= 0) z[i] = to_float(in[column[i]]);
   const float z_target = target >= 0 ? to_float(in[target]) : 0.f;
   const float scale = a.scale * *grad_out;
-  const RowGrad g = row_grad(a, live_s != 0, target >= 0, scale, stats[3 * row], stats[3 * row + 1], stats[3 * row + 2],
-                             powers(a));
+  const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
+  const RowGrad g = row_grad(a, live_s != 0, target >= 0, scale, st.y, st.z, st.w, powers(a));
   T* out = grad + row * a.vocab;
   write_gradient(in, cut, out, a.vocab, g);
   __syncthreads();
   write_named(a, out, g, a.temperature * scale, a.hard_weight * scale, p, column, z, target, z_target);
+}
+
+__global__ void __launch_bounds__(1024)
+distill_mean_kernel(const float* __restrict__ stats, int64_t rows, float* __restrict__ mean) {
+  __shared__ float red[32];
+  float sum = 0.f;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) sum += stats[4 * r];
+  sum = warp_sum(sum);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    sum = warp_sum(red[threadIdx.x]);
+    if (threadIdx.x == 0) *mean = sum / float(rows);
+  }
 }
 
 template <typename T>
@@ -450,7 +461,7 @@ bool valid(const DistillArgs& a) {
 
 }  // namespace
 
-cudaError_t distill_fwd(DType type, const DistillArgs& a, float* loss, float* stats, void* grad, cudaStream_t stream) {
+cudaError_t distill_fwd(DType type, const DistillArgs& a, float* stats, void* grad, cudaStream_t stream) {
   if (!valid(a)) return cudaErrorInvalidValue;
   if (a.rows == 0) return cudaSuccess;
   MB_SWITCH_FLOAT(type, T, {
@@ -464,11 +475,16 @@ cudaError_t distill_fwd(DType type, const DistillArgs& a, float* loss, float* st
                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
         if (rc != cudaSuccess) return rc;
       }
-      distill_fwd_kernel<T, true><<<unsigned(a.rows), threads, shared, stream>>>(a, loss, stats, static_cast<T*>(grad));
+      distill_fwd_kernel<T, true><<<unsigned(a.rows), threads, shared, stream>>>(a, stats, static_cast<T*>(grad));
     } else {
-      distill_fwd_kernel<T, false><<<unsigned(a.rows), threads, slots, stream>>>(a, loss, stats, static_cast<T*>(grad));
+      distill_fwd_kernel<T, false><<<unsigned(a.rows), threads, slots, stream>>>(a, stats, static_cast<T*>(grad));
     }
   })
+  return cudaGetLastError();
+}
+
+cudaError_t distill_mean(const float* stats, int64_t rows, float* mean, cudaStream_t stream) {
+  distill_mean_kernel<<<1, 1024, 0, stream>>>(stats, rows, mean);
   return cudaGetLastError();
 }
 

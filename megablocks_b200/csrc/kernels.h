@@ -108,9 +108,11 @@ struct DistillArgs {
   float scale;                         // of the gradient (1 / rows)
   int* status;                         // receives kDistillTimeout when a copy never completes
 };
-// Per-row loss and `stats` [rows, 3]: the largest logit and the sums of e^((z - max) / T) and e^(z - max);
+// `stats` [rows, 4]: a row's loss, its largest logit and the sums of e^((z - max) / T) and e^(z - max);
 // with `grad` (may be the logits themselves) also the gradient of scale * sum(loss).
-cudaError_t distill_fwd(DType type, const DistillArgs& args, float* loss, float* stats, void* grad, cudaStream_t stream);
+cudaError_t distill_fwd(DType type, const DistillArgs& args, float* stats, void* grad, cudaStream_t stream);
+// Mean of the rows' losses, in a fixed order.
+cudaError_t distill_mean(const float* stats, int64_t rows, float* mean, cudaStream_t stream);
 // The gradient alone, from the statistics of a forward pass, times *grad_out.
 cudaError_t distill_bwd(DType type, const DistillArgs& args, const float* stats, const float* grad_out, void* grad,
                         cudaStream_t stream);
@@ -135,7 +137,8 @@ struct Params {
   const int* lengths;                  // [batch] valid tokens, nullable (all of them)
   float scale;                         // of the scores
   float* lse;                          // [batch, heads, seq_pad] base-2 log-sum-exp of the scaled scores
-  float* delta;                        // [batch, heads, seq_pad] sum over dim of dout * out
+  void* out_low;                       // nullable: what the rounding of `out` left, [batch, seq, heads, dim]
+  float* delta;                        // [batch, heads, seq_pad] sum over dim of dout * (out + out_low)
   int seq_pad;
   // Backward pass over the keys: queries a window away from the first tokens are split into `far_splits`
   // parts of `far_tiles` tiles, whose shares of the first tokens' gradients are summed afterwards.
@@ -145,7 +148,7 @@ struct Params {
 };
 
 cudaError_t forward(bool bf16, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                    const CUtensorMap& out, const Params& params, cudaStream_t stream);
+                    const CUtensorMap& out, const CUtensorMap& out_low, const Params& params, cudaStream_t stream);
 // delta, and zeros behind the sequences' ends.
 cudaError_t row_sums(bool bf16, const void* out, const void* dout, const Params& params, cudaStream_t stream);
 // Maps with 128-row boxes (`q`, `k`, ...: resident tiles and results) and 64-row boxes (`q_half`, ...: streamed).

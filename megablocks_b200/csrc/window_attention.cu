@@ -52,7 +52,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
-                  const __grid_constant__ Params p) {
+                  const __grid_constant__ CUtensorMap map_low, const __grid_constant__ Params p) {
   using L = Layout<D>;
   constexpr int kTileBytes = L::kTileBytes, kStages = L::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -285,32 +285,39 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
     const bool live = rows && i < len && ok;
     const float inv = live ? 1.f / sum : 0.f;
-    uint8_t* staged = tile_q + g * kTileBytes;        // the queries have been used
-#pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t raw[32];
-      if (rows && ok) {
-        tmem_ld_32x32(to + c * 32, raw);
-        tmem_ld_wait();
-      }
-      if (!live) {                                    // zeros behind the end, whatever was computed there
-#pragma unroll
-        for (int x = 0; x < 32; ++x) raw[x] = 0u;
-      }
-      stage_row<T>(staged, r, c, raw, inv);
-    }
     if (p.lse != nullptr)
       p.lse[(int64_t(b) * p.heads + head) * p.seq_pad + i] = live ? m + __log2f(sum) : INFINITY;
-    fence_proxy_async_smem();
-    group_barrier(1 + g);
-    if (quarter == 0 && lane == 0 && q0 + g * kTile < p.seq) {
-      for (int box = 0; box < D / 64; ++box)
-        if (box * 64 < p.dim)
-          tma_store_4d(&map_o, smem_u32(staged + box * (kTile * 128)), box * 64, q0 + g * kTile, head, b);
-      bulk_commit_group();
-      bulk_wait_read_all();
+    // The result, and for a backward pass what its rounding left (the row sums delta want it), one after the
+    // other through the queries' tile, which has been used.
+    uint8_t* staged = tile_q + g * kTileBytes;
+    for (int part = 0; part < (p.out_low != nullptr ? 2 : 1); ++part) {
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t raw[32];
+        if (rows && ok) {
+          tmem_ld_32x32(to + c * 32, raw);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {                // zeros behind the end, whatever was computed there
+          float o = live ? __uint_as_float(raw[x]) * inv : 0.f;
+          if (part == 1) o -= to_float(from_float<T>(o));
+          raw[x] = __float_as_uint(o);
+        }
+        stage_row<T>(staged, r, c, raw, 1.f);
+      }
+      fence_proxy_async_smem();
+      group_barrier(1 + g);
+      if (quarter == 0 && lane == 0 && q0 + g * kTile < p.seq) {
+        for (int box = 0; box < D / 64; ++box)
+          if (box * 64 < p.dim)
+            tma_store_4d(part == 0 ? &map_o : &map_low, smem_u32(staged + box * (kTile * 128)), box * 64,
+                         q0 + g * kTile, head, b);
+        bulk_commit_group();
+        bulk_wait_read_all();
+      }
+      group_barrier(1 + g);
     }
-    __syncwarp();
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -323,24 +330,24 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
 template <typename T, int D>
 cudaError_t launch_forward(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& out,
-                           const Params& p, cudaStream_t stream) {
+                           const CUtensorMap& low, const Params& p, cudaStream_t stream) {
   auto kernel = window_fwd_kernel<T, D>;
   const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes);
   if (rc != cudaSuccess) return rc;
   const dim3 grid((p.seq + 2 * kTile - 1) / (2 * kTile), p.heads, p.batch);
-  kernel<<<grid, kThreads, Layout<D>::kBytes, stream>>>(q, k, v, out, p);
+  kernel<<<grid, kThreads, Layout<D>::kBytes, stream>>>(q, k, v, out, low, p);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t forward(bool bf16, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                    const CUtensorMap& out, const Params& p, cudaStream_t stream) {
+                    const CUtensorMap& out, const CUtensorMap& low, const Params& p, cudaStream_t stream) {
   if (p.dim <= 64)
-    return bf16 ? launch_forward<__nv_bfloat16, 64>(q, k, v, out, p, stream)
-                : launch_forward<__half, 64>(q, k, v, out, p, stream);
-  return bf16 ? launch_forward<__nv_bfloat16, 128>(q, k, v, out, p, stream)
-              : launch_forward<__half, 128>(q, k, v, out, p, stream);
+    return bf16 ? launch_forward<__nv_bfloat16, 64>(q, k, v, out, low, p, stream)
+                : launch_forward<__half, 64>(q, k, v, out, low, p, stream);
+  return bf16 ? launch_forward<__nv_bfloat16, 128>(q, k, v, out, low, p, stream)
+              : launch_forward<__half, 128>(q, k, v, out, low, p, stream);
 }
 
 }  // namespace attn

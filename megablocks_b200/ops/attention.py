@@ -14,35 +14,13 @@ the scores.
 """
 
 import math
-from typing import Any, Optional
+from typing import Optional
 
 import torch
 
 from megablocks_b200._ext import ext
 
 _KERNEL_DTYPES = (torch.bfloat16, torch.float16)
-
-
-class _WindowAttention(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx: Any, q, k, v, window, sinks, lengths, scale):
-        out, lse = ext().window_attention_forward(q, k, v, window, sinks, lengths, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
-        ctx.how = window, sinks, scale
-        return out
-
-    @staticmethod
-    def backward(ctx: Any, dout):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
-        window, sinks, scale = ctx.how
-        need = ctx.needs_input_grad
-        dout = dout.contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
-        dq, dk, dv = ext().window_attention_backward(dout, q, k, v, out, lse, window, sinks, lengths, scale, need[0],
-                                                     need[1] or need[2])
-        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 
 def _check(q, k, v, window, sinks, lengths, scale, batch):
@@ -69,10 +47,6 @@ def _kernel_dim(q: torch.Tensor) -> bool:
     return q.is_cuda and q.dtype in _KERNEL_DTYPES and q.shape[-1] % 8 == 0 and q.shape[-1] <= 128
 
 
-def _int32(lengths):
-    return None if lengths is None else lengths.to(torch.int32).contiguous()
-
-
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
                      lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
     """Attention of ``q[batch, seq, heads, dim]`` over ``k, v[batch, seq, kv_heads, dim]``; returns a contiguous
@@ -88,12 +62,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     window = max(q.shape[1], 1) if window is None else int(window)
     if not _kernel_dim(q) or q.numel() == 0:
         return _composed(q, k, v, window, int(sinks), lengths, scale)
-    in_place = ext().window_attention_in_place
-    q, k, v = (t if in_place(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-    args = (q, k, v, window, int(sinks), _int32(lengths), scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _WindowAttention.apply(*args)
-    return ext().window_attention_forward(*args, False)[0]
+    return ext().window_attention(q, k, v, window, int(sinks), lengths, scale)
 
 
 def _attend(q, k, v, seen, scale):
@@ -144,7 +113,7 @@ def window_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     window = max(k.shape[1], 1) if window is None else int(window)
     if _kernel_dim(q) and q.numel() and k.numel() and all(ext().window_attention_in_place(t) for t in (k, v)):
         q = q.contiguous()
-        return ext().window_attention_decode(q if q.data_ptr() % 4 == 0 else q.clone(), k, v, _int32(lengths), window,
+        return ext().window_attention_decode(q if q.data_ptr() % 4 == 0 else q.clone(), k, v, lengths, window,
                                              int(sinks), scale)
     return _composed_decode(q, k, v, lengths, window, int(sinks), scale)
 

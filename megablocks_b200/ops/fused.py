@@ -93,35 +93,6 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     return F.cross_entropy(logits.float(), targets)
 
 
-def _mean_rows(loss: torch.Tensor) -> torch.Tensor:
-    return loss.sum() / max(loss.shape[0], 1)
-
-
-class _Distillation(torch.autograd.Function):
-    """The forward pass takes the gradient of the loss while it has the row, into a tensor of its own; the
-    backward pass multiplies it by the incoming scalar where that is not one.  fp16 logits take it in the
-    backward pass instead: unscaled it underflows, and the loss scale is only known there."""
-
-    @staticmethod
-    def forward(ctx: Any, logits, values, ids, targets, temperature, hard_weight):
-        ctx.how = temperature, hard_weight, 1.0 / max(logits.shape[0], 1)
-        loss, stats, ctx.grad = ext().distill_forward(logits, values, ids, targets, *ctx.how,
-                                                      logits.dtype != torch.float16, False)
-        ctx.save_for_backward(logits, values, ids, targets, stats)
-        return _mean_rows(loss)
-
-    @staticmethod
-    def backward(ctx: Any, grad_out: torch.Tensor):
-        grad, ctx.grad = ctx.grad, None         # a second backward pass takes it again from the logits
-        scale = grad_out.detach().float().reshape(1)
-        if grad is not None:
-            ext().scale_unless_one_(grad, scale)
-        else:
-            logits, values, ids, targets, stats = ctx.saved_tensors
-            grad = ext().distill_backward(logits, values, ids, targets, stats, scale, *ctx.how)
-        return grad, None, None, None, None, None
-
-
 class _LinearDistillation(torch.autograd.Function):
     """The language-model head and the loss: the gradient of the logits over the logits, as in
     :class:`_LinearCrossEntropy`."""
@@ -129,10 +100,9 @@ class _LinearDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, hidden, weight, values, ids, targets, temperature, hard_weight):
         logits = hidden @ weight.t()
-        loss, _, dlogits = ext().distill_forward(logits, values, ids, targets, temperature, hard_weight,
-                                                 1.0 / max(logits.shape[0], 1), True, True)
+        loss, dlogits = ext().distill_in_place(logits, values, ids, targets, temperature, hard_weight)
         ctx.save_for_backward(hidden, weight, dlogits)
-        return _mean_rows(loss)
+        return loss
 
     @staticmethod
     def backward(ctx: Any, grad_out: torch.Tensor):
@@ -144,6 +114,7 @@ class _LinearDistillation(torch.autograd.Function):
 
 
 MAX_TEACHER_TOP = 1024
+_DISTILL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _check_distillation(rows, device, teacher_logits, teacher_ids, temperature, targets, hard_weight):
@@ -167,11 +138,6 @@ def _check_distillation(rows, device, teacher_logits, teacher_ids, temperature, 
         raise ValueError('the teacher\'s logits, its ids and the targets must be on the device of the logits')
 
 
-def _teacher(teacher_logits, teacher_ids, targets, hard_weight):
-    return (teacher_logits.detach().contiguous(), teacher_ids.contiguous(),
-            targets.contiguous() if targets is not None and hard_weight else None)
-
-
 def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                       temperature: float = 1.0, targets=None, hard_weight: float = 0.0) -> torch.Tensor:
     """Mean over the rows of ``T^2 KL(p || q) + hard_weight * cross_entropy(logits, targets)``.
@@ -182,16 +148,11 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     a row without a used slot has no such term, one whose target lies outside the vocabulary no cross
     entropy, and a row with neither has a gradient of zero, whatever its logits.  Every row counts in the mean.
     The teacher gets no gradient; the logits stay as they are."""
+    if logits.is_cuda and logits.dtype in _DISTILL_DTYPES and teacher_logits.dtype != torch.float64:
+        return ext().distillation_loss(logits, teacher_logits, teacher_ids, targets, temperature, hard_weight)
     if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] < 1:
         raise ValueError('distillation expects floating-point logits[rows, vocab]')
     _check_distillation(logits.shape[0], logits.device, teacher_logits, teacher_ids, temperature, targets, hard_weight)
-    if (logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float16, torch.float32)
-            and teacher_logits.dtype != torch.float64):
-        logits = logits.contiguous()
-        args = (*_teacher(teacher_logits, teacher_ids, targets, hard_weight), float(temperature), float(hard_weight))
-        if torch.is_grad_enabled() and logits.requires_grad:
-            return _Distillation.apply(logits, *args)
-        return _mean_rows(ext().distill_forward(logits, *args, 1.0, False, False)[0])
     return _composed_distillation(logits, teacher_logits, teacher_ids, temperature, targets, hard_weight)
 
 
@@ -227,12 +188,9 @@ def linear_distillation_loss(hidden: torch.Tensor, weight: torch.Tensor, teacher
     if (hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float32) and hidden.dim() == 2
             and weight.dtype == hidden.dtype and teacher_logits.dtype != torch.float64
             and not torch.is_autocast_enabled() and os.environ.get('MB200_FUSED_LM_LOSS', '1') != '0'):
-        _check_distillation(hidden.shape[0], hidden.device, teacher_logits, teacher_ids, temperature, targets,
-                            hard_weight)
         if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-            args = _teacher(teacher_logits, teacher_ids, targets, hard_weight)
-            return _LinearDistillation.apply(hidden.contiguous(), weight, *args, float(temperature),
-                                             float(hard_weight))
+            return _LinearDistillation.apply(hidden.contiguous(), weight, teacher_logits, teacher_ids, targets,
+                                             temperature, hard_weight)
     return distillation_loss(F.linear(hidden, weight), teacher_logits, teacher_ids, temperature, targets, hard_weight)
 
 

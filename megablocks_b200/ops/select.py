@@ -21,7 +21,7 @@ On CUDA the forward and the backward pass are one kernel each (``csrc/select_exp
 """
 
 import math
-from typing import Any, Optional, Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -29,39 +29,13 @@ from megablocks_b200._ext import ext
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 32, 32
 _SCORES = ('softmax', 'sigmoid')
+_KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-class _SelectExperts(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx: Any, logits, top_k, use_sigmoid, bias, groups, top_groups, norm_p, scale):
-        scores, weights, experts = ext().select_experts_forward(logits, top_k, use_sigmoid, bias, groups, top_groups,
-                                                                norm_p, scale)
-        ctx.save_for_backward(logits, experts)
-        ctx.how = use_sigmoid, norm_p, scale
-        ctx.mark_non_differentiable(experts)
-        ctx.set_materialize_grads(False)
-        return scores, weights, experts
-
-    @staticmethod
-    def backward(ctx: Any, dscores, dweights, _dexperts):
-        none = (None,) * 7
-        if dscores is None and dweights is None:
-            return (None, *none)
-        logits, experts = ctx.saved_tensors
-        if dscores is not None and not (dscores.stride(1) == 1 and dscores.stride(0) in (0, dscores.shape[1])):
-            dscores = dscores.contiguous()          # but one row that is expanded over the tokens is read as it is
-        if dweights is not None:
-            dweights = dweights.contiguous()
-        return (ext().select_experts_backward(logits, experts, dscores, dweights, *ctx.how), *none)
-
-
-def _check(logits, top_k, score, bias, groups, top_groups, norm_p):
+def _check(logits, top_k, bias, groups, top_groups):
     if logits.dim() != 2 or logits.dtype not in (torch.float16, torch.bfloat16, torch.float32, torch.float64):
         raise ValueError('select_experts expects floating-point logits[tokens, experts]')
     experts = logits.shape[1]
-    if score not in _SCORES:
-        raise ValueError(f'score must be one of {_SCORES}, got {score!r}')
     if not 1 <= experts <= MAX_EXPERTS:
         raise ValueError(f'select_experts takes 1 to {MAX_EXPERTS} experts, got {experts}')
     if not 1 <= groups <= MAX_GROUPS or experts % groups:
@@ -71,8 +45,6 @@ def _check(logits, top_k, score, bias, groups, top_groups, norm_p):
     if not 1 <= top_k <= min(MAX_TOP_K, top_groups * (experts // groups)):
         raise ValueError(f'top_k must lie in [1, {min(MAX_TOP_K, top_groups * (experts // groups))}] (at most '
                          f'{MAX_TOP_K}, and what the chosen groups hold), got {top_k}')
-    if norm_p not in (None, 0, 1, 2):
-        raise ValueError(f'norm_p must be None, 1 or 2, got {norm_p!r}')
     if bias is not None and (bias.shape != (experts,) or bias.dtype != torch.float32 or bias.device != logits.device):
         raise ValueError('bias must be a float32 vector with one entry per expert, on the device of the logits')
 
@@ -85,17 +57,15 @@ def select_experts(logits: torch.Tensor, top_k: int, *, score: str = 'softmax', 
     Scores and weights have the type of the logits, the ids are int64.  ``bias`` is fp32; ``top_groups`` is by
     default all of them.  Up to 1024 experts, 32 groups and ``top_k`` 32."""
     top_groups = groups if top_groups is None else top_groups
-    _check(logits, top_k, score, bias, groups, top_groups, norm_p)
-    if bias is not None:
-        bias = bias.detach()
+    if score not in _SCORES:
+        raise ValueError(f'score must be one of {_SCORES}, got {score!r}')
+    if norm_p not in (None, 0, 1, 2):
+        raise ValueError(f'norm_p must be None, 1 or 2, got {norm_p!r}')
     norm_p = int(norm_p or 0)
-    if logits.is_cuda and logits.dtype != torch.float64:
-        args = (logits.contiguous(), int(top_k), score == 'sigmoid', None if bias is None else bias.contiguous(),
-                int(groups), int(top_groups), norm_p, float(scale))
-        if torch.is_grad_enabled() and logits.requires_grad:
-            return _SelectExperts.apply(*args)
-        return tuple(ext().select_experts_forward(*args))
-    return _composed(logits, top_k, score, bias, groups, top_groups, norm_p, scale)
+    if logits.is_cuda and logits.dtype in _KERNEL_DTYPES:
+        return tuple(ext().select_experts(logits, top_k, score == 'sigmoid', bias, groups, top_groups, norm_p, scale))
+    _check(logits, top_k, bias, groups, top_groups)
+    return _composed(logits, top_k, score, None if bias is None else bias.detach(), groups, top_groups, norm_p, scale)
 
 
 def _scores(x: torch.Tensor, score: str) -> torch.Tensor:
