@@ -99,7 +99,7 @@ std::vector<at::Tensor> window_forward(const at::Tensor& q, const at::Tensor& k,
     low = at::empty_like(out);
     p.out_low = low.data_ptr();
     lse = at::empty({p.batch, p.heads, p.seq_pad}, q.options().dtype(at::kFloat));
-    p.lse = lse.data_ptr<float>();
+    p.neg_lse = lse.data_ptr<float>();
   }
   const CUtensorMap map_out = make_map(out, attn::kTile);
   C10_CUDA_CHECK(attn::forward(q.scalar_type() == at::kBFloat16, make_map(q, attn::kTile), make_map(k, attn::kTile),
@@ -125,9 +125,9 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
   const bool bf16 = q.scalar_type() == at::kBFloat16;
   at::Tensor dq, dk, dv, far;
   at::Tensor delta = at::empty_like(lse);
-  p.lse = lse.data_ptr<float>();
+  p.neg_lse = lse.data_ptr<float>();
   p.out_low = low.data_ptr();
-  p.delta = delta.data_ptr<float>();
+  p.neg_delta = delta.data_ptr<float>();
   C10_CUDA_CHECK(attn::row_sums(bf16, out.data_ptr(), dout.data_ptr(), p, stream()));
   count_launches(1);
   if (want_kv) {

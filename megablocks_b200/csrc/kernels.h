@@ -136,9 +136,11 @@ struct Params {
   int window, sinks;                   // 1 <= window <= seq, 0 <= sinks <= seq
   const int* lengths;                  // [batch] valid tokens, nullable (all of them)
   float scale;                         // of the scores
-  float* lse;                          // [batch, heads, seq_pad] base-2 log-sum-exp of the scaled scores
+  // Per-row statistics, negative because that is how they are added: base-2 log-sum-exp of the scaled scores
+  // (infinite behind a sequence's end) and sum over dim of dout * (out + out_low), [batch, heads, seq_pad].
+  float* neg_lse;
+  float* neg_delta;
   void* out_low;                       // nullable: what the rounding of `out` left, [batch, seq, heads, dim]
-  float* delta;                        // [batch, heads, seq_pad] sum over dim of dout * (out + out_low)
   int seq_pad;
   // Backward pass over the keys: queries a window away from the first tokens are split into `far_splits`
   // parts of `far_tiles` tiles, whose shares of the first tokens' gradients are summed afterwards.

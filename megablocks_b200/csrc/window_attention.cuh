@@ -18,6 +18,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float2 splat2(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 pair_of(uint32_t lo, uint32_t hi) {
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(exp2_approx(x.x), exp2_approx(x.y)); }
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -60,6 +66,12 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int lane) {
       *reinterpret_cast<uint4*>(tile + box * (ROWS * 128) + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
+}
+
+// Columns 32 c to 32 c + 31 of an array of 32-bit registers.
+template <int N>
+__device__ __forceinline__ uint32_t (&chunk_of(uint32_t (&r)[N], int c))[32] {
+  return *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]);
 }
 
 // 32 columns of a thread's row, scaled and rounded, into a staged tile of 128 rows.

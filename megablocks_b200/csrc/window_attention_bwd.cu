@@ -10,7 +10,9 @@
 // rows on the lanes), which a group of 128 threads turns into P and dS in place; those are A operands of
 // the sums, which stay in tensor memory.  Nothing is transposed and nothing is added atomically: the scores
 // are computed once for either kernel, 7 products of a tile where one pass with atomic sums for dQ would
-// take 5, and gradients come out the same in every run.  Two groups of row threads take alternate pairs.
+// take 5, and gradients come out the same in every run.  Two groups of row threads share an SM, one taking
+// exponentials while the tensor cores work for the other: as two CTAs for heads of up to 64, as one CTA whose
+// groups take alternate pairs for larger ones (tensor memory holds no more).
 #include "window_attention.cuh"
 
 namespace mb {
@@ -18,13 +20,15 @@ namespace attn {
 
 namespace {
 
-constexpr int kThreads = 384;          // warp 0 loads, warp 1 issues MMAs, warps 4-7 and 8-11 own the rows
-
 template <int D>
 struct Layout {
+  static constexpr int kGroups = D == 128 ? 2 : 1;
+  static constexpr int kThreads = 64 + kGroups * 128;              // warp 0 loads, warp 1 issues MMAs, the others own rows
+  static constexpr int kResident = D == 128 ? 1 : 2;               // CTAs of an SM
+  static constexpr int kColumns = D == 128 ? 512 : 256;
   static constexpr int kResidentBytes = kTile * D * 2;
   static constexpr int kStreamBytes = kHalfTile * D * 2;
-  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kStages = 4;
   static constexpr int kStatBytes = 2 * kHalfTile * 4;             // lse and delta of a streamed tile's rows
   static constexpr int kBytes = 2 * kResidentBytes + kStages * (2 * kStreamBytes + kStatBytes) + 1024 + 256;
 };
@@ -39,14 +43,58 @@ struct Stream {
   }
 };
 
+// P and dS of a row's 64 pairs, in place of the two products.  Statistics and bounds of the columns in the
+// keys' kernel (`lse`, `delta` in shared memory), of the row in the queries' kernel.
+template <typename T, bool KEYS, bool EDGE>
+__device__ __forceinline__ void row_pairs(uint32_t ts, uint32_t td, float scale, const float* lse, const float* delta,
+                                          float row_lse, float row_delta, int from, int to, int keep) {
+  uint32_t s[kHalfTile], d[kHalfTile];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    tmem_ld_32x32(ts + c * 32, chunk_of(s, c));
+    tmem_ld_32x32(td + c * 32, chunk_of(d, c));
+  }
+  tmem_ld_wait();
+  const float2 scale2 = splat2(scale);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t pp[16], dd[16];
+#pragma unroll
+    for (int x = 0; x < 16; x += 2) {
+      float2 l[2] = {splat2(row_lse), splat2(row_lse)}, dl[2] = {splat2(row_delta), splat2(row_delta)};
+      if constexpr (KEYS) {
+        const float4 l4 = *reinterpret_cast<const float4*>(lse + c * 32 + 2 * x);
+        const float4 d4 = *reinterpret_cast<const float4*>(delta + c * 32 + 2 * x);
+        l[0] = make_float2(l4.x, l4.y), l[1] = make_float2(l4.z, l4.w);
+        dl[0] = make_float2(d4.x, d4.y), dl[1] = make_float2(d4.z, d4.w);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k = c * 32 + 2 * (x + u);
+        float2 pr = exp2_pair(__ffma2_rn(pair_of(s[k], s[k + 1]), scale2, l[u]));
+        float2 ds = __fmul2_rn(pr, __fadd2_rn(pair_of(d[k], d[k + 1]), dl[u]));
+        if constexpr (EDGE) {
+          if (!(k < to && (k >= from || (!KEYS && k < keep)))) pr.x = ds.x = 0.f;
+          if (!(k + 1 < to && (k + 1 >= from || (!KEYS && k + 1 < keep)))) pr.y = ds.y = 0.f;
+        }
+        if constexpr (KEYS) pp[x + u] = pack2<T>(pr.x, pr.y);
+        dd[x + u] = pack2<T>(ds.x, ds.y);
+      }
+    }
+    if constexpr (KEYS) tmem_st_32x16(ts + c * 16, pp);
+    tmem_st_32x16(td + c * 16, dd);
+  }
+  tmem_st_wait();
+}
+
 template <typename T, int D, bool KEYS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Layout<D>::kThreads, Layout<D>::kResident)
 window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_constant__ CUtensorMap map_x1,
                   const __grid_constant__ CUtensorMap map_y0, const __grid_constant__ CUtensorMap map_y1,
                   const __grid_constant__ CUtensorMap map_out0, const __grid_constant__ CUtensorMap map_out1,
                   const __grid_constant__ Params p) {
   using L = Layout<D>;
-  constexpr int kStages = L::kStages, kStream = L::kStreamBytes, kResident = L::kResidentBytes;
+  constexpr int kStages = L::kStages, kStream = L::kStreamBytes, kResident = L::kResidentBytes, G = L::kGroups;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* tile_x = smem;                                          // x0, x1
@@ -56,9 +104,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
   uint64_t* full = bars;
   uint64_t* empty = bars + kStages;
   uint64_t* x_full = bars + 2 * kStages;
-  uint64_t* s_full = x_full + 1;                   // [2] both products of a group's pair are in tensor memory
-  uint64_t* d_full = s_full + 2;                   // [2] P and dS are
-  uint64_t* acc_full = d_full + 2;
+  uint64_t* s_full = x_full + 1;                   // [G] both products of a group's pair are in tensor memory
+  uint64_t* d_full = s_full + G;                   // [G] P and dS are
+  uint64_t* acc_full = d_full + G;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -107,19 +155,23 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
     }
     mbar_init(smem_u32(x_full), 1);
     mbar_init(smem_u32(acc_full), 1);
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < G; ++g) {
       mbar_init(smem_u32(&s_full[g]), 1);
       mbar_init(smem_u32(&d_full[g]), 4);
     }
     fence_barrier_init();
+    prefetch_tensormap(&map_x0);
+    prefetch_tensormap(&map_x1);
+    prefetch_tensormap(&map_y0);
+    prefetch_tensormap(&map_y1);
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), L::kColumns);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // Group g: scores at g * 128, the other product at g * 128 + 64.  Sums: at 256 (dV, or dQ) and 256 + D (dK).
-  const uint32_t tmem_acc = tmem + 256;
+  // Group g: scores at g * 128, the other product at g * 128 + 64.  Behind them the sums: dV (or dQ), dK.
+  const uint32_t tmem_acc = tmem + G * 128;
 
   if (warp == 0) {
     // ---- loader ----------------------------------------------------------------------------------
@@ -145,8 +197,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
         if constexpr (KEYS) {
           const int64_t at = (int64_t(b) * p.heads + h) * p.seq_pad + row;
           float* s = stats + stage * 2 * kHalfTile;
-          bulk_load(smem_u32(s), p.lse + at, kHalfTile * 4, bar);
-          bulk_load(smem_u32(s + kHalfTile), p.delta + at, kHalfTile * 4, bar);
+          bulk_load(smem_u32(s), p.neg_lse + at, kHalfTile * 4, bar);
+          bulk_load(smem_u32(s + kHalfTile), p.neg_delta + at, kHalfTile * 4, bar);
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
@@ -163,59 +215,61 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
       ok = __all_sync(0xffffffffu, ok);
       tcgen05_fence_after();
     };
-    int stage = 0, old = 0;            // stage of pair t and of pair t - 1
+    int stage = 0, old = 0;            // stages of the next pair to take products of, and to sum
     uint32_t phase = 0;
-    if (st.count > 0) wait(x_full, 0);
-    for (int t = 0; t <= st.count && ok; ++t) {
-      if (t < st.count) {
-        const int g = t & 1;
-        wait(&full[stage], phase);
-        if (!ok) break;
-        uint8_t* y = ring + stage * 2 * kStream;
-        const int left = len - st.tile(t, KEYS) * kHalfTile;
-        if (left < kHalfTile) {
-          zero_rows<kHalfTile, D>(y, left, lane);
-          zero_rows<kHalfTile, D>(y + kStream, left, lane);
-        }
-        if (lane == 0) {
-          const uint32_t y0 = smem_u32(y), y1 = smem_u32(y + kStream);
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            umma_f16(tmem + g * 128, desc_along_dim<kTile>(x0, i), desc_along_dim<kHalfTile>(y0, i), idesc_s, i != 0);
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            umma_f16(tmem + g * 128 + 64, desc_along_dim<kTile>(x1, i), desc_along_dim<kHalfTile>(y1, i), idesc_s,
-                     i != 0);
-          umma_commit(smem_u32(&s_full[g]));
-        }
-        __syncwarp();
+    auto products = [&](int t) {
+      const int g = t % G;
+      wait(&full[stage], phase);
+      if (!ok) return;
+      uint8_t* y = ring + stage * 2 * kStream;
+      const int left = len - st.tile(t, KEYS) * kHalfTile;
+      if (left < kHalfTile) {
+        zero_rows<kHalfTile, D>(y, left, lane);
+        zero_rows<kHalfTile, D>(y + kStream, left, lane);
       }
-      if (t > 0) {
-        const int g = (t - 1) & 1;
-        wait(&d_full[g], ((t - 1) >> 1) & 1);
-        if (!ok) break;
-        if (lane == 0) {
-          const uint32_t y0 = smem_u32(ring + old * 2 * kStream), y1 = y0 + kStream;
-          if constexpr (KEYS) {
+      if (lane == 0) {
+        const uint32_t y0 = smem_u32(y), y1 = smem_u32(y + kStream);
 #pragma unroll
-            for (int i = 0; i < kHalfTile / 16; ++i)
-              umma_f16_ta(tmem_acc, tmem + g * 128 + i * 8, desc_along_rows<kHalfTile>(y1, i), idesc_a, t > 1 || i != 0);
-          }
+        for (int i = 0; i < D / 16; ++i)
+          umma_f16(tmem + g * 128, desc_along_dim<kTile>(x0, i), desc_along_dim<kHalfTile>(y0, i), idesc_s, i != 0);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          umma_f16(tmem + g * 128 + 64, desc_along_dim<kTile>(x1, i), desc_along_dim<kHalfTile>(y1, i), idesc_s, i != 0);
+        umma_commit(smem_u32(&s_full[g]));
+      }
+      __syncwarp();
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    };
+    auto sums = [&](int t) {
+      const int g = t % G;
+      wait(&d_full[g], (t / G) & 1);
+      if (!ok) return;
+      if (lane == 0) {
+        const uint32_t y0 = smem_u32(ring + old * 2 * kStream), y1 = y0 + kStream;
+        if constexpr (KEYS) {
 #pragma unroll
           for (int i = 0; i < kHalfTile / 16; ++i)
-            umma_f16_ta(tmem_acc + (KEYS ? D : 0), tmem + g * 128 + 64 + i * 8, desc_along_rows<kHalfTile>(y0, i),
-                        idesc_a, t > 1 || i != 0);
-          umma_commit(smem_u32(&empty[old]));
-          if (t == st.count) umma_commit(smem_u32(acc_full));
+            umma_f16_ta(tmem_acc, tmem + g * 128 + i * 8, desc_along_rows<kHalfTile>(y1, i), idesc_a, t > 0 || i != 0);
         }
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kHalfTile / 16; ++i)
+          umma_f16_ta(tmem_acc + (KEYS ? D : 0), tmem + g * 128 + 64 + i * 8, desc_along_rows<kHalfTile>(y0, i), idesc_a,
+                      t > 0 || i != 0);
+        umma_commit(smem_u32(&empty[old]));
+        if (t + 1 == st.count) umma_commit(smem_u32(acc_full));
       }
-      old = stage;
-      if (t < st.count && ++stage == kStages) { stage = 0; phase ^= 1u; }
+      __syncwarp();
+      if (++old == kStages) old = 0;
+    };
+    if (st.count > 0) wait(x_full, 0);
+    for (int t = 0; t < G && t < st.count && ok; ++t) products(t);
+    for (int t = 0; t < st.count && ok; ++t) {
+      sums(t);                         // which frees the group's place in tensor memory for the next products
+      if (ok && t + G < st.count) products(t + G);
     }
-  } else if (warp >= 4) {
+  } else {
     // ---- rows ------------------------------------------------------------------------------------
-    const int g = (warp - 4) >> 2, quarter = warp & 3;
+    const int g = (warp - 2) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane, mine = x_row + r;          // this thread's key (or query)
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t ts = tmem + g * 128 + lanes, td = ts + 64;
@@ -224,15 +278,15 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
     if constexpr (!KEYS) {
       if (mine < p.seq_pad) {
         const int64_t at = (int64_t(b) * p.heads + own_head) * p.seq_pad + mine;
-        row_lse = p.lse[at];
-        row_delta = p.delta[at];
+        row_lse = p.neg_lse[at];
+        row_delta = p.neg_delta[at];
       }
     }
     bool ok = true;
     int stage = g;
-    for (int t = g; t < st.count && ok; t += 2) {
-      while (stage >= kStages) stage -= kStages;
-      ok = mbar_wait(smem_u32(&s_full[g]), (t >> 1) & 1, abort_flag, p.status, kErrRows, kWaitNs);
+    for (int t = g; t < st.count && ok; t += G) {
+      if (stage >= kStages) stage -= kStages;
+      ok = mbar_wait(smem_u32(&s_full[g]), (t / G) & 1, abort_flag, p.status, kErrRows, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
@@ -257,96 +311,68 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
         edge = y_row + kHalfTile - 1 > x_row || (x_row + kTile - 1) - y_row >= p.window || x_row + kTile > len;
       }
       const float* col_lse = stats + stage * 2 * kHalfTile;
-      const float* col_delta = col_lse + kHalfTile;
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], d[32];
-        tmem_ld_32x32(ts + c * 32, s);
-        tmem_ld_32x32(td + c * 32, d);
-        tmem_ld_wait();
-        uint32_t pp[16], dd[16];
-#pragma unroll
-        for (int x = 0; x < 32; x += 2) {
-          float pr[2], ds[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int k = c * 32 + x + u;
-            const float lse = KEYS ? col_lse[k] : row_lse, delta = KEYS ? col_delta[k] : row_delta;
-            pr[u] = exp2_approx(fmaf(__uint_as_float(s[x + u]), scale, -lse));
-            ds[u] = pr[u] * (__uint_as_float(d[x + u]) - delta);
-            if (edge && !(k < to && (k >= from || (!KEYS && k < keep)))) pr[u] = ds[u] = 0.f;
-          }
-          if constexpr (KEYS) pp[x / 2] = pack2<T>(pr[0], pr[1]);
-          dd[x / 2] = pack2<T>(ds[0], ds[1]);
-        }
-        if constexpr (KEYS) tmem_st_32x16(ts + c * 16, pp);
-        tmem_st_32x16(td + c * 16, dd);
-      }
-      tmem_st_wait();
+      if (edge)
+        row_pairs<T, KEYS, true>(ts, td, scale, col_lse, col_lse + kHalfTile, row_lse, row_delta, from, to, keep);
+      else
+        row_pairs<T, KEYS, false>(ts, td, scale, col_lse, col_lse + kHalfTile, row_lse, row_delta, from, to, keep);
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&d_full[g]));
-      stage += 2;
+      stage += G;
     }
     if (st.count > 0 && ok) {
       ok = mbar_wait(smem_u32(acc_full), 0, abort_flag, p.status, kErrRows, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
       tcgen05_fence_after();
     }
-    // Group 0: dV, or the first half of dQ; group 1: dK, or the other half.
-    constexpr int kChunks = KEYS ? D / 32 : D / 64;
-    const uint32_t acc = tmem_acc + lanes + (KEYS ? g * D : g * (D / 2));
-    const float factor = KEYS && g == 0 ? 1.f : p.scale;
+    // The keys' kernel has two results, dV and dK: one a group, or both of the one group.  The queries' kernel
+    // has dQ, whose columns the groups share.
     const bool some = st.count > 0 && ok;
     const bool live = some && mine < len;
-    uint8_t* staged = KEYS ? tile_x + (1 - g) * kResident : tile_x;    // all products have been taken
     // A first token whose far queries are other CTAs': this CTA's share goes to the workspace.
     const bool shared_sum = KEYS && p.far_splits > 0 && mine < p.sinks && mine < p.seq;
-    float* far = nullptr;
-    if (shared_sum)
-      far = p.far + ((((int64_t(part) * p.batch + b) * p.kv_heads + own_head) * 2 + (1 - g)) * p.sinks + mine) * p.dim;
+    constexpr int kChunks = KEYS ? D / 32 : D / 32 / G;
 #pragma unroll 1
-    for (int c = 0; c < kChunks; ++c) {
-      uint32_t raw[32];
-      if (some) {
-        tmem_ld_32x32(acc + c * 32, raw);
-        tmem_ld_wait();
-      }
-      if (!live) {
+    for (int which = KEYS ? g : 0; which < (KEYS ? 2 : 1); which += KEYS ? G : 1) {          // 0: dV (dQ), 1: dK
+      const uint32_t acc = tmem_acc + lanes + (KEYS ? which * D : g * (D / G));
+      const float factor = KEYS && which == 0 ? 1.f : p.scale;
+      uint8_t* staged = tile_x + (KEYS ? which * kResident : 0);     // all products have been taken
+      float* far = nullptr;
+      if (shared_sum)
+        far = p.far + ((((int64_t(part) * p.batch + b) * p.kv_heads + own_head) * 2 + (1 - which)) * p.sinks + mine) * p.dim;
+#pragma unroll 1
+      for (int c = 0; c < kChunks; ++c) {
+        uint32_t raw[32];
+        if (some) {
+          tmem_ld_32x32(acc + c * 32, raw);
+          tmem_ld_wait();
+        }
+        if (!live) {
 #pragma unroll
-        for (int x = 0; x < 32; ++x) raw[x] = 0u;
-      }
-      if (far != nullptr) {
+          for (int x = 0; x < 32; ++x) raw[x] = 0u;
+        }
+        if (far != nullptr) {
 #pragma unroll
-        for (int x = 0; x < 32; x += 4)
-          if (c * 32 + x < p.dim)
-            *reinterpret_cast<float4*>(far + c * 32 + x) =
-                make_float4(__uint_as_float(raw[x]) * factor, __uint_as_float(raw[x + 1]) * factor,
-                            __uint_as_float(raw[x + 2]) * factor, __uint_as_float(raw[x + 3]) * factor);
+          for (int x = 0; x < 32; x += 4)
+            if (c * 32 + x < p.dim)
+              *reinterpret_cast<float4*>(far + c * 32 + x) =
+                  make_float4(__uint_as_float(raw[x]) * factor, __uint_as_float(raw[x + 1]) * factor,
+                              __uint_as_float(raw[x + 2]) * factor, __uint_as_float(raw[x + 3]) * factor);
+        }
+        if (part == 0) stage_row<T>(staged, r, KEYS ? c : g * kChunks + c, raw, factor);
       }
-      if (part == 0) stage_row<T>(staged, r, KEYS ? c : g * kChunks + c, raw, factor);
-    }
-    fence_proxy_async_smem();
-    if (KEYS) {
-      group_barrier(1 + g);
-      if (part == 0 && quarter == 0 && lane == 0 && x_row < p.seq) {
+      fence_proxy_async_smem();
+      if (KEYS || G == 1) group_barrier(1 + g);
+      else asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (part == 0 && (KEYS || g == 0) && quarter == 0 && lane == 0 && x_row < p.seq) {
         for (int box = 0; box < D / 64; ++box)
           if (box * 64 < p.dim)
-            tma_store_4d(g == 0 ? &map_out1 : &map_out0, smem_u32(staged + box * (kTile * 128)), box * 64, x_row,
-                         own_head, b);
+            tma_store_4d(KEYS && which == 0 ? &map_out1 : &map_out0, smem_u32(staged + box * (kTile * 128)), box * 64,
+                         x_row, own_head, b);
         bulk_commit_group();
-        bulk_wait_read_all();
-      }
-    } else {
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (g == 0 && quarter == 0 && lane == 0 && x_row < p.seq) {
-        for (int box = 0; box < D / 64; ++box)
-          if (box * 64 < p.dim)
-            tma_store_4d(&map_out0, smem_u32(staged + box * (kTile * 128)), box * 64, x_row, own_head, b);
-        bulk_commit_group();
-        bulk_wait_read_all();
       }
     }
+    if (quarter == 0 && lane == 0) bulk_wait_read_all();
     __syncwarp();
   }
   tcgen05_fence_before();
@@ -354,7 +380,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
   if (warp == 1) {
     settle(abort_flag);
     tcgen05_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, L::kColumns);
   }
 }
 
@@ -379,7 +405,7 @@ row_sums_kernel(const T* __restrict__ out, const T* __restrict__ low, const T* _
   }
 #pragma unroll
   for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) p.delta[(int64_t(b) * p.heads + h) * p.seq_pad + i] = sum;
+  if (lane == 0) p.neg_delta[(int64_t(b) * p.heads + h) * p.seq_pad + i] = -sum;
 }
 
 // One warp a first token of a key head: its parts in order, rounded once.
@@ -412,7 +438,7 @@ cudaError_t launch_backward(const CUtensorMap& x0, const CUtensorMap& x1, const 
   if (rc != cudaSuccess) return rc;
   const int far = KEYS ? p.far_splits * ((p.sinks + kTile - 1) / kTile) : 0;
   const dim3 grid((KEYS ? p.kv_heads : p.heads) * p.batch, far + (p.seq + kTile - 1) / kTile);
-  kernel<<<grid, kThreads, Layout<D>::kBytes, stream>>>(x0, x1, y0, y1, o0, o1, p);
+  kernel<<<grid, Layout<D>::kThreads, Layout<D>::kBytes, stream>>>(x0, x1, y0, y1, o0, o1, p);
   return cudaGetLastError();
 }
 
