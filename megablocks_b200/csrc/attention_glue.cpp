@@ -123,6 +123,7 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
   TORCH_CHECK(lse.device() == q.device() && lse.is_contiguous() && lse.scalar_type() == at::kFloat &&
                   lse.numel() == int64_t(p.batch) * p.heads * p.seq_pad, "window_attention: bad log-sum-exp");
   const bool bf16 = q.scalar_type() == at::kBFloat16;
+  const int rows = attn::streamed_rows(p.dim);
   at::Tensor dq, dk, dv, far;
   at::Tensor delta = at::empty_like(lse);
   p.neg_lse = lse.data_ptr<float>();
@@ -136,18 +137,17 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
     if (p.sinks > 0) {
       // Every query sees the first tokens: their tile's stream is as long as the sequence, the others' a
       // window.  What exceeds that is split into parts of a window's length.
-      const int half = attn::kHalfTile;
-      const int usual = (p.window + attn::kTile + half - 1) / half;
-      const int far_tiles = std::max(0, (p.seq + half - 1) / half - usual);
+      const int usual = (p.window + attn::kTile + rows - 1) / rows;
+      const int far_tiles = std::max(0, (p.seq + rows - 1) / rows - usual);
       if (far_tiles > usual / 2) {
-        p.far_tiles = std::max({usual, 16, (far_tiles + 63) / 64});
+        p.far_tiles = std::max({usual, 1024 / rows, (far_tiles + 63) / 64});
         p.far_splits = (far_tiles + p.far_tiles - 1) / p.far_tiles;
         far = at::empty({p.far_splits + 1, p.batch, p.kv_heads, 2, p.sinks, p.dim}, lse.options());
         p.far = far.data_ptr<float>();
       }
     }
     C10_CUDA_CHECK(attn::backward_keys(bf16, make_map(k, attn::kTile), make_map(v, attn::kTile),
-                                       make_map(q, attn::kHalfTile), make_map(dout, attn::kHalfTile),
+                                       make_map(q, rows), make_map(dout, rows),
                                        make_map(dk, attn::kTile), make_map(dv, attn::kTile), p, stream()));
     count_launches(1);
     if (p.far_splits > 0) {
@@ -158,7 +158,7 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
   if (want_q) {
     dq = at::empty({p.batch, p.seq, p.heads, p.dim}, q.options());
     C10_CUDA_CHECK(attn::backward_queries(bf16, make_map(q, attn::kTile), make_map(dout, attn::kTile),
-                                          make_map(k, attn::kHalfTile), make_map(v, attn::kHalfTile),
+                                          make_map(k, rows), make_map(v, rows),
                                           make_map(dq, attn::kTile), p, stream()));
     count_launches(1);
   }

@@ -127,7 +127,8 @@ cudaError_t scale_unless_one(DType type, void* x, int64_t numel, const float* fa
 namespace attn {
 
 constexpr int kTile = 128;             // rows of a resident tile, keys of a streamed one in the forward pass
-constexpr int kHalfTile = 64;          // rows of a streamed tile in the backward pass
+// Rows of a streamed tile in the backward pass.
+constexpr int streamed_rows(int dim) { return dim > 64 ? 128 : 64; }
 constexpr int kPadRows = 256;          // per-row statistics are padded to a multiple of this
 constexpr int kErrLoad = 48, kErrMma = 49, kErrRows = 50;
 
@@ -153,12 +154,12 @@ cudaError_t forward(bool bf16, const CUtensorMap& q, const CUtensorMap& k, const
                     const CUtensorMap& out, const CUtensorMap& out_low, const Params& params, cudaStream_t stream);
 // delta, and zeros behind the sequences' ends.
 cudaError_t row_sums(bool bf16, const void* out, const void* dout, const Params& params, cudaStream_t stream);
-// Maps with 128-row boxes (`q`, `k`, ...: resident tiles and results) and 64-row boxes (`q_half`, ...: streamed).
-cudaError_t backward_keys(bool bf16, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q_half,
-                          const CUtensorMap& dout_half, const CUtensorMap& dk, const CUtensorMap& dv,
+// Maps with 128-row boxes (`q`, `k`, ...: resident tiles and results) and of streamed tiles (`q_stream`, ...).
+cudaError_t backward_keys(bool bf16, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q_stream,
+                          const CUtensorMap& dout_stream, const CUtensorMap& dk, const CUtensorMap& dv,
                           const Params& params, cudaStream_t stream);
-cudaError_t backward_queries(bool bf16, const CUtensorMap& q, const CUtensorMap& dout, const CUtensorMap& k_half,
-                             const CUtensorMap& v_half, const CUtensorMap& dq, const Params& params,
+cudaError_t backward_queries(bool bf16, const CUtensorMap& q, const CUtensorMap& dout, const CUtensorMap& k_stream,
+                             const CUtensorMap& v_stream, const CUtensorMap& dq, const Params& params,
                              cudaStream_t stream);
 // The first tokens' gradients from the parts of `far`.
 cudaError_t sum_far(bool bf16, void* dk, void* dv, const Params& params, cudaStream_t stream);

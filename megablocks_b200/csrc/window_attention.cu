@@ -189,6 +189,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // ---- MMA issuer ------------------------------------------------------------------------------
     constexpr uint32_t idesc_s = instr_desc_f16(kIsBf16<T>, false, false, kTile, kTile);
     constexpr uint32_t idesc_o = instr_desc_f16(kIsBf16<T>, false, true, kTile, D);
+    const uint32_t q_base = uniform(smem_u32(tile_q)), ring_base = uniform(smem_u32(ring)), ts = uniform(tmem_s),
+                   to = uniform(tmem_o);
     int stage = 0;
     uint32_t phase = 0, p_phase[G] = {};
     bool started[G] = {}, ok = true;
@@ -201,11 +203,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       tcgen05_fence_after();
     };
     auto scores = [&](int g) {         // S_g = Q_g K^T with K in the current stage
-      if (lane == 0) {
-        const uint32_t q = smem_u32(tile_q + g * kTileBytes), k = smem_u32(ring + stage * kTileBytes);
+      if (elect_one()) {
+        const uint32_t q = q_base + g * kTileBytes, k = ring_base + stage * kTileBytes;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
-          umma_f16(tmem_s + g * kTile, desc_along_dim<kTile>(q, i), desc_along_dim<kTile>(k, i), idesc_s, i != 0);
+          umma_f16(ts + g * kTile, desc_along_dim<kTile>(q, i), desc_along_dim<kTile>(k, i), idesc_s, i != 0);
         umma_commit(smem_u32(&s_full[g]));
       }
       __syncwarp();
@@ -218,7 +220,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         wait(&q_full[g], 0);
         if (ok) scores(g);
       }
-      if (lane == 0 && ok) umma_commit(smem_u32(&empty[stage]));
+      if (ok && elect_one()) umma_commit(smem_u32(&empty[stage]));
+      __syncwarp();
       next();
     }
     for (int t = 0; t < tiles.count && ok; ++t) {
@@ -236,11 +239,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (ok && tiles.wanted(g, j)) {
           wait(&p_full[g], p_phase[g]);
           p_phase[g] ^= 1u;
-          if (ok && lane == 0) {
-            const uint32_t v = smem_u32(ring + v_stage * kTileBytes);
+          if (ok && elect_one()) {
+            const uint32_t v = ring_base + v_stage * kTileBytes;
 #pragma unroll
             for (int i = 0; i < kTile / 16; ++i)
-              umma_f16_ta(tmem_o + g * D, tmem_s + g * kTile + i * 8, desc_along_rows<kTile>(v, i), idesc_o,
+              umma_f16_ta(to + g * D, ts + g * kTile + i * 8, desc_along_rows<kTile>(v, i), idesc_o,
                           started[g] || i != 0);
             if (j == tiles.hi[g]) umma_commit(smem_u32(&o_full[g]));
           }
@@ -252,7 +255,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (ok) scores(g);
         }
       }
-      if (lane == 0 && ok) {
+      if (ok && elect_one()) {
         umma_commit(smem_u32(&empty[v_stage]));
         if (more) umma_commit(smem_u32(&empty[stage]));
       }

@@ -45,15 +45,19 @@ __device__ __forceinline__ int length_of(const Params& p, int b) {
   return p.lengths == nullptr ? p.seq : max(0, min(p.seq, p.lengths[b]));
 }
 
+// A value that all lanes have, in a uniform register: what an MMA's descriptors are made of.  From ordinary
+// registers each descriptor is moved there again, which took longer than the MMA itself.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // Tiles are stored as D / 64 boxes of [rows][64] 16-bit values with 128-byte swizzle: one layout that
 // serves as a K-major operand (contraction along dim) and as an MN-major one (contraction along the rows).
 template <int ROWS>
 __device__ __forceinline__ uint64_t desc_along_dim(uint32_t tile, int k) {      // k-th 16 of dim
-  return smem_desc_sw128(tile + (k >> 2) * (ROWS * 128) + (k & 3) * 32, 16, 1024);
+  return smem_desc_sw128(tile, 16, 1024) + (((k >> 2) * (ROWS * 128) + (k & 3) * 32) >> 4);
 }
 template <int ROWS>
 __device__ __forceinline__ uint64_t desc_along_rows(uint32_t tile, int k) {     // k-th 16 of the rows
-  return smem_desc_sw128(tile + k * 2048, ROWS * 128, 1024);
+  return smem_desc_sw128(tile, ROWS * 128, 1024) + ((k * 2048) >> 4);
 }
 
 // Rows [first, ROWS) of a tile set to zero by one warp, visible to the tensor cores afterwards: what lies

@@ -3,16 +3,20 @@
 //   P_ij  = exp(scale q_i k_j - lse_i)             dS_ij = P_ij (dO_i v_j - delta_i),  delta_i = dO_i O_i
 //   dV_j  = sum_i P_ij dO_i     dK_j = scale sum_i dS_ij q_i     dQ_i = scale sum_j dS_ij k_j
 //
-// Two kernels of one shape.  A CTA holds two resident tiles of 128 rows and streams pairs of 64-row tiles
-// past them: the keys' kernel holds K and V and streams Q and dO of every query head that shares them (so
-// the heads' gradients are summed where they are made, in a fixed order), the queries' kernel holds Q and dO
-// and streams K and V.  Each pair gives two products in tensor memory (scores and dO V^T, with the resident
-// rows on the lanes), which a group of 128 threads turns into P and dS in place; those are A operands of
-// the sums, which stay in tensor memory.  Nothing is transposed and nothing is added atomically: the scores
-// are computed once for either kernel, 7 products of a tile where one pass with atomic sums for dQ would
-// take 5, and gradients come out the same in every run.  Two groups of row threads share an SM, one taking
-// exponentials while the tensor cores work for the other: as two CTAs for heads of up to 64, as one CTA whose
-// groups take alternate pairs for larger ones (tensor memory holds no more).
+// Two kernels of one shape.  A CTA holds two resident tiles of 128 rows and streams pairs of tiles past them:
+// the keys' kernel holds K and V and streams Q and dO of every query head that shares them (so the heads'
+// gradients are summed where they are made, in a fixed order), the queries' kernel holds Q and dO and streams
+// K and V.  Each pair gives two products in tensor memory (scores and dO V^T, with the resident rows on the
+// lanes), which the row threads, 64 columns of a row each, turn into P and dS in place; those are A operands
+// of the sums, which stay in tensor memory.  Nothing is transposed and nothing is added atomically: the scores
+// are computed once for either kernel, 7 products of a tile where one pass with atomic sums for dQ would take
+// 5, and gradients come out the same in every run.
+//
+// The two products are handled one after the other, so that the tensor cores always have the other half to
+// do: while the rows take exponentials of scores t, the sum with dS t - 1 and product t of dO V^T run; while they
+// make dS t, the sum with P t and scores t + 1.  Heads of up to 64 leave room for two CTAs on an SM with
+// streamed tiles of 64 rows; larger ones fill tensor memory with one, whose streamed tiles have 128 rows:
+// with 64, reading the resident operand from shared memory again for half the columns set the pace.
 #include "window_attention.cuh"
 
 namespace mb {
@@ -22,14 +26,14 @@ namespace {
 
 template <int D>
 struct Layout {
-  static constexpr int kGroups = D == 128 ? 2 : 1;
-  static constexpr int kThreads = 64 + kGroups * 128;              // warp 0 loads, warp 1 issues MMAs, the others own rows
+  static constexpr int kRows = D == 128 ? 128 : 64;                // rows of a streamed tile
+  static constexpr int kThreads = 64 + kRows * 2;                  // warp 0 loads, warp 1 issues MMAs, the others own rows
   static constexpr int kResident = D == 128 ? 1 : 2;               // CTAs of an SM
-  static constexpr int kColumns = D == 128 ? 512 : 256;
+  static constexpr int kColumns = D == 128 ? 512 : 256;            // scores, other product, two sums
   static constexpr int kResidentBytes = kTile * D * 2;
-  static constexpr int kStreamBytes = kHalfTile * D * 2;
-  static constexpr int kStages = 4;
-  static constexpr int kStatBytes = 2 * kHalfTile * 4;             // lse and delta of a streamed tile's rows
+  static constexpr int kStreamBytes = kRows * D * 2;
+  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kStatBytes = 2 * kRows * 4;                 // lse and delta of a streamed tile's rows
   static constexpr int kBytes = 2 * kResidentBytes + kStages * (2 * kStreamBytes + kStatBytes) + 1024 + 256;
 };
 
@@ -43,48 +47,76 @@ struct Stream {
   }
 };
 
-// P and dS of a row's 64 pairs, in place of the two products.  Statistics and bounds of the columns in the
-// keys' kernel (`lse`, `delta` in shared memory), of the row in the queries' kernel.
+// Whether pair k of a row's 64 is visible: [from, to), and in the queries' kernel also [0, keep) below `to`.
+struct Seen {
+  int from, to, keep;
+  template <bool KEYS>
+  __device__ __forceinline__ bool at(int k) const { return k < to && (k >= from || (!KEYS && k < keep)); }
+};
+
+// Exponentials of a row's 64 scores; in the keys' kernel also rounded over the scores.  The statistics are the
+// columns' in the keys' kernel (in shared memory), the row's in the queries'.
 template <typename T, bool KEYS, bool EDGE>
-__device__ __forceinline__ void row_pairs(uint32_t ts, uint32_t td, float scale, const float* lse, const float* delta,
-                                          float row_lse, float row_delta, int from, int to, int keep) {
-  uint32_t s[kHalfTile], d[kHalfTile];
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    tmem_ld_32x32(ts + c * 32, chunk_of(s, c));
-    tmem_ld_32x32(td + c * 32, chunk_of(d, c));
-  }
-  tmem_ld_wait();
+__device__ __forceinline__ void row_exp(const uint32_t (&s)[64], uint32_t ts, float scale, const float* col, float row,
+                                        const Seen& seen, float2 (&pr)[32]) {
   const float2 scale2 = splat2(scale);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t pp[16], dd[16];
+    uint32_t packed[16];
 #pragma unroll
     for (int x = 0; x < 16; x += 2) {
-      float2 l[2] = {splat2(row_lse), splat2(row_lse)}, dl[2] = {splat2(row_delta), splat2(row_delta)};
+      float2 l[2] = {splat2(row), splat2(row)};
       if constexpr (KEYS) {
-        const float4 l4 = *reinterpret_cast<const float4*>(lse + c * 32 + 2 * x);
-        const float4 d4 = *reinterpret_cast<const float4*>(delta + c * 32 + 2 * x);
+        const float4 l4 = *reinterpret_cast<const float4*>(col + c * 32 + 2 * x);
         l[0] = make_float2(l4.x, l4.y), l[1] = make_float2(l4.z, l4.w);
-        dl[0] = make_float2(d4.x, d4.y), dl[1] = make_float2(d4.z, d4.w);
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int k = c * 32 + 2 * (x + u);
-        float2 pr = exp2_pair(__ffma2_rn(pair_of(s[k], s[k + 1]), scale2, l[u]));
-        float2 ds = __fmul2_rn(pr, __fadd2_rn(pair_of(d[k], d[k + 1]), dl[u]));
+        float2 e = exp2_pair(__ffma2_rn(pair_of(s[k], s[k + 1]), scale2, l[u]));
         if constexpr (EDGE) {
-          if (!(k < to && (k >= from || (!KEYS && k < keep)))) pr.x = ds.x = 0.f;
-          if (!(k + 1 < to && (k + 1 >= from || (!KEYS && k + 1 < keep)))) pr.y = ds.y = 0.f;
+          if (!seen.at<KEYS>(k)) e.x = 0.f;
+          if (!seen.at<KEYS>(k + 1)) e.y = 0.f;
         }
-        if constexpr (KEYS) pp[x + u] = pack2<T>(pr.x, pr.y);
-        dd[x + u] = pack2<T>(ds.x, ds.y);
+        pr[c * 16 + x + u] = e;
+        if constexpr (KEYS) packed[x + u] = pack2<T>(e.x, e.y);
       }
     }
-    if constexpr (KEYS) tmem_st_32x16(ts + c * 16, pp);
-    tmem_st_32x16(td + c * 16, dd);
+    if constexpr (KEYS) tmem_st_32x16(ts + c * 16, packed);
   }
-  tmem_st_wait();
+}
+
+// dS over the other product.  P = 0 does not do for hidden pairs, whose product may be infinite or NaN.
+template <typename T, bool KEYS, bool EDGE>
+__device__ __forceinline__ void row_ds(uint32_t td, const float* col, float row, const Seen& seen,
+                                       const float2 (&pr)[32]) {
+  uint32_t d[64];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) tmem_ld_32x32(td + c * 32, chunk_of(d, c));
+  tmem_ld_wait();
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int x = 0; x < 16; x += 2) {
+      float2 l[2] = {splat2(row), splat2(row)};
+      if constexpr (KEYS) {
+        const float4 l4 = *reinterpret_cast<const float4*>(col + c * 32 + 2 * x);
+        l[0] = make_float2(l4.x, l4.y), l[1] = make_float2(l4.z, l4.w);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k = c * 32 + 2 * (x + u);
+        float2 ds = __fmul2_rn(pr[c * 16 + x + u], __fadd2_rn(pair_of(d[k], d[k + 1]), l[u]));
+        if constexpr (EDGE) {
+          if (!seen.at<KEYS>(k)) ds.x = 0.f;
+          if (!seen.at<KEYS>(k + 1)) ds.y = 0.f;
+        }
+        packed[x + u] = pack2<T>(ds.x, ds.y);
+      }
+    }
+    tmem_st_32x16(td + c * 16, packed);
+  }
 }
 
 template <typename T, int D, bool KEYS>
@@ -94,19 +126,22 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
                   const __grid_constant__ CUtensorMap map_out0, const __grid_constant__ CUtensorMap map_out1,
                   const __grid_constant__ Params p) {
   using L = Layout<D>;
-  constexpr int kStages = L::kStages, kStream = L::kStreamBytes, kResident = L::kResidentBytes, G = L::kGroups;
+  constexpr int kStages = L::kStages, kStream = L::kStreamBytes, kResident = L::kResidentBytes, R = L::kRows;
+  constexpr int kRowWarps = R / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* tile_x = smem;                                          // x0, x1
   uint8_t* ring = smem + 2 * kResident;                            // [stage]: y0, y1
-  float* stats = reinterpret_cast<float*>(ring + kStages * 2 * kStream);       // [stage]: lse, delta
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + kStages * 2 * kHalfTile);
+  float* stats = reinterpret_cast<float*>(ring + kStages * 2 * kStream);       // [stage]: lse, delta of the R rows
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + kStages * 2 * R);
   uint64_t* full = bars;
   uint64_t* empty = bars + kStages;
   uint64_t* x_full = bars + 2 * kStages;
-  uint64_t* s_full = x_full + 1;                   // [G] both products of a group's pair are in tensor memory
-  uint64_t* d_full = s_full + G;                   // [G] P and dS are
-  uint64_t* acc_full = d_full + G;
+  uint64_t* s_full = x_full + 1;                   // scores are in tensor memory
+  uint64_t* d_full = s_full + 1;                   // the other product is
+  uint64_t* p_done = d_full + 1;                   // P is there (queries' kernel: the scores have been read)
+  uint64_t* ds_done = p_done + 1;                  // dS is there
+  uint64_t* acc_full = ds_done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -124,11 +159,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
 
   Stream st{0, 1, 0, 0};
   if (x_row < len) {
-    const int tiles = (len + kHalfTile - 1) / kHalfTile;
+    const int tiles = (len + R - 1) / R;
     if constexpr (KEYS) {
       // Queries from the tile's own on; up to a window behind its last key, or all for first tokens.
-      const int near = int(min(int64_t(tiles), (int64_t(x_row) + kTile + p.window - 2) / kHalfTile + 1));
-      st.lo = x_row / kHalfTile;
+      const int near = int(min(int64_t(tiles), (int64_t(x_row) + kTile + p.window - 2) / R + 1));
+      st.lo = x_row / R;
       int hi = near;
       if (x_row < p.sinks) {
         if (p.far_splits == 0) hi = tiles;
@@ -140,9 +175,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
       st.per_head = max(0, hi - st.lo);
       st.count = st.per_head * ratio;
     } else {
-      st.lo = max(0, x_row - p.window + 1) / kHalfTile;
-      st.head_tiles = min((p.sinks + kHalfTile - 1) / kHalfTile, st.lo);
-      st.count = st.head_tiles + (min(x_row + kTile, len) - 1) / kHalfTile - st.lo + 1;
+      st.lo = max(0, x_row - p.window + 1) / R;
+      st.head_tiles = min((p.sinks + R - 1) / R, st.lo);
+      st.count = st.head_tiles + (min(x_row + kTile, len) - 1) / R - st.lo + 1;
     }
   }
   auto stream_head = [&](int t) { return KEYS ? own_head * ratio + t / st.per_head : own_head / ratio; };
@@ -154,11 +189,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
       mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(x_full), 1);
+    mbar_init(smem_u32(s_full), 1);
+    mbar_init(smem_u32(d_full), 1);
+    mbar_init(smem_u32(p_done), kRowWarps);
+    mbar_init(smem_u32(ds_done), kRowWarps);
     mbar_init(smem_u32(acc_full), 1);
-    for (int g = 0; g < G; ++g) {
-      mbar_init(smem_u32(&s_full[g]), 1);
-      mbar_init(smem_u32(&d_full[g]), 4);
-    }
     fence_barrier_init();
     prefetch_tensormap(&map_x0);
     prefetch_tensormap(&map_x1);
@@ -170,8 +205,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // Group g: scores at g * 128, the other product at g * 128 + 64.  Behind them the sums: dV (or dQ), dK.
-  const uint32_t tmem_acc = tmem + G * 128;
+  // Scores, the other product, and the sums: dV (or dQ), dK.
+  const uint32_t tmem_d = tmem + R, tmem_acc = tmem + 2 * R;
 
   if (warp == 0) {
     // ---- loader ----------------------------------------------------------------------------------
@@ -187,18 +222,18 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
       for (int t = 0; t < st.count; ++t) {
         if (!mbar_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.status, kErrLoad, kWaitNs)) break;
         const uint32_t bar = smem_u32(&full[stage]);
-        const int row = st.tile(t, KEYS) * kHalfTile, h = stream_head(t);
+        const int row = st.tile(t, KEYS) * R, h = stream_head(t);
         uint8_t* y = ring + stage * 2 * kStream;
         mbar_arrive_expect_tx(bar, 2 * kStream + (KEYS ? L::kStatBytes : 0));
-        for (int box = 0; box < D / 64; ++box) {
-          tma_load_4d(smem_u32(y + box * (kHalfTile * 128)), &map_y0, bar, box * 64, row, h, b);
-          tma_load_4d(smem_u32(y + kStream + box * (kHalfTile * 128)), &map_y1, bar, box * 64, row, h, b);
-        }
+        for (int box = 0; box < D / 64; ++box)
+          tma_load_4d(smem_u32(y + box * (R * 128)), &map_y0, bar, box * 64, row, h, b);
+        for (int box = 0; box < D / 64; ++box)
+          tma_load_4d(smem_u32(y + kStream + box * (R * 128)), &map_y1, bar, box * 64, row, h, b);
         if constexpr (KEYS) {
           const int64_t at = (int64_t(b) * p.heads + h) * p.seq_pad + row;
-          float* s = stats + stage * 2 * kHalfTile;
-          bulk_load(smem_u32(s), p.neg_lse + at, kHalfTile * 4, bar);
-          bulk_load(smem_u32(s + kHalfTile), p.neg_delta + at, kHalfTile * 4, bar);
+          float* s = stats + stage * 2 * R;
+          bulk_load(smem_u32(s), p.neg_lse + at, R * 4, bar);
+          bulk_load(smem_u32(s + R), p.neg_delta + at, R * 4, bar);
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
@@ -206,127 +241,161 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
     __syncwarp();
   } else if (warp == 1) {
     // ---- MMA issuer ------------------------------------------------------------------------------
-    constexpr uint32_t idesc_s = instr_desc_f16(kIsBf16<T>, false, false, kTile, kHalfTile);
+    constexpr uint32_t idesc_s = instr_desc_f16(kIsBf16<T>, false, false, kTile, R);
     constexpr uint32_t idesc_a = instr_desc_f16(kIsBf16<T>, false, true, kTile, D);
-    const uint32_t x0 = smem_u32(tile_x), x1 = smem_u32(tile_x + kResident);
+    const uint32_t x0 = uniform(smem_u32(tile_x)), x1 = x0 + kResident, y_base = uniform(smem_u32(ring));
+    const uint32_t ts = uniform(tmem), td = ts + R, ta = ts + 2 * R;
+    // P and dS of 64 columns take the first 32 of the columns that their products took.
+    auto at = [](int i) { return (i / 4) * 64 + (i % 4) * 8; };
     bool ok = true;
+    int stage = 0, next = 0;           // stages of pair t and of pair t + 1
+    uint32_t next_phase = 0;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       ok = ok && mbar_wait(smem_u32(bar), parity, abort_flag, p.status, kErrMma, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
       tcgen05_fence_after();
     };
-    int stage = 0, old = 0;            // stages of the next pair to take products of, and to sum
-    uint32_t phase = 0;
-    auto products = [&](int t) {
-      const int g = t % G;
-      wait(&full[stage], phase);
+    // Products of the resident tiles with the streamed ones of stage `next`.
+    auto scores = [&](int t) {
+      wait(&full[next], next_phase);
       if (!ok) return;
-      uint8_t* y = ring + stage * 2 * kStream;
-      const int left = len - st.tile(t, KEYS) * kHalfTile;
-      if (left < kHalfTile) {
-        zero_rows<kHalfTile, D>(y, left, lane);
-        zero_rows<kHalfTile, D>(y + kStream, left, lane);
+      const int left = len - st.tile(t, KEYS) * R;
+      if (left < R) {
+        uint8_t* y = ring + next * 2 * kStream;
+        zero_rows<R, D>(y, left, lane);
+        zero_rows<R, D>(y + kStream, left, lane);
       }
-      if (lane == 0) {
-        const uint32_t y0 = smem_u32(y), y1 = smem_u32(y + kStream);
+      if (elect_one()) {
+        const uint32_t y0 = y_base + next * 2 * kStream;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
-          umma_f16(tmem + g * 128, desc_along_dim<kTile>(x0, i), desc_along_dim<kHalfTile>(y0, i), idesc_s, i != 0);
+          umma_f16(ts, desc_along_dim<kTile>(x0, i), desc_along_dim<R>(y0, i), idesc_s, i != 0);
+        umma_commit(smem_u32(s_full));
+      }
+      __syncwarp();
+    };
+    auto other = [&] {
+      if (elect_one()) {
+        const uint32_t y1 = y_base + next * 2 * kStream + kStream;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
-          umma_f16(tmem + g * 128 + 64, desc_along_dim<kTile>(x1, i), desc_along_dim<kHalfTile>(y1, i), idesc_s, i != 0);
-        umma_commit(smem_u32(&s_full[g]));
+          umma_f16(td, desc_along_dim<kTile>(x1, i), desc_along_dim<R>(y1, i), idesc_s, i != 0);
+        umma_commit(smem_u32(d_full));
       }
       __syncwarp();
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
     };
-    auto sums = [&](int t) {
-      const int g = t % G;
-      wait(&d_full[g], (t / G) & 1);
-      if (!ok) return;
-      if (lane == 0) {
-        const uint32_t y0 = smem_u32(ring + old * 2 * kStream), y1 = y0 + kStream;
-        if constexpr (KEYS) {
-#pragma unroll
-          for (int i = 0; i < kHalfTile / 16; ++i)
-            umma_f16_ta(tmem_acc, tmem + g * 128 + i * 8, desc_along_rows<kHalfTile>(y1, i), idesc_a, t > 0 || i != 0);
-        }
-#pragma unroll
-        for (int i = 0; i < kHalfTile / 16; ++i)
-          umma_f16_ta(tmem_acc + (KEYS ? D : 0), tmem + g * 128 + 64 + i * 8, desc_along_rows<kHalfTile>(y0, i), idesc_a,
-                      t > 0 || i != 0);
-        umma_commit(smem_u32(&empty[old]));
-        if (t + 1 == st.count) umma_commit(smem_u32(acc_full));
-      }
-      __syncwarp();
-      if (++old == kStages) old = 0;
-    };
-    if (st.count > 0) wait(x_full, 0);
-    for (int t = 0; t < G && t < st.count && ok; ++t) products(t);
+    if (st.count > 0) {
+      wait(x_full, 0);
+      if (ok) scores(0);
+      if (ok) other();
+    }
     for (int t = 0; t < st.count && ok; ++t) {
-      sums(t);                         // which frees the group's place in tensor memory for the next products
-      if (ok && t + G < st.count) products(t + G);
+      const bool more = t + 1 < st.count;
+      if (more && ++next == kStages) { next = 0; next_phase ^= 1u; }
+      const uint32_t y0 = y_base + stage * 2 * kStream, y1 = y0 + kStream;
+      wait(p_done, t & 1);
+      if (!ok) break;
+      if constexpr (KEYS) {
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < R / 16; ++i)
+            umma_f16_ta(ta, ts + at(i), desc_along_rows<R>(y1, i), idesc_a, t > 0 || i != 0);
+        }
+        __syncwarp();
+      }
+      if (more) scores(t + 1);
+      if (!ok) break;
+      wait(ds_done, t & 1);
+      if (!ok) break;
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i)
+          umma_f16_ta(ta + (KEYS ? D : 0), td + at(i), desc_along_rows<R>(y0, i), idesc_a, t > 0 || i != 0);
+        umma_commit(smem_u32(&empty[stage]));
+        if (!more) umma_commit(smem_u32(acc_full));
+      }
+      __syncwarp();
+      if (more) other();
+      stage = next;
     }
   } else {
     // ---- rows ------------------------------------------------------------------------------------
-    const int g = (warp - 2) >> 2, quarter = warp & 3;
+    const int half = (warp - 2) >> 2, quarter = warp & 3;         // columns 64 half to 64 half + 63 of the products
     const int r = quarter * 32 + lane, mine = x_row + r;          // this thread's key (or query)
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const uint32_t ts = tmem + g * 128 + lanes, td = ts + 64;
+    const uint32_t ts = tmem + lanes + half * 64, td = tmem_d + lanes + half * 64;
     const float scale = p.scale * kLog2e;
     float row_lse = 0.f, row_delta = 0.f;
     if constexpr (!KEYS) {
-      if (mine < p.seq_pad) {
-        const int64_t at = (int64_t(b) * p.heads + own_head) * p.seq_pad + mine;
-        row_lse = p.neg_lse[at];
-        row_delta = p.neg_delta[at];
-      }
+      const int64_t at = (int64_t(b) * p.heads + own_head) * p.seq_pad + mine;
+      row_lse = p.neg_lse[at];
+      row_delta = p.neg_delta[at];
     }
     bool ok = true;
-    int stage = g;
-    for (int t = g; t < st.count && ok; t += G) {
-      if (stage >= kStages) stage -= kStages;
-      ok = mbar_wait(smem_u32(&s_full[g]), (t / G) & 1, abort_flag, p.status, kErrRows, kWaitNs);
+    int stage = 0;
+    for (int t = 0; t < st.count && ok; ++t) {
+      const int y_tile = st.tile(t, KEYS) * R, y_row = y_tile + half * 64;
+      // Keys' kernel: queries i = y_row + column see this key when key <= i < key + window, or from the key on
+      // for a first token; behind the end none does.  Queries' kernel: keys of the window, and first tokens.
+      Seen seen{0, 64, 0};
+      bool edge;
+      if constexpr (KEYS) {
+        seen.from = mine - y_row;
+        seen.to = mine < p.sinks ? 64 : int(min(int64_t(64), int64_t(mine) + p.window - y_row));
+        seen.to = min(seen.to, len - y_row);
+        edge = x_row + kTile - 1 > y_tile || (y_tile + R - 1) - x_row >= p.window || y_tile + R > len;
+      } else {
+        seen.from = mine - p.window + 1 - y_row;
+        seen.to = min(64, mine + 1 - y_row);
+        seen.keep = p.sinks - y_row;
+        edge = y_tile + R - 1 > x_row || (x_row + kTile - 1) - y_tile >= p.window;
+      }
+      const float* col = stats + stage * 2 * R + half * 64;
+      ok = mbar_wait(smem_u32(s_full), t & 1, abort_flag, p.status, kErrRows, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
-      const int y_row = st.tile(t, KEYS) * kHalfTile;
-      // Columns whose pair is visible.  Keys' kernel: queries i = y_row + column see this key when
-      // key <= i < key + window, or from the key on for a first token; rows behind the end have an infinite
-      // lse.  Queries' kernel: keys of the window, and first tokens.
-      int from, to, keep;              // [from, to), and in the queries' kernel also [0, keep) where it is below `to`
-      bool edge;
-      if constexpr (KEYS) {
-        from = mine - y_row;
-        to = mine < p.sinks ? kHalfTile : int(min(int64_t(kHalfTile), int64_t(mine) + p.window - y_row));
-        // Far queries belong to the first tokens only, and are another CTA's where they are split.
-        keep = 0;
-        edge = x_row + kTile - 1 > y_row || (y_row + kHalfTile - 1) - x_row >= p.window ||
-               y_row + kHalfTile > len || x_row + kTile > len;
-        to = min(to, len - y_row);
-      } else {
-        from = mine - p.window + 1 - y_row;
-        to = min(kHalfTile, mine + 1 - y_row);
-        keep = p.sinks - y_row;
-        edge = y_row + kHalfTile - 1 > x_row || (x_row + kTile - 1) - y_row >= p.window || x_row + kTile > len;
+      float2 pr[32];
+      {
+        uint32_t s[64];
+        tmem_ld_32x32(ts, chunk_of(s, 0));
+        tmem_ld_32x32(ts + 32, chunk_of(s, 1));
+        tmem_ld_wait();
+        if constexpr (!KEYS) {
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(p_done));
+        }
+        if (edge) row_exp<T, KEYS, true>(s, ts, scale, col, row_lse, seen, pr);
+        else row_exp<T, KEYS, false>(s, ts, scale, col, row_lse, seen, pr);
       }
-      const float* col_lse = stats + stage * 2 * kHalfTile;
-      if (edge)
-        row_pairs<T, KEYS, true>(ts, td, scale, col_lse, col_lse + kHalfTile, row_lse, row_delta, from, to, keep);
-      else
-        row_pairs<T, KEYS, false>(ts, td, scale, col_lse, col_lse + kHalfTile, row_lse, row_delta, from, to, keep);
+      if constexpr (KEYS) {
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(p_done));
+      }
+      ok = mbar_wait(smem_u32(d_full), t & 1, abort_flag, p.status, kErrRows, kWaitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after();
+      if (edge) row_ds<T, KEYS, true>(td, col + R, row_delta, seen, pr);
+      else row_ds<T, KEYS, false>(td, col + R, row_delta, seen, pr);
+      tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&d_full[g]));
-      stage += G;
+      if (lane == 0) mbar_arrive(smem_u32(ds_done));
+      if (++stage == kStages) stage = 0;
     }
     if (st.count > 0 && ok) {
       ok = mbar_wait(smem_u32(acc_full), 0, abort_flag, p.status, kErrRows, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
       tcgen05_fence_after();
     }
-    // The keys' kernel has two results, dV and dK: one a group, or both of the one group.  The queries' kernel
-    // has dQ, whose columns the groups share.
+    // The keys' kernel has two results, dV and dK: one for either half of the row threads where there are two.
+    // The queries' kernel has dQ, whose columns they share.
+    constexpr int G = R / 64;
+    const int g = half;
     const bool some = st.count > 0 && ok;
     const bool live = some && mine < len;
     // A first token whose far queries are other CTAs': this CTA's share goes to the workspace.
@@ -467,15 +536,15 @@ cudaError_t row_sums(bool bf16, const void* out, const void* dout, const Params&
   return cudaGetLastError();
 }
 
-cudaError_t backward_keys(bool bf16, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q_half,
-                          const CUtensorMap& dout_half, const CUtensorMap& dk, const CUtensorMap& dv, const Params& p,
+cudaError_t backward_keys(bool bf16, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q_stream,
+                          const CUtensorMap& dout_stream, const CUtensorMap& dk, const CUtensorMap& dv, const Params& p,
                           cudaStream_t stream) {
-  return backward<true>(bf16, k, v, q_half, dout_half, dk, dv, p, stream);
+  return backward<true>(bf16, k, v, q_stream, dout_stream, dk, dv, p, stream);
 }
 
-cudaError_t backward_queries(bool bf16, const CUtensorMap& q, const CUtensorMap& dout, const CUtensorMap& k_half,
-                             const CUtensorMap& v_half, const CUtensorMap& dq, const Params& p, cudaStream_t stream) {
-  return backward<false>(bf16, q, dout, k_half, v_half, dq, dq, p, stream);
+cudaError_t backward_queries(bool bf16, const CUtensorMap& q, const CUtensorMap& dout, const CUtensorMap& k_stream,
+                             const CUtensorMap& v_stream, const CUtensorMap& dq, const Params& p, cudaStream_t stream) {
+  return backward<false>(bf16, q, dout, k_stream, v_stream, dq, dq, p, stream);
 }
 
 cudaError_t sum_far(bool bf16, void* dk, void* dv, const Params& p, cudaStream_t stream) {
