@@ -83,7 +83,7 @@ struct SelectArgs {
   bool use_sigmoid;
   float scale;
   const float* bias;                   // [experts], nullable
-  int group_lanes, shared_stride;      // filled by the launchers
+  int group_lanes, aligned_lanes, shared_stride;       // filled by the launchers
 };
 cudaError_t select_experts_fwd(DType type, const void* logits, SelectArgs args, void* scores, void* weights,
                                int64_t* ids, cudaStream_t stream);

@@ -5,10 +5,14 @@
 //   the top_k largest c of those groups are chosen, w_i = scale * s_i / ||s_chosen||_p  (p = 0: not divided)
 //   scores_e = s_e / sum_e s_e   (for the softmax that is s_e itself)
 //
-// One warp owns a token and holds its experts in registers, PL a lane, fetched V at a time.  The order of
-// the experts is exact: equal values go to the lowest id, and values that 32 bits cannot tell apart are
-// ordered by their 64-bit ones.  Without a bias the scores have the order of the logits, which are compared
-// as they are.  With one, each comparison that decides (neighbours in the chosen order, the last chosen one
+// One warp owns a token and holds its experts in registers, PL consecutive ones a lane, fetched V at a time.
+// A lane with up to eight sorts them once, as keys whose last three bits are the place, and a round of the
+// choice is one reduction of the lanes' heads; it is bound by instructions (1678 a token with the places
+// compared anew in every round: 80 us for 32768 x 256).
+//
+// The order of the experts is exact: equal values go to the lowest id, and values that 32 bits cannot tell
+// apart are ordered by their 64-bit ones.  Without a bias the scores have the order of the logits, which are
+// compared as they are.  Each comparison that decides (neighbours in the chosen order, the last chosen one
 // and the next, the last group that stays and the next) is checked against a bound of the arithmetic's
 // error; a token with a closer pair, a few in a thousand, is chosen again from scores in 64 bits.
 #include "common.cuh"
@@ -30,16 +34,16 @@ __device__ __forceinline__ unsigned ordered(float v) {
   unsigned u = __float_as_uint(v);
   if ((u & 0x7fffffffu) > 0x7f800000u) u = 0x7f800000u;
   if (u == 0x80000000u) u = 0u;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return u ^ (unsigned(int(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float from_ordered(unsigned k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// Expert of slot j of a lane; ascending in j.
-template <int V>
+// Experts of a lane: PL consecutive ones, so that a lower lane has lower ids.
+template <int PL>
 __device__ __forceinline__ int expert_of(int j, int lane) {
-  return (j / V) * (32 * V) + lane * V + j % V;
+  return lane * PL + j;
 }
 
 template <typename T, int V>
@@ -51,7 +55,7 @@ template <typename T, int PL, int V>
 __device__ __forceinline__ void load_slots(const T* row, int lane, int experts, float fill, float (&x)[PL]) {
 #pragma unroll
   for (int j = 0; j < PL; j += V) {
-    const int e = expert_of<V>(j, lane);
+    const int e = expert_of<PL>(j, lane);
     if (e < experts) {          // experts % V == 0
       const Slots<T, V> p = *reinterpret_cast<const Slots<T, V>*>(row + e);
 #pragma unroll
@@ -79,7 +83,7 @@ __device__ __forceinline__ RowStat scores_of(const float (&x)[PL], int lane, int
   if (use_sigmoid) {
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-      s[j] = expert_of<V>(j, lane) < experts ? sigmoid(x[j]) : 0.f;
+      s[j] = expert_of<PL>(j, lane) < experts ? sigmoid(x[j]) : 0.f;
       sum += s[j];
     }
     r.total = warp_sum_f(sum);
@@ -92,7 +96,7 @@ __device__ __forceinline__ RowStat scores_of(const float (&x)[PL], int lane, int
     r.top = top == -INFINITY ? 0.f : top;         // nothing but -inf: every score is zero
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-      s[j] = expert_of<V>(j, lane) < experts ? __expf(x[j] - r.top) : 0.f;
+      s[j] = expert_of<PL>(j, lane) < experts ? __expf(x[j] - r.top) : 0.f;
       sum += s[j];
     }
     sum = warp_sum_f(sum);
@@ -175,42 +179,50 @@ __device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, doubl
 
 __host__ __device__ constexpr int padded_slot(int e) { return e + (e >> 5) * 4; }
 
-// Groups that stay, as lane bits: bit (g * lanes per group).  `c` are the choice values (NaN as +inf).
-// Sets `doubt` when the last group that stays and the next are closer than the arithmetic tells apart.
-template <int PL, int V>
-__device__ __forceinline__ unsigned choose_groups(const float (&c)[PL], const SelectArgs& a, float* shared, int lane,
-                                                  float margin, bool& doubt) {
-  const int size = a.experts / a.groups;
+// Descending sort by a fixed network (Batcher's odd-even merge).
+template <int N>
+__device__ __forceinline__ void sort_down(unsigned (&k)[N]) {
 #pragma unroll
-  for (int j = 0; j < PL; ++j) {
-    const int e = expert_of<V>(j, lane);
-    if (e < a.experts) shared[padded_slot(e)] = c[j];
-  }
-  __syncwarp();
-  const int lanes = a.group_lanes, g = lane / lanes;
-  float b1 = -INFINITY, b2 = -INFINITY;
-  if (g < a.groups) {
-    for (int i = lane % lanes; i < size; i += lanes) {
-      const float v = shared[padded_slot(g * size + i)];
-      b2 = fmaxf(b2, fminf(b1, v));
-      b1 = fmaxf(b1, v);
-    }
-  }
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const unsigned hi = max(k[i + j], k[i + j + q]), lo = min(k[i + j], k[i + j + q]);
+            k[i + j] = hi;
+            k[i + j + q] = lo;
+          }
+}
+
+// The two largest of a group that spans `lanes` lanes, in all of them.
+__device__ __forceinline__ void join_best(float& b1, float& b2, int lanes) {
   for (int d = lanes / 2; d > 0; d >>= 1) {
     const float o1 = __shfl_xor_sync(0xffffffffu, b1, d), o2 = __shfl_xor_sync(0xffffffffu, b2, d);
     b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
     b1 = fmaxf(b1, o1);
   }
-  const unsigned value = g < a.groups ? ordered(size > 1 ? b1 + b2 : b1) : 0u;
+}
+
+// Whether this lane's group stays, as lane bits: bit (g * lanes per group).  `b1`, `b2`: the largest values of
+// group lane / lanes.  Sets `doubt` when the last group that stays and the next are closer than the arithmetic
+// tells apart.
+__device__ __forceinline__ unsigned choose_groups(float b1, float b2, int lanes, int size, const SelectArgs& a, int lane,
+                                                  float margin, bool& doubt) {
+  const int g = lane / lanes;
+  const bool there = g < a.groups;
+  const unsigned value = there ? ordered(size > 1 ? b1 + b2 : b1) : 0u;
   int rank = 0;
   for (int h = 0; h < a.groups; ++h) {
     const unsigned o = __shfl_sync(0xffffffffu, value, h * lanes);
     rank += o > value || (o == value && h < g);
   }
-  const bool stays = g < a.groups && rank < a.top_groups;
+  const bool stays = there && rank < a.top_groups;
   const float last = from_ordered(__reduce_min_sync(0xffffffffu, stays ? value : 0xffffffffu));
   const float next = from_ordered(__reduce_max_sync(0xffffffffu, stays ? 0u : value));
-  doubt = !(last - next > 2.f * margin + 0x1p-21f * fmaxf(fabsf(last), fabsf(next)));
+  doubt = !(last - next > 2.f * margin + 0x1p-19f * fmaxf(fabsf(last), fabsf(next)));
   return __ballot_sync(0xffffffffu, stays);
 }
 
@@ -218,6 +230,8 @@ template <typename T, int PL, int V>
 __global__ void __launch_bounds__(kWarps * 32)
 select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restrict__ scores, T* __restrict__ weights,
                   int64_t* __restrict__ ids) {
+  constexpr bool kSorted = PL <= 8;
+  constexpr unsigned kPlace = kSorted ? 7u : 0u;          // key bits that hold 7 - place instead of value
   extern __shared__ double shared[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = a.experts;
   const int64_t t = int64_t(blockIdx.x) * kWarps + warp;
@@ -229,7 +243,7 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
   const float inv_total = a.use_sigmoid && r.total != 0.f ? 1.f / r.total : 1.f;
 #pragma unroll
   for (int j = 0; j < PL; j += V) {
-    const int e = expert_of<V>(j, lane);
+    const int e = expert_of<PL>(j, lane);
     if (e < E) {
       Slots<T, V> p;
 #pragma unroll
@@ -238,60 +252,116 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
     }
   }
 
-  // Twice the error of a score: exponent's rounding and unit, division, sum (see the bound's terms: 1.6 x
-  // 2^-22 for the sigmoid, 1.6 x 2^-20 of the largest for the softmax); the sum with the bias adds its own
-  // rounding where two values are compared.
+  // Twice the error of a score: exponent's rounding and unit, division, sum (1.6 x 2^-22 for the sigmoid,
+  // 1.6 x 2^-20 of the largest for the softmax).  Where two values are compared, the rounding of the sum with the
+  // bias and the bits that a key gives to the place come on top: 2^-20 of the values.
   const float margin = a.use_sigmoid ? 0x1p-20f : 0x1p-18f * r.inv;
   const bool biased = a.bias != nullptr;
+  float* const mine_shared = reinterpret_cast<float*>(shared + warp * a.shared_stride);
+  const bool grouped = a.top_groups < a.groups;
   bool doubt = false;
   unsigned key[PL];
-  {
-    float c[PL];
 #pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      const int e = expert_of<V>(j, lane);
-      c[j] = biased && e < E ? s[j] + __ldg(a.bias + e) : s[j];
-      key[j] = e < E ? ordered(biased ? c[j] : x[j]) : 0u;
-    }
-    if (a.top_groups < a.groups) {
+  for (int j = 0; j < PL; ++j) {
+    const int e = expert_of<PL>(j, lane);
+    const bool there = e < E;
+    const float c = biased && there ? s[j] + __ldg(a.bias + e) : s[j];
+    if (grouped && a.aligned_lanes == 0 && there) mine_shared[padded_slot(e)] = c != c ? INFINITY : c;
+    s[j] = c;
+    key[j] = there ? (ordered(biased ? c : x[j]) & ~kPlace) | (kPlace - (unsigned(j) & kPlace)) : 0u;
+  }
+  if constexpr (kSorted) sort_down(key);
+  if (grouped) {
+    const int size = E / a.groups;
+    float b1 = -INFINITY, b2 = -INFINITY;
+    if (a.aligned_lanes > 0) {                            // groups of whole lanes, a power of two of them
 #pragma unroll
-      for (int j = 0; j < PL; ++j) c[j] = c[j] != c[j] ? INFINITY : c[j];
-      const unsigned stays = choose_groups<PL, V>(c, a, reinterpret_cast<float*>(shared + warp * a.shared_stride),
-                                                  lane, margin, doubt);
+      for (int j = 0; j < PL; ++j) {
+        const float v = expert_of<PL>(j, lane) < E ? (s[j] != s[j] ? INFINITY : s[j]) : -INFINITY;
+        b2 = fmaxf(b2, fminf(b1, v));
+        b1 = fmaxf(b1, v);
+      }
+      join_best(b1, b2, a.aligned_lanes);
+      const unsigned stays = choose_groups(b1, b2, a.aligned_lanes, size, a, lane, margin, doubt);
+      if (!(stays >> (lane / a.aligned_lanes * a.aligned_lanes) & 1u)) {
+#pragma unroll
+        for (int j = 0; j < PL; ++j) key[j] = 0u;
+      }
+    } else {
+      __syncwarp();
+      const int lanes = a.group_lanes, g = lane / lanes;
+      if (g < a.groups) {
+        for (int i = lane % lanes; i < size; i += lanes) {
+          const float v = mine_shared[padded_slot(g * size + i)];
+          b2 = fmaxf(b2, fminf(b1, v));
+          b1 = fmaxf(b1, v);
+        }
+      }
+      join_best(b1, b2, lanes);
+      const unsigned stays = choose_groups(b1, b2, lanes, size, a, lane, margin, doubt);
       const float inv_size = float(a.groups) / float(E);
 #pragma unroll
       for (int j = 0; j < PL; ++j) {
-        const int g = int((expert_of<V>(j, lane) + 0.5f) * inv_size);       // exact: at most 1024 experts
-        if (!(stays >> (g * a.group_lanes) & 1u)) key[j] = 0u;
+        const int place = kSorted ? int(kPlace - (key[j] & kPlace)) : j;
+        const int g2 = int((lane * PL + place + 0.5f) * inv_size);           // exact: at most 1024 experts
+        if (!(stays >> (g2 * lanes & 31) & 1u)) key[j] = 0u;
       }
+      if constexpr (kSorted) sort_down(key);
     }
   }
 
-  int mine = 0, before = 0;
-  float before_c = 0.f;
-  // With a bias one expert more than is chosen: the last one has to be told from the next.
-  const int rounds = a.top_k + (biased ? 1 : 0);
-  for (int i = 0; i < rounds && !doubt; ++i) {
-    unsigned best = 0u;
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int j = 0; j < PL; ++j)
-      if (key[j] > best) { best = key[j]; at = expert_of<V>(j, lane); }
-    const unsigned top = __reduce_max_sync(0xffffffffu, best);
-    if (top == 0u) break;                         // all experts are chosen
-    const int e = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
-    if (biased) {
-      const float c = from_ordered(top);
-      if (i > 0 && !(before_c - c > margin + 0x1p-22f * fmaxf(fabsf(before_c), fabsf(c))))
-        doubt = !(ordered(to_float(row[before])) == ordered(to_float(row[e])) && a.bias[before] == a.bias[e]);
-      before_c = c;
-      before = e;
-    }
-    if (lane == i) mine = e;
-    if (at == e) {
+  // With values that a key does not hold exactly one expert more than is chosen: the last has to be told from
+  // the next.
+  const bool inexact = biased || (kSorted && sizeof(T) == 4);
+  const int rounds = a.top_k + (inexact ? 1 : 0);
+  int mine = 0;                        // this lane's choice and its key; the key after all choices
+  unsigned mine_key = 0u, next_key = 0u;
+  for (int i = 0; i < rounds; ++i) {
+    unsigned head;
+    int at;
+    if constexpr (kSorted) {
+      head = key[0] & ~kPlace;
+      at = lane * PL + int(kPlace - (key[0] & kPlace));
+    } else {
+      head = 0u;
+      at = 0;
 #pragma unroll
       for (int j = 0; j < PL; ++j)
-        if (expert_of<V>(j, lane) == e) key[j] = 0u;
+        if (key[j] > head) { head = key[j]; at = expert_of<PL>(j, lane); }
+    }
+    const unsigned top = __reduce_max_sync(0xffffffffu, head);
+    const int from = __ffs(__ballot_sync(0xffffffffu, head == top)) - 1;      // the lowest lane has the lowest id
+    const int e = __shfl_sync(0xffffffffu, at, from);
+    if (lane == i && i < a.top_k) { mine = e; mine_key = top; }
+    next_key = top;
+    if (lane == from) {
+      if constexpr (kSorted) {
+#pragma unroll
+        for (int j = 0; j + 1 < PL; ++j) key[j] = key[j + 1];
+        key[PL - 1] = 0u;
+      } else {
+#pragma unroll
+        for (int j = 0; j < PL; ++j)
+          if (expert_of<PL>(j, lane) == e) key[j] = 0u;
+      }
+    }
+  }
+  if (inexact) {                                          // all neighbours at once; a key of 0: no expert was left
+    const bool last = lane == a.top_k - 1;
+    const unsigned down = __shfl_down_sync(0xffffffffu, mine_key, 1), next = last ? next_key : down;
+    bool close = false;
+    if (lane < a.top_k && next != 0u) {
+      const float c = from_ordered(mine_key), d = from_ordered(next);
+      close = biased ? !(c - d > margin + 0x1p-20f * fmaxf(fabsf(c), fabsf(d))) : mine_key == next;
+    }
+    if (__any_sync(0xffffffffu, close)) {
+      // Experts that are alike in logit and bias are equal.  Not so behind the last choice, where others that are
+      // as close may follow.
+      const int other = __shfl_down_sync(0xffffffffu, mine, 1);
+      if (close && !last)
+        close = !(ordered(to_float(row[mine])) == ordered(to_float(row[other])) &&
+                  (!biased || a.bias[mine] == a.bias[other]));
+      if (__any_sync(0xffffffffu, close)) doubt = true;
     }
   }
   if (doubt) {
@@ -357,7 +427,7 @@ select_bwd_kernel(const T* __restrict__ logits, const SelectArgs a, const int64_
   T* out = dlogits + t * E;
 #pragma unroll
   for (int j = 0; j < PL; j += V) {
-    const int e = expert_of<V>(j, lane);
+    const int e = expert_of<PL>(j, lane);
     if (e < E) {
       Slots<T, V> p;
 #pragma unroll
@@ -387,21 +457,23 @@ bool row_vectors(int experts, const void* p) {
   return experts % V == 0 && reinterpret_cast<uintptr_t>(p) % (V * sizeof(T)) == 0;
 }
 
-// PL slots a lane, fetched min(PL, 16 bytes) at a time where the rows allow it, else one by one.
+// PL slots a lane, fetched up to 16 bytes at a time where the rows allow it, else one by one.
 #define MB_SELECT_SWITCH(T, experts, aligned, CALL)                       \
   if (experts <= 32) { CALL(1, 1); }                                      \
   else if (experts <= 64) { if (aligned(2)) { CALL(2, 2); } else { CALL(2, 1); } } \
   else if (experts <= 128) { if (aligned(4)) { CALL(4, 4); } else { CALL(4, 1); } } \
-  else if (experts <= 256) {                                              \
-    constexpr int W = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;            \
-    if (aligned(W)) { CALL(8, W); } else { CALL(8, 1); }                  \
-  } else if (experts <= 512) {                                            \
+  else {                                                                  \
     constexpr int W = 16 / sizeof(T);                                     \
-    if (aligned(W)) { CALL(16, W); } else { CALL(16, 1); }                \
-  } else {                                                                \
-    constexpr int W = 16 / sizeof(T);                                     \
-    if (aligned(W)) { CALL(32, W); } else { CALL(32, 1); }                \
+    if (experts <= 256) { if (aligned(W)) { CALL(8, W); } else { CALL(8, 1); } }        \
+    else if (experts <= 512) { if (aligned(W)) { CALL(16, W); } else { CALL(16, 1); } } \
+    else { if (aligned(W)) { CALL(32, W); } else { CALL(32, 1); } }       \
   }
+
+int slots_per_lane(int experts) {
+  int n = 1;
+  while (n * 32 < experts) n *= 2;
+  return n;
+}
 
 bool complete(SelectArgs& a) {
   if (a.experts < 1 || a.experts > kRouterMaxExperts || a.top_k < 1 || a.top_k > kSelectMaxTopK) return false;
@@ -410,7 +482,11 @@ bool complete(SelectArgs& a) {
     return false;
   a.group_lanes = 1;
   while (a.group_lanes * 2 * a.groups <= 32) a.group_lanes *= 2;
-  a.shared_stride = a.bias != nullptr || a.top_groups < a.groups ? (a.experts > 16 ? a.experts : 16) : 0;
+  // Lanes of a group where it takes whole ones, a power of two of them; 0: it does not.
+  const int size = a.experts / a.groups, per_lane = slots_per_lane(a.experts);
+  const int span = size % per_lane == 0 ? size / per_lane : 0;
+  a.aligned_lanes = span > 0 && (span & (span - 1)) == 0 && span * a.groups <= 32 ? span : 0;
+  a.shared_stride = a.experts;
   return true;
 }
 

@@ -61,6 +61,9 @@ CASES = [
     (20, 512, 8, 'sigmoid', True, 8, 2, 1, 2.5),
     (20, 1024, 32, 'softmax', True, 32, 5, 1, 1.0),
     (20, 1023, 32, 'sigmoid', False, 1, 1, 1, 1.0),
+    (9, 32, 32, 'sigmoid', True, 1, 1, 1, 1.0),
+    (33, 250, 9, 'softmax', True, 5, 2, 2, 1.0),
+    (33, 192, 6, 'sigmoid', True, 12, 3, 1, 1.0),
 ]
 
 
@@ -110,6 +113,21 @@ def test_order_beyond_32_bits(device, score, groups, top_groups):
     logits = logits[:1].repeat(64, 1)
     logits[1:] += torch.randn(63, 1, device=device) * 1e-6
     got, want = both(logits, top_k=6, score=score, bias=bias, groups=groups, top_groups=top_groups, norm_p=1)
+    assert torch.equal(got[2].cpu(), want[2])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('experts,top_k', [(24, 5), (64, 32), (200, 8), (256, 32), (700, 32)])
+def test_neighbouring_values(device, experts, top_k):
+    """fp32 logits, and scores with a bias, that differ in their last bits or not at all."""
+    base = torch.rand(60, 1, device=device) + 0.5
+    logits = (base.view(torch.int32) + torch.randint(0, 12, (60, experts), device=device, dtype=torch.int32)).view(FP32)
+    for groups, top_groups in ((1, 1), (4, 4), (4, 2)):
+        got, want = both(logits, top_k=min(top_k, experts // 2), groups=groups, top_groups=top_groups)
+        assert torch.equal(got[2].cpu(), want[2])
+    bias = torch.zeros(experts, device=device)
+    bias[::3] = 2.0**-24
+    got, want = both(logits, top_k=top_k, bias=bias, score='sigmoid')
     assert torch.equal(got[2].cpu(), want[2])
 
 
