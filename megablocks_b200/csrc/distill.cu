@@ -4,11 +4,14 @@
 //   loss = T^2 sum_i p_i (log p_i - log q_{id_i}) + hard * (logsumexp(z) - z_target)
 //   dloss / dz_j = T (q_j - sum_{i: id_i = j} p_i) + hard * (softmax(z)_j - [j = target])
 //
-// Bound by memory: a logit is read once and its gradient written once.  A CTA takes a row.  Where the row
-// fits shared memory it is fetched there by bulk copies, all of them in flight from the start, and both
-// passes (the running maximum and sum; the gradient) run on that copy; longer rows take the second pass
-// from L2.  The few columns that the teacher or the target names are written again, with their whole
-// value and one rounding, after the row.
+// Bound by memory: a logit is read once and its gradient written once.  Where two rows fit shared memory, CTAs
+// stay and walk the rows: a row's successor is fetched by bulk copies while the row is worked on, in three
+// passes over shared memory (maximum; sums; gradient, stored straight to memory), and a warp of its own
+// prepares the teacher's probabilities of the next row meanwhile.  A CTA a row, with two on an SM, took twice
+// as long (542 against 279 us for 8192 rows of 51200 bf16): each phase of a row left another unit idle.
+// Longer rows, and passes without a gradient, stream the row from memory with a running maximum; a gradient
+// then reads it again, from L2.  The few columns that the teacher or the target names are written again, with
+// their whole value and one rounding, after the row.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -16,9 +19,10 @@ namespace mb {
 
 namespace {
 
-constexpr int kChunks = 8;                        // bulk copies of a row, each with a barrier of its own
+constexpr int kCopies = 8;                        // bulk copies of a row
 constexpr int kMaxThreads = 512;
-constexpr int kSharedRow = 200 * 1024;            // longest row, in bytes, that is kept in shared memory
+constexpr int kRowThreads = 768;                  // most threads that work on a row in shared memory
+constexpr int kSharedBytes = 226 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -127,37 +131,75 @@ __device__ __forceinline__ Online block_sums(Online o, const Powers& w, bool two
   return part;
 }
 
-// The teacher's row in shared memory: p (0 in unused slots) and column (-1 there).  One warp; returns
-// whether any slot is used, and sum p log p.
-__device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t row, float* p, int* column, float* entropy) {
+// The teacher's row in shared memory: `slots` values each of p (0 in unused slots), column (-1 there) and z, the
+// named columns' logits, which the row's threads fill in.
+__host__ __device__ constexpr int padded_slots(int top) { return (top + 3) / 4 * 4; }
+struct Teacher {
+  float* p;
+  int* column;
+  float* z;
+  __device__ __forceinline__ Teacher(void* place, int top)
+      : p(static_cast<float*>(place)), column(reinterpret_cast<int*>(p + padded_slots(top))),
+        z(p + 2 * padded_slots(top)) {}
+};
+
+// Fills it, with one warp; returns whether any slot is used, and sum p log p.
+__device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t row, const Teacher& t, float* entropy) {
   const int lane = threadIdx.x & 31;
   const float inv_t = 1.f / a.temperature;
   float top = -INFINITY;
-  for (int i = lane; i < a.top; i += 32) {
-    const int64_t at = row * a.top + i;
-    const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
-    const bool used = id >= 0 && id < a.vocab;
-    column[i] = used ? int(id) : -1;
-    p[i] = used ? load_value(a.values, a.value_type, at) * inv_t : -INFINITY;
-    top = fmaxf(top, p[i]);
+  for (int i0 = lane; i0 < padded_slots(a.top); i0 += 128) {      // 128 slots in flight
+    int64_t id[4];
+    float value[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 32 * u;
+      const int64_t at = row * a.top + i;
+      id[u] = -1;
+      value[u] = -INFINITY;
+      if (i < a.top) {
+        id[u] = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
+        value[u] = load_value(a.values, a.value_type, at) * inv_t;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 32 * u;
+      if (i >= padded_slots(a.top)) break;
+      const bool used = id[u] >= 0 && id[u] < a.vocab;
+      t.column[i] = used ? int(id[u]) : -1;
+      t.p[i] = used ? value[u] : -INFINITY;
+      top = fmaxf(top, t.p[i]);
+    }
   }
   top = warp_max(top);
   const bool live = top > -INFINITY;
   float sum = 0.f;
-  for (int i = lane; i < a.top; i += 32) sum += live ? exp2_approx((p[i] - top) * kLog2e) : 0.f;
+  for (int i = lane; i < a.top; i += 32) sum += live ? exp2_approx((t.p[i] - top) * kLog2e) : 0.f;
   sum = warp_sum(sum);
   const float log_sum = kLn2 * __log2f(sum), inv = 1.f / sum;
   float ent = 0.f;
   for (int i = lane; i < a.top; i += 32) {
-    const float x = p[i] - top;
+    const float x = t.p[i] - top;
     const float w = live ? exp2_approx(x * kLog2e) * inv : 0.f;
     if (w != 0.f) ent += w * (x - log_sum);
-    p[i] = w;
-    if (w == 0.f) column[i] = -1;
+    t.p[i] = w;
+    if (w == 0.f) t.column[i] = -1;
   }
   *entropy = warp_sum(ent);
   __syncwarp();
   return live;
+}
+
+// Slots that name column c, other than slot i.
+__device__ __forceinline__ bool named_elsewhere(const Teacher& t, int top, int c, int i) {
+  int found = 0;
+  for (int k = 0; k < padded_slots(top); k += 4) {
+    const int4 q = *reinterpret_cast<const int4*>(t.column + k);
+    found |= int(q.x == c && k != i) | int(q.y == c && k + 1 != i) | int(q.z == c && k + 2 != i) |
+             int(q.w == c && k + 3 != i);
+  }
+  return found != 0;
 }
 
 // Coefficients of a row's gradient, probabilities' sums included.
@@ -234,31 +276,29 @@ __device__ __forceinline__ void write_gradient(const T* src, const Cut<T>& cut, 
 // row was written.  A column named more than once is written by its first slot, with all its shares.
 template <typename T>
 __device__ __forceinline__ void write_named(const DistillArgs& a, T* grad, const RowGrad& g, float soft_scale,
-                                            float hard_scale, const float* p, const int* column, const float* z,
-                                            int target, float z_target) {
-  for (int i = threadIdx.x; i < a.top; i += blockDim.x) {
-    const int c = column[i];
+                                            float hard_scale, const Teacher& t, int target, float z_target, int threads) {
+  for (int i = threadIdx.x; i < a.top; i += threads) {
+    const int c = t.column[i];
     if (c < 0) continue;
-    float share = 0.f;
-    bool first = true;
-    for (int k = 0; k < a.top; ++k) {
-      if (column[k] != c) continue;
-      if (k < i) { first = false; break; }
-      share += p[k];
+    float share = t.p[i];
+    if (named_elsewhere(t, a.top, c, i)) {
+      share = 0.f;
+      bool first = true;
+      for (int k = 0; k < a.top; ++k) {
+        if (t.column[k] != c) continue;
+        first &= k >= i;
+        share += t.p[k];
+      }
+      if (!first) continue;
     }
-    if (!first) continue;
-    float x[1] = {z[i]};
+    float x[1] = {t.z[i]};
     gradient(g, x);
     grad[c] = from_float<T>(x[0] - soft_scale * share - (c == target ? hard_scale : 0.f));
   }
-  if (threadIdx.x == 0 && target >= 0) {
-    bool named = false;
-    for (int k = 0; k < a.top; ++k) named |= column[k] == target;
-    if (!named) {
-      float x[1] = {z_target};
-      gradient(g, x);
-      grad[target] = from_float<T>(x[0] - hard_scale);
-    }
+  if (int(threadIdx.x) == threads - 1 && target >= 0 && !named_elsewhere(t, a.top, target, -1)) {
+    float x[1] = {z_target};
+    gradient(g, x);
+    grad[target] = from_float<T>(x[0] - hard_scale);
   }
 }
 
@@ -267,111 +307,267 @@ __device__ __forceinline__ Powers powers(const DistillArgs& a) {
   return {kLog2e / t, t == 1.f ? 0 : (t == 2.f ? 1 : (t == 4.f ? 2 : 3))};
 }
 
-template <typename T, bool CACHED>
+// Maximum of a pack; of 16-bit types in their own arithmetic, which is exact.
+template <typename T, int N>
+__device__ __forceinline__ float pack_max(const Pack<T, N>& v) {
+  if constexpr (sizeof(T) == 4) {
+    float m = v.v[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) m = fmaxf(m, v.v[k]);
+    return m;
+  } else {
+    using P2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    const P2* q = reinterpret_cast<const P2*>(&v);
+    const P2 m = __hmax2(__hmax2(q[0], q[1]), __hmax2(q[2], q[3]));
+    return fmaxf(to_float(m.x), to_float(m.y));
+  }
+}
+
+// Rows in shared memory.  All warps but the last work on a row; the last fetches the next one and prepares its
+// teacher.  `row_bytes`: room for a row, a multiple of 16 with 16 to spare for its phase.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads + 32)
+distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stats, T* grad) {
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ float red[4][kRowThreads / 32];
+  __shared__ alignas(8) uint64_t full[2];
+  __shared__ int abort_flag;
+  __shared__ float entropy_s[3];
+  __shared__ int live_s[3];
+  const int threads = blockDim.x - 32, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slots = padded_slots(a.top);
+  float* teachers = reinterpret_cast<float*>(shared + 2 * row_bytes);      // [3]
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    ptx::mbar_init(ptx::smem_u32(&full[0]), 1);
+    ptx::mbar_init(ptx::smem_u32(&full[1]), 1);
+    ptx::fence_barrier_init();
+  }
+  __syncthreads();
+  auto row_of = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
+  auto place_of = [&](int64_t row, int buffer) {                           // where a row's element 0 lies (or would)
+    return reinterpret_cast<T*>(shared + buffer * row_bytes + reinterpret_cast<uintptr_t>(row_of(row)) % 16);
+  };
+
+  if (warp == warps) {
+    // The teacher has three places: the named columns of the row before are still being written.
+    auto prepare = [&](int64_t row, int buffer, int set) {
+      if (row >= a.rows) return;
+      if (lane == 0) {
+        const T* in = row_of(row);
+        const Cut<T> cut(in, a.vocab);
+        const uint32_t bar = ptx::smem_u32(&full[buffer]);
+        T* copy = place_of(row, buffer);
+        ptx::mbar_arrive_expect_tx(bar, uint32_t(cut.packs) * 16);
+        const int piece = (cut.packs + kCopies - 1) / kCopies;
+        for (int c = 0; c < cut.packs; c += piece)
+          ptx::bulk_load(ptx::smem_u32(copy + cut.head + c * VEC), in + cut.head + c * VEC,
+                         uint32_t(min(piece, cut.packs - c)) * 16, bar);
+      }
+      __syncwarp();
+      float entropy;
+      const bool live = teacher_row(a, row, Teacher(teachers + set * 3 * slots, a.top), &entropy);
+      if (lane == 0) { entropy_s[set] = entropy; live_s[set] = live; }
+    };
+    prepare(blockIdx.x, 0, 0);
+    __syncthreads();
+    int buffer = 1, set = 1;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+      prepare(row + gridDim.x, buffer, set);
+      __syncthreads();                 // the row's shared memory is free
+      buffer ^= 1;
+      set = set == 2 ? 0 : set + 1;
+    }
+    if (*static_cast<volatile int*>(&abort_flag) != 0) {           // a wait ran out: let the copies in flight end
+      const uint64_t t0 = ptx::globaltimer_ns();
+      while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+    return;
+  }
+
+  const Powers w = powers(a);
+  auto group_sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
+  __syncthreads();
+  int buffer = 0, set = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* in = row_of(row);
+    const Cut<T> cut(in, a.vocab);
+    const T* copy = place_of(row, buffer);
+    const Pack<T, VEC>* body = reinterpret_cast<const Pack<T, VEC>*>(copy + cut.head);
+    const Teacher t(teachers + set * 3 * slots, a.top);
+    const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
+    const int target = wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
+    const bool two = target >= 0 && w.squares != 0;
+    const bool live = live_s[set] != 0;
+    // The elements before the first and behind the last 16-byte boundary stay in memory: one thread's each.
+    const int tail0 = a.vocab - cut.tail;
+    const int mine = int(threadIdx.x) < cut.head ? int(threadIdx.x)
+                     : int(threadIdx.x) - cut.head < cut.tail ? tail0 + int(threadIdx.x) - cut.head : -1;
+    const float edge = mine >= 0 ? to_float(in[mine]) : -INFINITY;
+    auto value_at = [&](int c) { return to_float(c < cut.head || c >= tail0 ? in[c] : copy[c]); };
+
+    const bool ok = ptx::mbar_wait(ptx::smem_u32(&full[buffer]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
+    float top = edge;
+    if (ok) {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < cut.packs; i += threads) top = fmaxf(top, pack_max(body[i]));
+    }
+    top = warp_max(top);
+    if (lane == 0) red[0][warp] = top;
+    group_sync();
+    top = warp_max(lane < warps ? red[0][lane] : -INFINITY);
+    const float base = top == -INFINITY ? 0.f : top;
+
+    float2 soft = make_float2(0.f, 0.f), hard = soft;
+    float cross = 0.f;
+    for (int i = threadIdx.x; i < a.top; i += threads) {
+      if (t.column[i] < 0) continue;
+      t.z[i] = value_at(t.column[i]);  // before the row may be overwritten
+      cross += t.p[i] * (t.z[i] - base);
+    }
+    const float z_target = target >= 0 ? value_at(target) : 0.f;
+    if (mine >= 0) {
+      soft.x = exp2_approx((edge - base) * w.k);
+      if (two) hard.x = w.second(soft.x, edge - base);
+    }
+    const float2 minus = make_float2(-base, -base), k2 = make_float2(w.k, w.k);
+    auto add = [&](auto with_hard) {
+#pragma unroll 2
+      for (int i = threadIdx.x; i < cut.packs; i += threads) {
+        const Pack<T, VEC> v = body[i];
+#pragma unroll
+        for (int k = 0; k < VEC; k += 2) {
+          const float2 d = __fadd2_rn(make_float2(to_float(v.v[k]), to_float(v.v[k + 1])), minus);
+          const float2 x = __fmul2_rn(d, k2);
+          const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          soft = __fadd2_rn(soft, e);
+          if constexpr (decltype(with_hard)::value)
+            hard = __fadd2_rn(hard, make_float2(w.second(e.x, d.x), w.second(e.y, d.y)));
+        }
+      }
+    };
+    if (ok) {
+      if (two) add(std::true_type{});
+      else add(std::false_type{});
+    }
+    {
+      const float s = warp_sum(soft.x + soft.y), h = two ? warp_sum(hard.x + hard.y) : 0.f, c = warp_sum(cross);
+      if (lane == 0) { red[1][warp] = s; red[2][warp] = h; red[3][warp] = c; }
+    }
+    group_sync();
+    const float sum_soft = warp_sum(lane < warps ? red[1][lane] : 0.f);
+    const float sum_hard = two ? warp_sum(lane < warps ? red[2][lane] : 0.f) : sum_soft;
+    if (warp == 0) {
+      const float c = warp_sum(lane < warps ? red[3][lane] : 0.f);
+      if (lane == 0) {
+        float l = 0.f;
+        if (live) l = a.temperature * a.temperature * (entropy_s[set] - kLn2 * (c * w.k - __log2f(sum_soft)));
+        if (target >= 0) l += a.hard_weight * (kLn2 * __log2f(sum_hard) + (top - z_target));
+        *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(ok ? l : NAN, top, sum_soft, sum_hard);
+      }
+    }
+    const RowGrad g = row_grad(a, live, target >= 0, a.scale, top, sum_soft, sum_hard, w);
+    T* out = grad + row * a.vocab;
+    if (mine >= 0) {
+      float x[1] = {edge};
+      gradient(g, x);
+      out[mine] = from_float<T>(x[0]);
+    }
+    const bool aligned = reinterpret_cast<uintptr_t>(out + cut.head) % 16 == 0;
+    if (ok) {
+#pragma unroll 2
+      for (int i = threadIdx.x; i < cut.packs; i += threads) {
+        Pack<T, VEC> v = body[i];
+        float x[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x[k] = to_float(v.v[k]);
+        gradient(g, x);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v.v[k] = from_float<T>(x[k]);
+        if (aligned) {
+          *reinterpret_cast<Pack<T, VEC>*>(out + cut.head + i * VEC) = v;
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) out[cut.head + i * VEC + k] = v.v[k];
+        }
+      }
+    }
+    __syncthreads();
+    write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, target, z_target, threads);
+    phase ^= uint32_t(buffer);
+    buffer ^= 1;
+    set = set == 2 ? 0 : set + 1;
+  }
+}
+
+// Rows streamed from memory, one a CTA.
+template <typename T>
 __global__ void __launch_bounds__(kMaxThreads)
 distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ float red[3 * kMaxThreads / 32];
-  __shared__ alignas(8) uint64_t bars[kChunks];
-  __shared__ int abort_flag;
   __shared__ float entropy_s;
   __shared__ int live_s;
   const int64_t row = blockIdx.x;
   const T* in = static_cast<const T*>(a.logits) + row * a.vocab;
   const Cut<T> cut(in, a.vocab);
-  float* p = reinterpret_cast<float*>(shared);
-  int* column = reinterpret_cast<int*>(p + a.top);
-  float* z = reinterpret_cast<float*>(column + a.top);
-  T* copy = nullptr;
-  int chunk_packs = 1;
-  if constexpr (CACHED) {
-    unsigned char* base = shared + (3 * size_t(a.top) * 4 + 15) / 16 * 16;
-    copy = reinterpret_cast<T*>(base + reinterpret_cast<uintptr_t>(in) % 16);
-    const int all = kChunks * int(blockDim.x);          // whole rounds of the block in every chunk
-    chunk_packs = max(1, (cut.packs + all - 1) / all) * int(blockDim.x);
-    if (threadIdx.x == 0) {
-      abort_flag = 0;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) ptx::mbar_init(ptx::smem_u32(&bars[c]), 1);
-      ptx::fence_barrier_init();
-      ptx::fence_proxy_async_smem();
-      for (int c = 0; c * chunk_packs < cut.packs; ++c) {
-        const int n = min(chunk_packs, cut.packs - c * chunk_packs);
-        const uint32_t bar = ptx::smem_u32(&bars[c]);
-        ptx::mbar_arrive_expect_tx(bar, uint32_t(n) * 16);
-        ptx::bulk_load(ptx::smem_u32(copy + cut.head + c * chunk_packs * VEC), in + cut.head + c * chunk_packs * VEC,
-                       uint32_t(n) * 16, bar);
-      }
-    }
-    if (int(threadIdx.x) < cut.head) copy[threadIdx.x] = in[threadIdx.x];
-    if (int(threadIdx.x) < cut.tail) copy[a.vocab - cut.tail + threadIdx.x] = in[a.vocab - cut.tail + threadIdx.x];
-  }
+  const Teacher t(shared, a.top);
   const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
   const int target = wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
-  if (threadIdx.x < 32) {
-    float entropy;
-    const bool live = teacher_row(a, row, p, column, &entropy);
-    if (threadIdx.x == 0) { entropy_s = entropy; live_s = live; }
-  }
-  __syncthreads();
-  const bool live = live_s != 0;
-  const T* src = CACHED ? copy : in;
-
   const Powers w = powers(a);
   const bool two = target >= 0 && w.squares != 0;               // a second sum, at temperature one
   Online sums;
   {
     auto one = [&](int i) {
-      const float x[1] = {to_float(src[i])};
+      const float x[1] = {to_float(in[i])};
       sums.add(x, w, two);
     };
     if (int(threadIdx.x) < cut.head) one(threadIdx.x);
     if (int(threadIdx.x) < cut.tail) one(a.vocab - cut.tail + threadIdx.x);
   }
-  for (int c = 0; c * chunk_packs < cut.packs; ++c) {
-    int first = c * chunk_packs + threadIdx.x, last = min(cut.packs, (c + 1) * chunk_packs);
-    if constexpr (CACHED) {
-      const uint32_t bar = ptx::smem_u32(&bars[c]);
-      if (!ptx::mbar_wait(bar, 0, &abort_flag, a.status, kDistillTimeout, kWaitNs)) {
-        // The row never came: no result, and no way out before the copies have ended or the limit is reached.
-        if (threadIdx.x == 0) stats[4 * row] = NAN;
-        for (; c * chunk_packs < cut.packs; ++c) {
-          const uint64_t t0 = ptx::globaltimer_ns();
-          while (!ptx::mbar_try_wait(ptx::smem_u32(&bars[c]), 0) && ptx::globaltimer_ns() - t0 < kWaitNs) {}
-        }
-        return;
-      }
-    } else {
-      last = cut.packs;
-    }
-    for (int i = first; i < last; i += blockDim.x) {
-      const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(src + cut.head + i * VEC);
+  const Pack<T, VEC>* body = reinterpret_cast<const Pack<T, VEC>*>(in + cut.head);
+  constexpr int kAhead = 4;            // packs of a thread in flight
+  for (int i = threadIdx.x; i < cut.packs; i += kAhead * blockDim.x) {
+    Pack<T, VEC> v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (i + u * int(blockDim.x) < cut.packs) v[u] = body[i + u * blockDim.x];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u * int(blockDim.x) >= cut.packs) break;
       float x[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = to_float(v.v[k]);
+      for (int k = 0; k < VEC; ++k) x[k] = to_float(v[u].v[k]);
       sums.add(x, w, two);
     }
-    if constexpr (!CACHED) break;
+  }
+  if (threadIdx.x < 32) {
+    float entropy;
+    const bool live = teacher_row(a, row, t, &entropy);
+    if (threadIdx.x == 0) { entropy_s = entropy; live_s = live; }
   }
   sums = block_sums(sums, w, two, red);
+  const bool live = live_s != 0;
   const float log_soft = __log2f(sums.soft);
 
   // Loss, and the named columns' logits before the row may be overwritten.
-  const float z_target = target >= 0 ? to_float(src[target]) : 0.f;
+  const float z_target = target >= 0 ? to_float(in[target]) : 0.f;
   float cross = 0.f;
   for (int i = threadIdx.x; i < a.top; i += blockDim.x) {
-    const int c = column[i];
+    const int c = t.column[i];
     if (c < 0) continue;
-    z[i] = to_float(src[c]);
-    cross += p[i] * fmaf(z[i] - sums.m, w.k, -log_soft);
+    t.z[i] = to_float(in[c]);
+    cross += t.p[i] * fmaf(t.z[i] - sums.m, w.k, -log_soft);
   }
   cross = warp_sum(cross);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = cross;
   __syncthreads();
   if (threadIdx.x == 0) {
     float sum = 0.f;
-    for (int w = 0; w < int(blockDim.x >> 5); ++w) sum += red[w];
+    for (int k = 0; k < int(blockDim.x >> 5); ++k) sum += red[k];
     float l = live ? a.temperature * a.temperature * (entropy_s - kLn2 * sum) : 0.f;
     if (target >= 0) l += a.hard_weight * (kLn2 * __log2f(sums.hard) + (sums.m - z_target));
     *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(l, sums.m, sums.soft, sums.hard);
@@ -379,9 +575,9 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
   if (grad == nullptr) return;
   T* out = grad + row * a.vocab;
   const RowGrad g = row_grad(a, live, target >= 0, a.scale, sums.m, sums.soft, sums.hard, w);
-  write_gradient(src, cut, out, a.vocab, g);
+  write_gradient(in, cut, out, a.vocab, g);
   __syncthreads();
-  write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, p, column, z, target, z_target);
+  write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, target, z_target, blockDim.x);
 }
 
 template <typename T>
@@ -393,19 +589,17 @@ distill_bwd_kernel(const DistillArgs a, const float* __restrict__ stats, const f
   const int64_t row = blockIdx.x;
   const T* in = static_cast<const T*>(a.logits) + row * a.vocab;
   const Cut<T> cut(in, a.vocab);
-  float* p = reinterpret_cast<float*>(shared);
-  int* column = reinterpret_cast<int*>(p + a.top);
-  float* z = reinterpret_cast<float*>(column + a.top);
+  const Teacher t(shared, a.top);
   const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
   const int target = wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
   if (threadIdx.x < 32) {
     float entropy;
-    const bool live = teacher_row(a, row, p, column, &entropy);
+    const bool live = teacher_row(a, row, t, &entropy);
     if (threadIdx.x == 0) live_s = live;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.top; i += blockDim.x)
-    if (column[i] >= 0) z[i] = to_float(in[column[i]]);
+    if (t.column[i] >= 0) t.z[i] = to_float(in[t.column[i]]);
   const float z_target = target >= 0 ? to_float(in[target]) : 0.f;
   const float scale = a.scale * *grad_out;
   const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
@@ -413,7 +607,7 @@ distill_bwd_kernel(const DistillArgs a, const float* __restrict__ stats, const f
   T* out = grad + row * a.vocab;
   write_gradient(in, cut, out, a.vocab, g);
   __syncthreads();
-  write_named(a, out, g, a.temperature * scale, a.hard_weight * scale, p, column, z, target, z_target);
+  write_named(a, out, g, a.temperature * scale, a.hard_weight * scale, t, target, z_target, blockDim.x);
 }
 
 __global__ void __launch_bounds__(1024)
@@ -461,23 +655,26 @@ bool valid(const DistillArgs& a) {
 
 }  // namespace
 
-cudaError_t distill_fwd(DType type, const DistillArgs& a, float* stats, void* grad, cudaStream_t stream) {
+cudaError_t distill_fwd(DType type, const DistillArgs& a, float* stats, void* grad, int sms, cudaStream_t stream) {
   if (!valid(a)) return cudaErrorInvalidValue;
   if (a.rows == 0) return cudaSuccess;
+  const size_t slots = 3 * size_t(padded_slots(a.top)) * 4;
   MB_SWITCH_FLOAT(type, T, {
     const int64_t bytes = int64_t(a.vocab) * sizeof(T);
-    const int threads = row_threads(bytes);
-    const size_t slots = (3 * size_t(a.top) * 4 + 15) / 16 * 16;
-    if (grad != nullptr && bytes <= kSharedRow) {
-      const size_t shared = slots + size_t(bytes) + 32;
+    const int64_t row_bytes = (bytes + 15) / 16 * 16 + 16, shared = 2 * row_bytes + 3 * int64_t(slots);
+    if (grad != nullptr && shared <= kSharedBytes) {
+      auto kernel = distill_rows_kernel<T>;
       if (shared > 48 * 1024) {
-        const cudaError_t rc = cudaFuncSetAttribute(distill_fwd_kernel<T, true>,
-                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
         if (rc != cudaSuccess) return rc;
       }
-      distill_fwd_kernel<T, true><<<unsigned(a.rows), threads, shared, stream>>>(a, stats, static_cast<T*>(grad));
+      // As many CTAs as fit an SM, 24 warps between them, but no more than leave each thread four packs.
+      const int resident = max(1, int(min(int64_t(16), kSharedBytes / (shared + 1024))));
+      const int threads = max(32, min(kRowThreads / resident, int((bytes + 63) / 64)) / 32 * 32);
+      const int64_t grid = min(a.rows, int64_t(sms) * resident);
+      kernel<<<unsigned(grid), threads + 32, shared, stream>>>(a, int(row_bytes), stats, static_cast<T*>(grad));
     } else {
-      distill_fwd_kernel<T, false><<<unsigned(a.rows), threads, slots, stream>>>(a, stats, static_cast<T*>(grad));
+      distill_fwd_kernel<T><<<unsigned(a.rows), row_threads(bytes), slots, stream>>>(a, stats, static_cast<T*>(grad));
     }
   })
   return cudaGetLastError();
@@ -492,7 +689,7 @@ cudaError_t distill_bwd(DType type, const DistillArgs& a, const float* stats, co
                         cudaStream_t stream) {
   if (!valid(a)) return cudaErrorInvalidValue;
   if (a.rows == 0) return cudaSuccess;
-  const size_t slots = (3 * size_t(a.top) * 4 + 15) / 16 * 16;
+  const size_t slots = 3 * size_t(padded_slots(a.top)) * 4;
   MB_SWITCH_FLOAT(type, T, {
     distill_bwd_kernel<T><<<unsigned(a.rows), row_threads(int64_t(a.vocab) * sizeof(T)), slots, stream>>>(
         a, stats, grad_out, static_cast<T*>(grad));

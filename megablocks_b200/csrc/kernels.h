@@ -83,7 +83,7 @@ struct SelectArgs {
   bool use_sigmoid;
   float scale;
   const float* bias;                   // [experts], nullable
-  int group_lanes, aligned_lanes, shared_stride;       // filled by the launchers
+  int group_size, group_shift, aligned_shift;          // filled by the launchers
 };
 cudaError_t select_experts_fwd(DType type, const void* logits, SelectArgs args, void* scores, void* weights,
                                int64_t* ids, cudaStream_t stream);
@@ -110,7 +110,7 @@ struct DistillArgs {
 };
 // `stats` [rows, 4]: a row's loss, its largest logit and the sums of e^((z - max) / T) and e^(z - max);
 // with `grad` (may be the logits themselves) also the gradient of scale * sum(loss).
-cudaError_t distill_fwd(DType type, const DistillArgs& args, float* stats, void* grad, cudaStream_t stream);
+cudaError_t distill_fwd(DType type, const DistillArgs& args, float* stats, void* grad, int sms, cudaStream_t stream);
 // Mean of the rows' losses, in a fixed order.
 cudaError_t distill_mean(const float* stats, int64_t rows, float* mean, cudaStream_t stream);
 // The gradient alone, from the statistics of a forward pass, times *grad_out.

@@ -18,6 +18,7 @@ namespace mb {
 namespace {
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+int sm_count() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 
 DType float_code(at::ScalarType t) {
   switch (t) {
@@ -193,7 +194,8 @@ Distilled distill_forward(const at::Tensor& logits, const at::Tensor& values, co
   d.loss = at::empty({}, fopts);
   d.stats = at::empty({a.rows, 4}, fopts);        // loss, maximum, sums
   a.status = device_status(logits.device());
-  C10_CUDA_CHECK(distill_fwd(code, a, d.stats.data_ptr<float>(), want_grad ? d.grad.data_ptr() : nullptr, stream()));
+  C10_CUDA_CHECK(distill_fwd(code, a, d.stats.data_ptr<float>(), want_grad ? d.grad.data_ptr() : nullptr, sm_count(),
+                             stream()));
   C10_CUDA_CHECK(distill_mean(d.stats.data_ptr<float>(), a.rows, d.loss.data_ptr<float>(), stream()));
   count_launches(2);
   return d;
@@ -222,8 +224,7 @@ struct Distill : torch::autograd::Function<Distill> {
       ctx->saved_data.erase(kept);
       c10::cuda::CUDAGuard guard(out[0].device());
       C10_CUDA_CHECK(scale_unless_one(float_code(out[0].scalar_type()), out[0].data_ptr(), out[0].numel(),
-                                      scale.data_ptr<float>(),
-                                      at::cuda::getCurrentDeviceProperties()->multiProcessorCount, stream()));
+                                      scale.data_ptr<float>(), sm_count(), stream()));
       count_launches(1);
       return out;
     }

@@ -8,7 +8,7 @@
 // One warp owns a token and holds its experts in registers, PL consecutive ones a lane, fetched V at a time.
 // A lane with up to eight sorts them once, as keys whose last three bits are the place, and a round of the
 // choice is one reduction of the lanes' heads; it is bound by instructions (1678 a token with the places
-// compared anew in every round: 80 us for 32768 x 256).
+// compared anew in every round: 80 us for 32768 x 256).  FULL: the experts fill all places of all lanes.
 //
 // The order of the experts is exact: equal values go to the lowest id, and values that 32 bits cannot tell
 // apart are ordered by their 64-bit ones.  Without a bias the scores have the order of the logits, which are
@@ -51,12 +51,12 @@ struct alignas(sizeof(T) * V) Slots {
   T v[V];
 };
 
-template <typename T, int PL, int V>
+template <typename T, int PL, int V, bool FULL>
 __device__ __forceinline__ void load_slots(const T* row, int lane, int experts, float fill, float (&x)[PL]) {
 #pragma unroll
   for (int j = 0; j < PL; j += V) {
     const int e = expert_of<PL>(j, lane);
-    if (e < experts) {          // experts % V == 0
+    if (FULL || e < experts) {  // experts % V == 0
       const Slots<T, V> p = *reinterpret_cast<const Slots<T, V>*>(row + e);
 #pragma unroll
       for (int k = 0; k < V; ++k) x[j + k] = to_float(p.v[k]);
@@ -67,7 +67,26 @@ __device__ __forceinline__ void load_slots(const T* row, int lane, int experts, 
   }
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+template <typename T, int PL, int V, bool FULL>
+__device__ __forceinline__ void store_slots(T* row, int lane, int experts, const float (&x)[PL]) {
+#pragma unroll
+  for (int j = 0; j < PL; j += V) {
+    const int e = expert_of<PL>(j, lane);
+    if (FULL || e < experts) {
+      Slots<T, V> p;
+#pragma unroll
+      for (int k = 0; k < V; ++k) p.v[k] = from_float<T>(x[j + k]);
+      *reinterpret_cast<Slots<T, V>*>(row + e) = p;
+    }
+  }
+}
+
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid(float x) { return reciprocal(1.f + __expf(-x)); }
 
 // Scores of a lane's slots; returns what a single score needs to be taken again (maximum and inverse sum
 // of the softmax) and the sum of all scores.
@@ -75,7 +94,7 @@ struct RowStat {
   float top, inv, total;
 };
 
-template <int PL, int V>
+template <int PL, bool FULL>
 __device__ __forceinline__ RowStat scores_of(const float (&x)[PL], int lane, int experts, bool use_sigmoid,
                                              float (&s)[PL]) {
   RowStat r{0.f, 1.f, 0.f};
@@ -83,7 +102,8 @@ __device__ __forceinline__ RowStat scores_of(const float (&x)[PL], int lane, int
   if (use_sigmoid) {
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-      s[j] = expert_of<PL>(j, lane) < experts ? sigmoid(x[j]) : 0.f;
+      s[j] = sigmoid(x[j]);
+      if (!FULL && expert_of<PL>(j, lane) >= experts) s[j] = 0.f;
       sum += s[j];
     }
     r.total = warp_sum_f(sum);
@@ -96,7 +116,8 @@ __device__ __forceinline__ RowStat scores_of(const float (&x)[PL], int lane, int
     r.top = top == -INFINITY ? 0.f : top;         // nothing but -inf: every score is zero
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-      s[j] = expert_of<PL>(j, lane) < experts ? __expf(x[j] - r.top) : 0.f;
+      s[j] = __expf(x[j] - r.top);
+      if (!FULL && expert_of<PL>(j, lane) >= experts) s[j] = 0.f;
       sum += s[j];
     }
     sum = warp_sum_f(sum);
@@ -136,7 +157,7 @@ __device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, doubl
   }
   __syncwarp();
   unsigned kept = 0xffffffffu;
-  const int size = E / a.groups;
+  const int size = a.group_size;
   if (a.top_groups < a.groups) {
     double value = -INFINITY;
     if (lane < a.groups) {
@@ -197,28 +218,30 @@ __device__ __forceinline__ void sort_down(unsigned (&k)[N]) {
           }
 }
 
-// The two largest of a group that spans `lanes` lanes, in all of them.
-__device__ __forceinline__ void join_best(float& b1, float& b2, int lanes) {
-  for (int d = lanes / 2; d > 0; d >>= 1) {
+// The two largest of a group that spans 2^shift lanes, in all of them.
+__device__ __forceinline__ void join_best(float& b1, float& b2, int shift) {
+  for (int d = 1 << shift >> 1; d > 0; d >>= 1) {
     const float o1 = __shfl_xor_sync(0xffffffffu, b1, d), o2 = __shfl_xor_sync(0xffffffffu, b2, d);
     b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
     b1 = fmaxf(b1, o1);
   }
 }
 
-// Whether this lane's group stays, as lane bits: bit (g * lanes per group).  `b1`, `b2`: the largest values of
-// group lane / lanes.  Sets `doubt` when the last group that stays and the next are closer than the arithmetic
-// tells apart.
-__device__ __forceinline__ unsigned choose_groups(float b1, float b2, int lanes, int size, const SelectArgs& a, int lane,
+// Whether groups stay, as lane bits: bit g << shift.  `b1`, `b2`: the largest values of group lane >> shift.  The
+// lanes of a group share its comparisons.  Sets `doubt` when the last group that stays and the next are closer
+// than the arithmetic tells apart.
+__device__ __forceinline__ unsigned choose_groups(float b1, float b2, int shift, const SelectArgs& a, int lane,
                                                   float margin, bool& doubt) {
-  const int g = lane / lanes;
+  const int g = lane >> shift;
   const bool there = g < a.groups;
-  const unsigned value = there ? ordered(size > 1 ? b1 + b2 : b1) : 0u;
+  const unsigned value = there ? ordered(a.group_size > 1 ? b1 + b2 : b1) : 0u;
   int rank = 0;
-  for (int h = 0; h < a.groups; ++h) {
-    const unsigned o = __shfl_sync(0xffffffffu, value, h * lanes);
-    rank += o > value || (o == value && h < g);
+  for (int h = 0; h < a.groups; h += 1 << shift) {
+    const int other = h + (lane & ((1 << shift) - 1));                // of another group's number
+    const unsigned o = __shfl_sync(0xffffffffu, value, other << shift);
+    rank += other < a.groups && (o > value || (o == value && other < g));
   }
+  for (int d = 1 << shift >> 1; d > 0; d >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
   const bool stays = there && rank < a.top_groups;
   const float last = from_ordered(__reduce_min_sync(0xffffffffu, stays ? value : 0xffffffffu));
   const float next = from_ordered(__reduce_max_sync(0xffffffffu, stays ? 0u : value));
@@ -226,7 +249,7 @@ __device__ __forceinline__ unsigned choose_groups(float b1, float b2, int lanes,
   return __ballot_sync(0xffffffffu, stays);
 }
 
-template <typename T, int PL, int V>
+template <typename T, int PL, int V, bool FULL>
 __global__ void __launch_bounds__(kWarps * 32)
 select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restrict__ scores, T* __restrict__ weights,
                   int64_t* __restrict__ ids) {
@@ -238,18 +261,14 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
   if (t >= a.tokens) return;
   const T* row = logits + t * E;
   float x[PL], s[PL];
-  load_slots<T, PL, V>(row, lane, E, -INFINITY, x);
-  const RowStat r = scores_of<PL, V>(x, lane, E, a.use_sigmoid, s);
-  const float inv_total = a.use_sigmoid && r.total != 0.f ? 1.f / r.total : 1.f;
+  load_slots<T, PL, V, FULL>(row, lane, E, -INFINITY, x);
+  const RowStat r = scores_of<PL, FULL>(x, lane, E, a.use_sigmoid, s);
+  {
+    const float inv_total = a.use_sigmoid && r.total != 0.f ? reciprocal(r.total) : 1.f;
+    float out[PL];
 #pragma unroll
-  for (int j = 0; j < PL; j += V) {
-    const int e = expert_of<PL>(j, lane);
-    if (e < E) {
-      Slots<T, V> p;
-#pragma unroll
-      for (int k = 0; k < V; ++k) p.v[k] = from_float<T>(s[j + k] * inv_total);
-      *reinterpret_cast<Slots<T, V>*>(scores + t * E + e) = p;
-    }
+    for (int j = 0; j < PL; ++j) out[j] = s[j] * inv_total;
+    store_slots<T, PL, V, FULL>(scores + t * E, lane, E, out);
   }
 
   // Twice the error of a score: exponent's rounding and unit, division, sum (1.6 x 2^-22 for the sigmoid,
@@ -257,54 +276,64 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
   // bias and the bits that a key gives to the place come on top: 2^-20 of the values.
   const float margin = a.use_sigmoid ? 0x1p-20f : 0x1p-18f * r.inv;
   const bool biased = a.bias != nullptr;
-  float* const mine_shared = reinterpret_cast<float*>(shared + warp * a.shared_stride);
+  float* const mine_shared = reinterpret_cast<float*>(shared + warp * E);
   const bool grouped = a.top_groups < a.groups;
   bool doubt = false;
   unsigned key[PL];
+  if (biased) {
+    float add[PL];
+    // 16-byte bias vectors; the launcher sees to the alignment where V > 1.
+    load_slots<float, PL, (V > 4 ? 4 : V), FULL>(a.bias, lane, E, 0.f, add);
+#pragma unroll
+    for (int j = 0; j < PL; ++j) s[j] += add[j];
+  }
 #pragma unroll
   for (int j = 0; j < PL; ++j) {
     const int e = expert_of<PL>(j, lane);
-    const bool there = e < E;
-    const float c = biased && there ? s[j] + __ldg(a.bias + e) : s[j];
-    if (grouped && a.aligned_lanes == 0 && there) mine_shared[padded_slot(e)] = c != c ? INFINITY : c;
-    s[j] = c;
-    key[j] = there ? (ordered(biased ? c : x[j]) & ~kPlace) | (kPlace - (unsigned(j) & kPlace)) : 0u;
+    const bool there = FULL || e < E;
+    if (grouped && a.aligned_shift < 0 && there) mine_shared[padded_slot(e)] = s[j] != s[j] ? INFINITY : s[j];
+    const unsigned k = (ordered(biased ? s[j] : x[j]) & ~kPlace) | (kPlace - (unsigned(j) & kPlace));
+    key[j] = there ? k : 0u;
   }
   if constexpr (kSorted) sort_down(key);
   if (grouped) {
-    const int size = E / a.groups;
     float b1 = -INFINITY, b2 = -INFINITY;
-    if (a.aligned_lanes > 0) {                            // groups of whole lanes, a power of two of them
+    if (a.aligned_shift >= 0) {                           // groups of whole lanes, a power of two of them
+      if (kSorted && biased) {                            // the places' bits are within what `doubt` allows
+        b1 = key[0] != 0u ? from_ordered(key[0] & ~kPlace) : -INFINITY;
+        if (PL > 1) b2 = key[PL > 1 ? 1 : 0] != 0u ? from_ordered(key[PL > 1 ? 1 : 0] & ~kPlace) : -INFINITY;
+      } else {
 #pragma unroll
-      for (int j = 0; j < PL; ++j) {
-        const float v = expert_of<PL>(j, lane) < E ? (s[j] != s[j] ? INFINITY : s[j]) : -INFINITY;
-        b2 = fmaxf(b2, fminf(b1, v));
-        b1 = fmaxf(b1, v);
+        for (int j = 0; j < PL; ++j) {
+          const float v = FULL || expert_of<PL>(j, lane) < E ? (s[j] != s[j] ? INFINITY : s[j]) : -INFINITY;
+          b2 = fmaxf(b2, fminf(b1, v));
+          b1 = fmaxf(b1, v);
+        }
       }
-      join_best(b1, b2, a.aligned_lanes);
-      const unsigned stays = choose_groups(b1, b2, a.aligned_lanes, size, a, lane, margin, doubt);
-      if (!(stays >> (lane / a.aligned_lanes * a.aligned_lanes) & 1u)) {
+      join_best(b1, b2, a.aligned_shift);
+      const unsigned stays = choose_groups(b1, b2, a.aligned_shift, a, lane, margin, doubt);
+      if (!(stays >> (lane >> a.aligned_shift << a.aligned_shift) & 1u)) {
 #pragma unroll
         for (int j = 0; j < PL; ++j) key[j] = 0u;
       }
     } else {
       __syncwarp();
-      const int lanes = a.group_lanes, g = lane / lanes;
+      const int shift = a.group_shift, g = lane >> shift;
       if (g < a.groups) {
-        for (int i = lane % lanes; i < size; i += lanes) {
-          const float v = mine_shared[padded_slot(g * size + i)];
+        for (int i = lane & ((1 << shift) - 1); i < a.group_size; i += 1 << shift) {
+          const float v = mine_shared[padded_slot(g * a.group_size + i)];
           b2 = fmaxf(b2, fminf(b1, v));
           b1 = fmaxf(b1, v);
         }
       }
-      join_best(b1, b2, lanes);
-      const unsigned stays = choose_groups(b1, b2, lanes, size, a, lane, margin, doubt);
-      const float inv_size = float(a.groups) / float(E);
+      join_best(b1, b2, shift);
+      const unsigned stays = choose_groups(b1, b2, shift, a, lane, margin, doubt);
+      const float inv_size = 1.f / float(a.group_size);
 #pragma unroll
       for (int j = 0; j < PL; ++j) {
         const int place = kSorted ? int(kPlace - (key[j] & kPlace)) : j;
         const int g2 = int((lane * PL + place + 0.5f) * inv_size);           // exact: at most 1024 experts
-        if (!(stays >> (g2 * lanes & 31) & 1u)) key[j] = 0u;
+        if (!(stays >> (g2 << shift & 31) & 1u)) key[j] = 0u;
       }
       if constexpr (kSorted) sort_down(key);
     }
@@ -366,7 +395,7 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
   }
   if (doubt) {
     __syncwarp();
-    mine = choose_wide<T>(row, a, shared + warp * a.shared_stride, lane);
+    mine = choose_wide<T>(row, a, shared + warp * E, lane);
   }
 
   const bool live = lane < a.top_k;
@@ -385,7 +414,7 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
 
 // dlogits from the gradients of the weights and (optionally) of the scores.  The scores are taken again
 // from the logits, which costs the bytes that stored scores would and keeps their 32 bits.
-template <typename T, int PL, int V>
+template <typename T, int PL, int V, bool FULL>
 __global__ void __launch_bounds__(kWarps * 32)
 select_bwd_kernel(const T* __restrict__ logits, const SelectArgs a, const int64_t* __restrict__ ids,
                   const T* __restrict__ dscores, int64_t dscores_stride, const T* __restrict__ dweights,
@@ -402,8 +431,8 @@ select_bwd_kernel(const T* __restrict__ logits, const SelectArgs a, const int64_
   RowStat r{0.f, 1.f, 0.f};
   const bool whole = !a.use_sigmoid || dscores != nullptr;      // more than the chosen experts' own logits
   if (whole) {
-    load_slots<T, PL, V>(row, lane, E, -INFINITY, x);
-    r = scores_of<PL, V>(x, lane, E, a.use_sigmoid, s);
+    load_slots<T, PL, V, FULL>(row, lane, E, -INFINITY, x);
+    r = scores_of<PL, FULL>(x, lane, E, a.use_sigmoid, s);
   }
   const float w = live ? score_at(mine_x, r, a.use_sigmoid) : 0.f;
   float dsel = dw;
@@ -417,7 +446,7 @@ select_bwd_kernel(const T* __restrict__ logits, const SelectArgs a, const int64_
   float g[PL];
   float inner = 0.f, inv_total = 1.f;
   if (dscores != nullptr) {
-    load_slots<T, PL, V>(dscores + t * dscores_stride, lane, E, 0.f, g);
+    load_slots<T, PL, V, FULL>(dscores + t * dscores_stride, lane, E, 0.f, g);
 #pragma unroll
     for (int j = 0; j < PL; ++j) inner += g[j] * s[j];
     if (a.use_sigmoid && r.total != 0.f) inv_total = 1.f / r.total;
@@ -425,22 +454,17 @@ select_bwd_kernel(const T* __restrict__ logits, const SelectArgs a, const int64_
   // softmax: inner = <ds, s> with both gradients; sigmoid: <g, scores> of the scores' gradient alone.
   inner = a.use_sigmoid ? (dscores != nullptr ? warp_sum_f(inner) * inv_total : 0.f) : warp_sum_f(inner + dsel * w);
   T* out = dlogits + t * E;
+  {
+    float d[PL];
 #pragma unroll
-  for (int j = 0; j < PL; j += V) {
-    const int e = expert_of<PL>(j, lane);
-    if (e < E) {
-      Slots<T, V> p;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        float d = 0.f;
-        if (whole) {
-          const float gs = dscores != nullptr ? g[j + k] : 0.f;
-          d = a.use_sigmoid ? (gs - inner) * inv_total * s[j + k] * sigmoid(-x[j + k]) : s[j + k] * (gs - inner);
-        }
-        p.v[k] = from_float<T>(d);
+    for (int j = 0; j < PL; ++j) {
+      d[j] = 0.f;
+      if (whole) {
+        const float gs = dscores != nullptr ? g[j] : 0.f;
+        d[j] = a.use_sigmoid ? (gs - inner) * inv_total * s[j] * sigmoid(-x[j]) : s[j] * (gs - inner);
       }
-      *reinterpret_cast<Slots<T, V>*>(out + e) = p;
     }
+    store_slots<T, PL, V, FULL>(out, lane, E, d);
   }
   __syncwarp();               // the chosen experts' values over the ones just stored
   if (live) {
@@ -458,21 +482,23 @@ bool row_vectors(int experts, const void* p) {
 }
 
 // PL slots a lane, fetched up to 16 bytes at a time where the rows allow it, else one by one.
-#define MB_SELECT_SWITCH(T, experts, aligned, CALL)                       \
-  if (experts <= 32) { CALL(1, 1); }                                      \
-  else if (experts <= 64) { if (aligned(2)) { CALL(2, 2); } else { CALL(2, 1); } } \
-  else if (experts <= 128) { if (aligned(4)) { CALL(4, 4); } else { CALL(4, 1); } } \
-  else {                                                                  \
-    constexpr int W = 16 / sizeof(T);                                     \
-    if (experts <= 256) { if (aligned(W)) { CALL(8, W); } else { CALL(8, 1); } }        \
-    else if (experts <= 512) { if (aligned(W)) { CALL(16, W); } else { CALL(16, 1); } } \
-    else { if (aligned(W)) { CALL(32, W); } else { CALL(32, 1); } }       \
-  }
+#define MB_SELECT_ONE(PL, V, aligned, CALL)                               \
+  if (!aligned(V)) { CALL(PL, 1, false); }                                \
+  else if (a.experts == 32 * PL) { CALL(PL, V, true); }                   \
+  else { CALL(PL, V, false); }
+#define MB_SELECT_SWITCH(T, aligned, CALL)                                \
+  constexpr int W = 16 / sizeof(T);                                       \
+  if (a.experts <= 32) { CALL(1, 1, false); }                             \
+  else if (a.experts <= 64) { MB_SELECT_ONE(2, 2, aligned, CALL) }        \
+  else if (a.experts <= 128) { MB_SELECT_ONE(4, 4, aligned, CALL) }       \
+  else if (a.experts <= 256) { MB_SELECT_ONE(8, W, aligned, CALL) }       \
+  else if (a.experts <= 512) { MB_SELECT_ONE(16, W, aligned, CALL) }      \
+  else { MB_SELECT_ONE(32, W, aligned, CALL) }
 
-int slots_per_lane(int experts) {
-  int n = 1;
-  while (n * 32 < experts) n *= 2;
-  return n;
+int ceil_log2(int n) {
+  int bits = 0;
+  while (1 << bits < n) ++bits;
+  return bits;
 }
 
 bool complete(SelectArgs& a) {
@@ -480,13 +506,13 @@ bool complete(SelectArgs& a) {
   if (a.groups < 1 || a.groups > kSelectMaxGroups || a.experts % a.groups != 0 || a.top_groups < 1 ||
       a.top_groups > a.groups || a.top_k > a.top_groups * (a.experts / a.groups) || a.norm_p < 0 || a.norm_p > 2)
     return false;
-  a.group_lanes = 1;
-  while (a.group_lanes * 2 * a.groups <= 32) a.group_lanes *= 2;
-  // Lanes of a group where it takes whole ones, a power of two of them; 0: it does not.
-  const int size = a.experts / a.groups, per_lane = slots_per_lane(a.experts);
-  const int span = size % per_lane == 0 ? size / per_lane : 0;
-  a.aligned_lanes = span > 0 && (span & (span - 1)) == 0 && span * a.groups <= 32 ? span : 0;
-  a.shared_stride = a.experts;
+  a.group_size = a.experts / a.groups;
+  a.group_shift = 0;
+  while (2 << a.group_shift << ceil_log2(a.groups) <= 32) ++a.group_shift;
+  // Lanes of a group where it takes whole ones, a power of two of them.
+  const int per_lane = 1 << ceil_log2((a.experts + 31) / 32);
+  const int span = a.group_size % per_lane == 0 ? a.group_size / per_lane : 0;
+  a.aligned_shift = span > 0 && (span & (span - 1)) == 0 && span * a.groups <= 32 ? ceil_log2(span) : -1;
   return true;
 }
 
@@ -496,13 +522,15 @@ cudaError_t select_experts_fwd(DType type, const void* logits, SelectArgs a, voi
                                int64_t* ids, cudaStream_t stream) {
   if (!complete(a)) return cudaErrorInvalidValue;
   if (a.tokens == 0) return cudaSuccess;
-  const size_t shared = size_t(a.shared_stride) * kWarps * sizeof(double);      // at most 32 KB
+  const size_t shared = size_t(a.experts) * kWarps * sizeof(double);       // at most 32 KB
   MB_SWITCH_FLOAT(type, T, {
-#define MB_SELECT_ALIGNED(v) (row_vectors<T, v>(a.experts, logits) && row_vectors<T, v>(a.experts, scores))
-#define MB_SELECT_FWD(PL, V)                                                                                     \
-  select_fwd_kernel<T, PL, V><<<ceil_div(a.tokens, kWarps), kWarps * 32, shared, stream>>>(                      \
+#define MB_SELECT_ALIGNED(v)                                                                                     \
+  (row_vectors<T, v>(a.experts, logits) && row_vectors<T, v>(a.experts, scores) &&                                \
+   row_vectors<float, (v > 4 ? 4 : v)>(a.experts, a.bias))
+#define MB_SELECT_FWD(PL, V, FULL)                                                                               \
+  select_fwd_kernel<T, PL, V, FULL><<<ceil_div(a.tokens, kWarps), kWarps * 32, shared, stream>>>(                      \
       static_cast<const T*>(logits), a, static_cast<T*>(scores), static_cast<T*>(weights), ids)
-    MB_SELECT_SWITCH(T, a.experts, MB_SELECT_ALIGNED, MB_SELECT_FWD)
+    MB_SELECT_SWITCH(T, MB_SELECT_ALIGNED, MB_SELECT_FWD)
   })
 #undef MB_SELECT_FWD
 #undef MB_SELECT_ALIGNED
@@ -517,11 +545,11 @@ cudaError_t select_experts_bwd(DType type, const void* logits, SelectArgs a, con
 #define MB_SELECT_ALIGNED(v)                                                              \
   (row_vectors<T, v>(a.experts, logits) && row_vectors<T, v>(a.experts, dlogits) &&        \
    (dscores == nullptr || row_vectors<T, v>(a.experts, dscores)))
-#define MB_SELECT_BWD(PL, V)                                                                                     \
-  select_bwd_kernel<T, PL, V><<<ceil_div(a.tokens, kWarps), kWarps * 32, 0, stream>>>(                           \
+#define MB_SELECT_BWD(PL, V, FULL)                                                                               \
+  select_bwd_kernel<T, PL, V, FULL><<<ceil_div(a.tokens, kWarps), kWarps * 32, 0, stream>>>(                           \
       static_cast<const T*>(logits), a, ids, static_cast<const T*>(dscores), dscores_stride,                     \
       static_cast<const T*>(dweights), static_cast<T*>(dlogits))
-    MB_SELECT_SWITCH(T, a.experts, MB_SELECT_ALIGNED, MB_SELECT_BWD)
+    MB_SELECT_SWITCH(T, MB_SELECT_ALIGNED, MB_SELECT_BWD)
   })
 #undef MB_SELECT_BWD
 #undef MB_SELECT_ALIGNED
