@@ -4,14 +4,14 @@
 //   loss = T^2 sum_i p_i (log p_i - log q_{id_i}) + hard * (logsumexp(z) - z_target)
 //   dloss / dz_j = T (q_j - sum_{i: id_i = j} p_i) + hard * (softmax(z)_j - [j = target])
 //
-// Bound by memory: a logit is read once and its gradient written once.  Where two rows fit shared memory, CTAs
-// stay and walk the rows: a row's successor is fetched by bulk copies while the row is worked on, in three
-// passes over shared memory (maximum; sums; gradient, stored straight to memory), and a warp of its own
-// prepares the teacher's probabilities of the next row meanwhile.  A CTA a row, with two on an SM, took twice
-// as long (542 against 279 us for 8192 rows of 51200 bf16): each phase of a row left another unit idle.
-// Longer rows, and passes without a gradient, stream the row from memory with a running maximum; a gradient
-// then reads it again, from L2.  The few columns that the teacher or the target names are written again, with
-// their whole value and one rounding, after the row.
+// Bound by memory: a logit is read once and its gradient written once.  Where a row fits shared memory, CTAs
+// stay and walk the rows.  A row is fetched by bulk copies, in chunks, and worked on in three passes over shared
+// memory (maximum; sums; gradient, stored straight to memory); the last pass hands its chunks back, and a warp
+// of its own fetches the next row's into them and prepares the next row's teacher.  Two CTAs share an SM where
+// two rows fit, so that one takes exponentials, of which there are two a logit, while the other waits for a
+// sum or a copy.  Longer rows, and passes without a gradient, stream the row from memory with a running maximum;
+// a gradient then reads it again, from L2.  The few columns that the teacher or the target names are written
+// again, with their whole value and one rounding, after the row.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -19,23 +19,69 @@ namespace mb {
 
 namespace {
 
-constexpr int kCopies = 8;                        // bulk copies of a row
+constexpr int kChunks = 8;                        // most chunks of a row in shared memory
 constexpr int kMaxThreads = 512;
 constexpr int kRowThreads = 768;                  // most threads that work on a row in shared memory
 constexpr int kSharedBytes = 226 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-  T v[N];
-};
+// 16 bytes of logits as pairs of fp32 values, on which the arithmetic runs two to an instruction.
+template <typename T>
+constexpr int kPairs = 8 / sizeof(T);
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, float2 (&x)[kPairs<T>]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (std::is_same<T, float>::value) {
+    x[0] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    x[1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        x[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      else
+        x[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float2 (&x)[kPairs<T>]) {
+  uint32_t w[4];
+  if constexpr (std::is_same<T, float>::value) {
+    w[0] = __float_as_uint(x[0].x), w[1] = __float_as_uint(x[0].y);
+    w[2] = __float_as_uint(x[1].x), w[3] = __float_as_uint(x[1].y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 q = __floats2bfloat162_rn(x[i].x, x[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&q);
+      } else {
+        const __half2 q = __floats2half2_rn(x[i].x, x[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&q);
+      }
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 load_shared(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ float2 splat2(float v) { return make_float2(v, v); }
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(exp2_approx(x.x), exp2_approx(x.y)); }
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -78,30 +124,48 @@ struct Powers {
     if (squares == 2) first *= first;
     return first;
   }
+  __device__ __forceinline__ float2 second(float2 first, float2 x_minus_max) const {
+    if (squares == 3) return exp2_pair(__fmul2_rn(x_minus_max, splat2(kLog2e)));
+    if (squares >= 1) first = __fmul2_rn(first, first);
+    if (squares == 2) first = __fmul2_rn(first, first);
+    return first;
+  }
 };
 
 // Running maximum and sums.  Differences are taken before they are scaled, so that logits far from zero
 // lose nothing.
 struct Online {
   float m = -INFINITY, soft = 0.f, hard = 0.f;
-  template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], const Powers& w, bool two) {
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  __device__ __forceinline__ void raise(float top, const Powers& w, bool two) {
     if (top > m) {
       const float f = exp2_approx((m - top) * w.k);
       if (two) hard *= w.second(f, m - top);
       soft *= f;
       m = top;
     }
-    const float base = m == -INFINITY ? 0.f : m;
+  }
+  __device__ __forceinline__ void add(float x, const Powers& w, bool two) {
+    raise(x, w, two);
+    const float d = x - (m == -INFINITY ? 0.f : m), e = exp2_approx(d * w.k);
+    soft += e;
+    if (two) hard += w.second(e, d);
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float2 (&x)[N], const Powers& w, bool two) {
+    float2 top = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = make_float2(fmaxf(top.x, x[i].x), fmaxf(top.y, x[i].y));
+    raise(fmaxf(top.x, top.y), w, two);
+    const float2 minus = splat2(m == -INFINITY ? 0.f : -m), k2 = splat2(w.k);
+    float2 s = splat2(0.f), h = s;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float e = exp2_approx((x[i] - base) * w.k);
-      soft += e;
-      if (two) hard += w.second(e, x[i] - base);
+      const float2 d = __fadd2_rn(x[i], minus), e = exp2_pair(__fmul2_rn(d, k2));
+      s = __fadd2_rn(s, e);
+      if (two) h = __fadd2_rn(h, w.second(e, d));
     }
+    soft += s.x + s.y;
+    hard += h.x + h.y;
   }
 };
 
@@ -211,20 +275,27 @@ struct RowGrad {
 };
 
 template <int N>
-__device__ __forceinline__ void gradient(const RowGrad& g, float (&x)[N]) {
+__device__ __forceinline__ void gradient(const RowGrad& g, float2 (&x)[N]) {
   if (g.soft == 0.f && g.hard == 0.f) {           // nothing to learn from this row, whatever its logits
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    for (int i = 0; i < N; ++i) x[i] = splat2(0.f);
   } else if (g.hard == 0.f) {
+    const float2 k2 = splat2(g.w.k), minus = splat2(-g.offset), soft = splat2(g.soft);
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = g.soft * exp2_approx(fmaf(x[i], g.w.k, -g.offset));
+    for (int i = 0; i < N; ++i) x[i] = __fmul2_rn(soft, exp2_pair(__ffma2_rn(x[i], k2, minus)));
   } else {
+    const float2 k2 = splat2(g.w.k), minus = splat2(-g.max), soft = splat2(g.soft), hard = splat2(g.hard);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float e = exp2_approx((x[i] - g.max) * g.w.k);
-      x[i] = fmaf(g.hard, g.w.second(e, x[i] - g.max), g.soft * e);
+      const float2 d = __fadd2_rn(x[i], minus), e = exp2_pair(__fmul2_rn(d, k2));
+      x[i] = __ffma2_rn(hard, g.w.second(e, d), __fmul2_rn(soft, e));
     }
   }
+}
+__device__ __forceinline__ float gradient(const RowGrad& g, float z) {
+  float2 x[1] = {make_float2(z, z)};
+  gradient(g, x);
+  return x[0].x;
 }
 
 __device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, bool live, bool has_target, float scale, float max,
@@ -243,29 +314,30 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, bool live, boo
   return g;
 }
 
-// Writes a row's gradient; `src` is the row in shared or global memory (`grad` itself, possibly).
+// Writes a row's gradient over a row in memory (`grad` itself, possibly).
 template <typename T>
 __device__ __forceinline__ void write_gradient(const T* src, const Cut<T>& cut, T* grad, int vocab, const RowGrad& g) {
   constexpr int VEC = 16 / sizeof(T);
-  const bool vector = reinterpret_cast<uintptr_t>(src + cut.head) % 16 == 0 &&
-                      reinterpret_cast<uintptr_t>(grad + cut.head) % 16 == 0;
-  auto one = [&](int i) {
-    float x[1] = {to_float(src[i])};
-    gradient(g, x);
-    grad[i] = from_float<T>(x[0]);
-  };
-  if (vector) {
+  auto one = [&](int i) { grad[i] = from_float<T>(gradient(g, to_float(src[i]))); };
+  if (reinterpret_cast<uintptr_t>(grad + cut.head) % 16 == 0) {
     if (int(threadIdx.x) < cut.head) one(threadIdx.x);
     if (int(threadIdx.x) < cut.tail) one(vocab - cut.tail + threadIdx.x);
-    for (int p = threadIdx.x; p < cut.packs; p += blockDim.x) {
-      Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(src + cut.head + p * VEC);
-      float x[VEC];
+    const uint4* from = reinterpret_cast<const uint4*>(src + cut.head);
+    uint4* to = reinterpret_cast<uint4*>(grad + cut.head);
+    constexpr int kAhead = 4;          // packs of a thread in flight
+    for (int i = threadIdx.x; i < cut.packs; i += kAhead * blockDim.x) {
+      uint4 v[kAhead];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = to_float(v.v[k]);
-      gradient(g, x);
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u * int(blockDim.x) < cut.packs) v[u] = from[i + u * blockDim.x];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v.v[k] = from_float<T>(x[k]);
-      *reinterpret_cast<Pack<T, VEC>*>(grad + cut.head + p * VEC) = v;
+      for (int u = 0; u < kAhead; ++u) {
+        if (i + u * int(blockDim.x) >= cut.packs) break;
+        float2 x[kPairs<T>];
+        unpack<T>(v[u], x);
+        gradient(g, x);
+        to[i + u * blockDim.x] = pack<T>(x);
+      }
     }
   } else {
     for (int i = threadIdx.x; i < vocab; i += blockDim.x) one(i);
@@ -291,15 +363,10 @@ __device__ __forceinline__ void write_named(const DistillArgs& a, T* grad, const
       }
       if (!first) continue;
     }
-    float x[1] = {t.z[i]};
-    gradient(g, x);
-    grad[c] = from_float<T>(x[0] - soft_scale * share - (c == target ? hard_scale : 0.f));
+    grad[c] = from_float<T>(gradient(g, t.z[i]) - soft_scale * share - (c == target ? hard_scale : 0.f));
   }
-  if (int(threadIdx.x) == threads - 1 && target >= 0 && !named_elsewhere(t, a.top, target, -1)) {
-    float x[1] = {z_target};
-    gradient(g, x);
-    grad[target] = from_float<T>(x[0] - hard_scale);
-  }
+  if (int(threadIdx.x) == threads - 1 && target >= 0 && !named_elsewhere(t, a.top, target, -1))
+    grad[target] = from_float<T>(gradient(g, z_target) - hard_scale);
 }
 
 __device__ __forceinline__ Powers powers(const DistillArgs& a) {
@@ -307,14 +374,11 @@ __device__ __forceinline__ Powers powers(const DistillArgs& a) {
   return {kLog2e / t, t == 1.f ? 0 : (t == 2.f ? 1 : (t == 4.f ? 2 : 3))};
 }
 
-// Maximum of a pack; of 16-bit types in their own arithmetic, which is exact.
-template <typename T, int N>
-__device__ __forceinline__ float pack_max(const Pack<T, N>& v) {
+// Maximum of 16 bytes; of 16-bit types in their own arithmetic, which is exact.
+template <typename T>
+__device__ __forceinline__ float pack_max(const uint4& v) {
   if constexpr (sizeof(T) == 4) {
-    float m = v.v[0];
-#pragma unroll
-    for (int k = 1; k < N; ++k) m = fmaxf(m, v.v[k]);
-    return m;
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
   } else {
     using P2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
     const P2* q = reinterpret_cast<const P2*>(&v);
@@ -324,60 +388,71 @@ __device__ __forceinline__ float pack_max(const Pack<T, N>& v) {
 }
 
 // Rows in shared memory.  All warps but the last work on a row; the last fetches the next one and prepares its
-// teacher.  `row_bytes`: room for a row, a multiple of 16 with 16 to spare for its phase.
+// teacher.  Shared memory holds the 16-byte blocks of memory that a row touches, `chunk` blocks to a chunk.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads + 32)
-distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stats, T* grad) {
+distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __restrict__ stats, T* grad) {
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ float red[4][kRowThreads / 32];
-  __shared__ alignas(8) uint64_t full[2];
+  __shared__ alignas(8) uint64_t full[kChunks], empty[kChunks];
   __shared__ int abort_flag;
   __shared__ float entropy_s[3];
   __shared__ int live_s[3];
   const int threads = blockDim.x - 32, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slots = padded_slots(a.top);
-  float* teachers = reinterpret_cast<float*>(shared + 2 * row_bytes);      // [3]
+  float* teachers = reinterpret_cast<float*>(shared + row_bytes);          // [3]
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    ptx::mbar_init(ptx::smem_u32(&full[0]), 1);
-    ptx::mbar_init(ptx::smem_u32(&full[1]), 1);
+    for (int c = 0; c < kChunks; ++c) {
+      ptx::mbar_init(ptx::smem_u32(&full[c]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty[c]), warps);
+    }
     ptx::fence_barrier_init();
   }
   __syncthreads();
   auto row_of = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
-  auto place_of = [&](int64_t row, int buffer) {                           // where a row's element 0 lies (or would)
-    return reinterpret_cast<T*>(shared + buffer * row_bytes + reinterpret_cast<uintptr_t>(row_of(row)) % 16);
-  };
+  const uint32_t blocks = ptx::smem_u32(shared);
 
   if (warp == warps) {
     // The teacher has three places: the named columns of the row before are still being written.
-    auto prepare = [&](int64_t row, int buffer, int set) {
-      if (row >= a.rows) return;
-      if (lane == 0) {
+    int set = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto prepare = [&](int64_t row, bool again) {
+      if (row < a.rows) {
+        float entropy;
+        const bool live = teacher_row(a, row, Teacher(teachers + set * 3 * slots, a.top), &entropy);
+        if (lane == 0) { entropy_s[set] = entropy; live_s[set] = live; }
         const T* in = row_of(row);
         const Cut<T> cut(in, a.vocab);
-        const uint32_t bar = ptx::smem_u32(&full[buffer]);
-        T* copy = place_of(row, buffer);
-        ptx::mbar_arrive_expect_tx(bar, uint32_t(cut.packs) * 16);
-        const int piece = (cut.packs + kCopies - 1) / kCopies;
-        for (int c = 0; c < cut.packs; c += piece)
-          ptx::bulk_load(ptx::smem_u32(copy + cut.head + c * VEC), in + cut.head + c * VEC,
-                         uint32_t(min(piece, cut.packs - c)) * 16, bar);
+        const int first = cut.head > 0 ? 1 : 0, last = first + cut.packs;  // blocks that are whole
+        const T* block0 = in + cut.head - first * VEC;
+        for (int c = 0; c < kChunks && c * chunk * 16 < row_bytes; ++c) {
+          if (again)
+            ok = ok && ptx::mbar_wait(ptx::smem_u32(&empty[c]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
+          ok = __all_sync(0xffffffffu, ok);
+          if (lane == 0) {
+            const uint32_t bar = ptx::smem_u32(&full[c]);
+            const int from = max(first, c * chunk), to = min(last, (c + 1) * chunk);
+            if (ok && from < to) {
+              ptx::mbar_arrive_expect_tx(bar, uint32_t(to - from) * 16);
+              ptx::bulk_load(blocks + from * 16, block0 + from * VEC, uint32_t(to - from) * 16, bar);
+            } else {
+              ptx::mbar_arrive(bar);
+            }
+          }
+          __syncwarp();
+        }
+        if (again) phase ^= 1u;
       }
-      __syncwarp();
-      float entropy;
-      const bool live = teacher_row(a, row, Teacher(teachers + set * 3 * slots, a.top), &entropy);
-      if (lane == 0) { entropy_s[set] = entropy; live_s[set] = live; }
-    };
-    prepare(blockIdx.x, 0, 0);
-    __syncthreads();
-    int buffer = 1, set = 1;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-      prepare(row + gridDim.x, buffer, set);
-      __syncthreads();                 // the row's shared memory is free
-      buffer ^= 1;
       set = set == 2 ? 0 : set + 1;
+    };
+    prepare(blockIdx.x, false);
+    __syncthreads();
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+      prepare(row + gridDim.x, true);
+      __syncthreads();
     }
     if (*static_cast<volatile int*>(&abort_flag) != 0) {           // a wait ran out: let the copies in flight end
       const uint64_t t0 = ptx::globaltimer_ns();
@@ -389,13 +464,14 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stat
   const Powers w = powers(a);
   auto group_sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
   __syncthreads();
-  int buffer = 0, set = 0;
+  int set = 0;
   uint32_t phase = 0;
+  bool ok = true;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* in = row_of(row);
     const Cut<T> cut(in, a.vocab);
-    const T* copy = place_of(row, buffer);
-    const Pack<T, VEC>* body = reinterpret_cast<const Pack<T, VEC>*>(copy + cut.head);
+    const int first = cut.head > 0 ? 1 : 0, last = first + cut.packs;
+    const T* copy = reinterpret_cast<const T*>(shared) + first * VEC - cut.head;         // where element 0 would lie
     const Teacher t(teachers + set * 3 * slots, a.top);
     const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
     const int target = wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
@@ -407,12 +483,21 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stat
                      : int(threadIdx.x) - cut.head < cut.tail ? tail0 + int(threadIdx.x) - cut.head : -1;
     const float edge = mine >= 0 ? to_float(in[mine]) : -INFINITY;
     auto value_at = [&](int c) { return to_float(c < cut.head || c >= tail0 ? in[c] : copy[c]); };
-
-    const bool ok = ptx::mbar_wait(ptx::smem_u32(&full[buffer]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
-    float top = edge;
-    if (ok) {
+    // The whole blocks of a chunk, a thread's share of them.
+    auto each = [&](auto&& body) {
 #pragma unroll 4
-      for (int i = threadIdx.x; i < cut.packs; i += threads) top = fmaxf(top, pack_max(body[i]));
+      for (int i = first + threadIdx.x; i < last; i += threads) body(i);
+    };
+
+    float top = edge;
+    for (int c = 0; c < kChunks && c * chunk < last; ++c) {
+      ok = ok && ptx::mbar_wait(ptx::smem_u32(&full[c]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
+      const int to = min(last, (c + 1) * chunk);
+      if (ok) {
+#pragma unroll 4
+        for (int i = max(first, c * chunk) + threadIdx.x; i < to; i += threads)
+          top = fmaxf(top, pack_max<T>(load_shared(blocks + i * 16)));
+      }
     }
     top = warp_max(top);
     if (lane == 0) red[0][warp] = top;
@@ -420,7 +505,9 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stat
     top = warp_max(lane < warps ? red[0][lane] : -INFINITY);
     const float base = top == -INFINITY ? 0.f : top;
 
-    float2 soft = make_float2(0.f, 0.f), hard = soft;
+    // 2^(z k - offset) is e^((z - max) / T) up to the rounding of the offset, which all of the row share.
+    const float offset = base * w.k;
+    float2 soft = splat2(0.f), hard = soft;
     float cross = 0.f;
     for (int i = threadIdx.x; i < a.top; i += threads) {
       if (t.column[i] < 0) continue;
@@ -429,24 +516,25 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stat
     }
     const float z_target = target >= 0 ? value_at(target) : 0.f;
     if (mine >= 0) {
-      soft.x = exp2_approx((edge - base) * w.k);
+      soft.x = two ? exp2_approx((edge - base) * w.k) : exp2_approx(fmaf(edge, w.k, -offset));
       if (two) hard.x = w.second(soft.x, edge - base);
     }
-    const float2 minus = make_float2(-base, -base), k2 = make_float2(w.k, w.k);
+    const float2 minus = splat2(two ? -base : -offset), k2 = splat2(w.k);
     auto add = [&](auto with_hard) {
-#pragma unroll 2
-      for (int i = threadIdx.x; i < cut.packs; i += threads) {
-        const Pack<T, VEC> v = body[i];
+      each([&](int i) {
+        float2 x[kPairs<T>];
+        unpack<T>(load_shared(blocks + i * 16), x);
 #pragma unroll
-        for (int k = 0; k < VEC; k += 2) {
-          const float2 d = __fadd2_rn(make_float2(to_float(v.v[k]), to_float(v.v[k + 1])), minus);
-          const float2 x = __fmul2_rn(d, k2);
-          const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-          soft = __fadd2_rn(soft, e);
-          if constexpr (decltype(with_hard)::value)
-            hard = __fadd2_rn(hard, make_float2(w.second(e.x, d.x), w.second(e.y, d.y)));
+        for (int k = 0; k < kPairs<T>; ++k) {
+          if constexpr (decltype(with_hard)::value) {
+            const float2 d = __fadd2_rn(x[k], minus), e = exp2_pair(__fmul2_rn(d, k2));
+            soft = __fadd2_rn(soft, e);
+            hard = __fadd2_rn(hard, w.second(e, d));
+          } else {
+            soft = __fadd2_rn(soft, exp2_pair(__ffma2_rn(x[k], k2, minus)));
+          }
         }
-      }
+      });
     };
     if (ok) {
       if (two) add(std::true_type{});
@@ -457,7 +545,8 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stat
       if (lane == 0) { red[1][warp] = s; red[2][warp] = h; red[3][warp] = c; }
     }
     group_sync();
-    const float sum_soft = warp_sum(lane < warps ? red[1][lane] : 0.f);
+    float sum_soft = warp_sum(lane < warps ? red[1][lane] : 0.f);
+    if (!two) sum_soft *= exp2_approx(-fmaf(base, w.k, -offset));
     const float sum_hard = two ? warp_sum(lane < warps ? red[2][lane] : 0.f) : sum_soft;
     if (warp == 0) {
       const float c = warp_sum(lane < warps ? red[3][lane] : 0.f);
@@ -470,34 +559,33 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, float* __restrict__ stat
     }
     const RowGrad g = row_grad(a, live, target >= 0, a.scale, top, sum_soft, sum_hard, w);
     T* out = grad + row * a.vocab;
-    if (mine >= 0) {
-      float x[1] = {edge};
-      gradient(g, x);
-      out[mine] = from_float<T>(x[0]);
-    }
-    const bool aligned = reinterpret_cast<uintptr_t>(out + cut.head) % 16 == 0;
-    if (ok) {
+    if (mine >= 0) out[mine] = from_float<T>(gradient(g, edge));
+    T* block0 = out + cut.head - first * VEC;      // where block 0 would lie
+    const bool aligned = reinterpret_cast<uintptr_t>(block0) % 16 == 0;
+    for (int c = 0; c < kChunks && c * chunk * 16 < row_bytes; ++c) {
+      const int to = min(last, (c + 1) * chunk);
+      if (ok) {
 #pragma unroll 2
-      for (int i = threadIdx.x; i < cut.packs; i += threads) {
-        Pack<T, VEC> v = body[i];
-        float x[VEC];
+        for (int i = max(first, c * chunk) + threadIdx.x; i < to; i += threads) {
+          float2 x[kPairs<T>];
+          unpack<T>(load_shared(blocks + i * 16), x);
+          gradient(g, x);
+          const uint4 v = pack<T>(x);
+          if (aligned) {
+            *reinterpret_cast<uint4*>(block0 + i * VEC) = v;
+          } else {
+            const T* one = reinterpret_cast<const T*>(&v);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) x[k] = to_float(v.v[k]);
-        gradient(g, x);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v.v[k] = from_float<T>(x[k]);
-        if (aligned) {
-          *reinterpret_cast<Pack<T, VEC>*>(out + cut.head + i * VEC) = v;
-        } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) out[cut.head + i * VEC + k] = v.v[k];
+            for (int k = 0; k < VEC; ++k) block0[i * VEC + k] = one[k];
+          }
         }
       }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&empty[c]));
     }
     __syncthreads();
     write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, target, z_target, threads);
-    phase ^= uint32_t(buffer);
-    buffer ^= 1;
+    phase ^= 1u;
     set = set == 2 ? 0 : set + 1;
   }
 }
@@ -521,26 +609,22 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
   const bool two = target >= 0 && w.squares != 0;               // a second sum, at temperature one
   Online sums;
   {
-    auto one = [&](int i) {
-      const float x[1] = {to_float(in[i])};
-      sums.add(x, w, two);
-    };
+    auto one = [&](int i) { sums.add(to_float(in[i]), w, two); };
     if (int(threadIdx.x) < cut.head) one(threadIdx.x);
     if (int(threadIdx.x) < cut.tail) one(a.vocab - cut.tail + threadIdx.x);
   }
-  const Pack<T, VEC>* body = reinterpret_cast<const Pack<T, VEC>*>(in + cut.head);
+  const uint4* body = reinterpret_cast<const uint4*>(in + cut.head);
   constexpr int kAhead = 4;            // packs of a thread in flight
   for (int i = threadIdx.x; i < cut.packs; i += kAhead * blockDim.x) {
-    Pack<T, VEC> v[kAhead];
+    uint4 v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (i + u * int(blockDim.x) < cut.packs) v[u] = body[i + u * blockDim.x];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (i + u * int(blockDim.x) >= cut.packs) break;
-      float x[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = to_float(v[u].v[k]);
+      float2 x[kPairs<T>];
+      unpack<T>(v[u], x);
       sums.add(x, w, two);
     }
   }
@@ -633,10 +717,11 @@ scale_unless_one_kernel(T* __restrict__ x, int64_t numel, const float* __restric
   const int64_t step = int64_t(gridDim.x) * 256, start = int64_t(blockIdx.x) * 256 + threadIdx.x;
   const int64_t packs = numel / VEC;
   for (int64_t i = start; i < packs; i += step) {
-    Pack<T, VEC> v = reinterpret_cast<Pack<T, VEC>*>(x)[i];
+    float2 v[kPairs<T>];
+    unpack<T>(reinterpret_cast<const uint4*>(x)[i], v);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v.v[k] = from_float<T>(to_float(v.v[k]) * f);
-    reinterpret_cast<Pack<T, VEC>*>(x)[i] = v;
+    for (int k = 0; k < kPairs<T>; ++k) v[k] = __fmul2_rn(v[k], splat2(f));
+    reinterpret_cast<uint4*>(x)[i] = pack<T>(v);
   }
   for (int64_t i = packs * VEC + start; i < numel; i += step) x[i] = from_float<T>(to_float(x[i]) * f);
 }
@@ -661,18 +746,20 @@ cudaError_t distill_fwd(DType type, const DistillArgs& a, float* stats, void* gr
   const size_t slots = 3 * size_t(padded_slots(a.top)) * 4;
   MB_SWITCH_FLOAT(type, T, {
     const int64_t bytes = int64_t(a.vocab) * sizeof(T);
-    const int64_t row_bytes = (bytes + 15) / 16 * 16 + 16, shared = 2 * row_bytes + 3 * int64_t(slots);
+    const int64_t row_bytes = (bytes + 15) / 16 * 16 + 16, shared = row_bytes + 3 * int64_t(slots);
     if (grad != nullptr && shared <= kSharedBytes) {
       auto kernel = distill_rows_kernel<T>;
       if (shared > 48 * 1024) {
         const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
         if (rc != cudaSuccess) return rc;
       }
-      // As many CTAs as fit an SM, 24 warps between them, but no more than leave each thread four packs.
+      // As many CTAs as fit an SM, 24 warps between them, but no more than leave each thread four blocks.
       const int resident = max(1, int(min(int64_t(16), kSharedBytes / (shared + 1024))));
       const int threads = max(32, min(kRowThreads / resident, int((bytes + 63) / 64)) / 32 * 32);
       const int64_t grid = min(a.rows, int64_t(sms) * resident);
-      kernel<<<unsigned(grid), threads + 32, shared, stream>>>(a, int(row_bytes), stats, static_cast<T*>(grad));
+      // Chunks of whole rounds of the threads.
+      const int chunk = int((row_bytes / 16 + kChunks * threads - 1) / (kChunks * threads)) * threads;
+      kernel<<<unsigned(grid), threads + 32, shared, stream>>>(a, int(row_bytes), chunk, stats, static_cast<T*>(grad));
     } else {
       distill_fwd_kernel<T><<<unsigned(a.rows), row_threads(bytes), slots, stream>>>(a, stats, static_cast<T*>(grad));
     }
