@@ -207,8 +207,28 @@ struct Teacher {
         z(p + 2 * padded_slots(top)) {}
 };
 
-// Fills it, with one warp; returns whether any slot is used, and sum p log p.
-__device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t row, const Teacher& t, float* entropy) {
+// What a row's threads have to know about it.
+struct TeacherFacts {
+  float entropy;               // sum p log p
+  int live;                    // any slot is used
+  int twice;                   // a column is named by more than one slot
+  int target_named;            // the target is a named column
+};
+
+// Slots that name column c, other than slot i.
+__device__ __forceinline__ bool named_elsewhere(const Teacher& t, int top, int c, int i) {
+  int found = 0;
+  for (int k = 0; k < padded_slots(top); k += 4) {
+    const int4 q = *reinterpret_cast<const int4*>(t.column + k);
+    found |= int(q.x == c && k != i) | int(q.y == c && k + 1 != i) | int(q.z == c && k + 2 != i) |
+             int(q.w == c && k + 3 != i);
+  }
+  return found != 0;
+}
+
+// Fills it, with one warp.  `named`: the facts about columns are wanted.
+__device__ __forceinline__ TeacherFacts teacher_row(const DistillArgs& a, int64_t row, const Teacher& t, int target,
+                                                    bool named) {
   const int lane = threadIdx.x & 31;
   const float inv_t = 1.f / a.temperature;
   float top = -INFINITY;
@@ -250,20 +270,23 @@ __device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t row, c
     t.p[i] = w;
     if (w == 0.f) t.column[i] = -1;
   }
-  *entropy = warp_sum(ent);
+  TeacherFacts f{warp_sum(ent), live, 0, 0};
   __syncwarp();
-  return live;
+  if (named) {
+    for (int i = lane; i < a.top; i += 32) {
+      const int c = t.column[i];
+      if (c >= 0) f.twice |= named_elsewhere(t, a.top, c, i);
+      f.target_named |= target >= 0 && c == target;
+    }
+    f.twice = __any_sync(0xffffffffu, f.twice);
+    f.target_named = __any_sync(0xffffffffu, f.target_named);
+  }
+  return f;
 }
 
-// Slots that name column c, other than slot i.
-__device__ __forceinline__ bool named_elsewhere(const Teacher& t, int top, int c, int i) {
-  int found = 0;
-  for (int k = 0; k < padded_slots(top); k += 4) {
-    const int4 q = *reinterpret_cast<const int4*>(t.column + k);
-    found |= int(q.x == c && k != i) | int(q.y == c && k + 1 != i) | int(q.z == c && k + 2 != i) |
-             int(q.w == c && k + 3 != i);
-  }
-  return found != 0;
+__device__ __forceinline__ int target_of(const DistillArgs& a, int64_t row) {
+  const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
+  return wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
 }
 
 // Coefficients of a row's gradient, probabilities' sums included.
@@ -274,12 +297,17 @@ struct RowGrad {
   Powers w;
 };
 
-template <int N>
+enum Parts { kNothing, kOne, kBoth };                // to learn from a row; whatever its logits where nothing
+__device__ __forceinline__ Parts parts_of(const RowGrad& g) {
+  return g.soft == 0.f && g.hard == 0.f ? kNothing : (g.hard == 0.f ? kOne : kBoth);
+}
+
+template <Parts P, int N>
 __device__ __forceinline__ void gradient(const RowGrad& g, float2 (&x)[N]) {
-  if (g.soft == 0.f && g.hard == 0.f) {           // nothing to learn from this row, whatever its logits
+  if constexpr (P == kNothing) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = splat2(0.f);
-  } else if (g.hard == 0.f) {
+  } else if constexpr (P == kOne) {
     const float2 k2 = splat2(g.w.k), minus = splat2(-g.offset), soft = splat2(g.soft);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = __fmul2_rn(soft, exp2_pair(__ffma2_rn(x[i], k2, minus)));
@@ -294,8 +322,19 @@ __device__ __forceinline__ void gradient(const RowGrad& g, float2 (&x)[N]) {
 }
 __device__ __forceinline__ float gradient(const RowGrad& g, float z) {
   float2 x[1] = {make_float2(z, z)};
-  gradient(g, x);
+  const Parts parts = parts_of(g);
+  if (parts == kNothing) return 0.f;
+  if (parts == kOne) gradient<kOne>(g, x);
+  else gradient<kBoth>(g, x);
   return x[0].x;
+}
+// Calls body(parts as a constant).
+template <typename F>
+__device__ __forceinline__ void with_parts(const RowGrad& g, F&& body) {
+  const Parts parts = parts_of(g);
+  if (parts == kNothing) body(std::integral_constant<Parts, kNothing>{});
+  else if (parts == kOne) body(std::integral_constant<Parts, kOne>{});
+  else body(std::integral_constant<Parts, kBoth>{});
 }
 
 __device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, bool live, bool has_target, float scale, float max,
@@ -317,28 +356,29 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, bool live, boo
 // Writes a row's gradient over a row in memory (`grad` itself, possibly).
 template <typename T>
 __device__ __forceinline__ void write_gradient(const T* src, const Cut<T>& cut, T* grad, int vocab, const RowGrad& g) {
-  constexpr int VEC = 16 / sizeof(T);
   auto one = [&](int i) { grad[i] = from_float<T>(gradient(g, to_float(src[i]))); };
   if (reinterpret_cast<uintptr_t>(grad + cut.head) % 16 == 0) {
     if (int(threadIdx.x) < cut.head) one(threadIdx.x);
     if (int(threadIdx.x) < cut.tail) one(vocab - cut.tail + threadIdx.x);
     const uint4* from = reinterpret_cast<const uint4*>(src + cut.head);
     uint4* to = reinterpret_cast<uint4*>(grad + cut.head);
-    constexpr int kAhead = 4;          // packs of a thread in flight
-    for (int i = threadIdx.x; i < cut.packs; i += kAhead * blockDim.x) {
-      uint4 v[kAhead];
+    with_parts(g, [&](auto parts) {
+      constexpr int kAhead = 4;        // packs of a thread in flight
+      for (int i = threadIdx.x; i < cut.packs; i += kAhead * blockDim.x) {
+        uint4 v[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (i + u * int(blockDim.x) < cut.packs) v[u] = from[i + u * blockDim.x];
+        for (int u = 0; u < kAhead; ++u)
+          if (i + u * int(blockDim.x) < cut.packs) v[u] = from[i + u * blockDim.x];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (i + u * int(blockDim.x) >= cut.packs) break;
-        float2 x[kPairs<T>];
-        unpack<T>(v[u], x);
-        gradient(g, x);
-        to[i + u * blockDim.x] = pack<T>(x);
+        for (int u = 0; u < kAhead; ++u) {
+          if (i + u * int(blockDim.x) >= cut.packs) break;
+          float2 x[kPairs<T>];
+          unpack<T>(v[u], x);
+          gradient<decltype(parts)::value>(g, x);
+          to[i + u * blockDim.x] = pack<T>(x);
+        }
       }
-    }
+    });
   } else {
     for (int i = threadIdx.x; i < vocab; i += blockDim.x) one(i);
   }
@@ -348,12 +388,13 @@ __device__ __forceinline__ void write_gradient(const T* src, const Cut<T>& cut, 
 // row was written.  A column named more than once is written by its first slot, with all its shares.
 template <typename T>
 __device__ __forceinline__ void write_named(const DistillArgs& a, T* grad, const RowGrad& g, float soft_scale,
-                                            float hard_scale, const Teacher& t, int target, float z_target, int threads) {
+                                            float hard_scale, const Teacher& t, const TeacherFacts& f, int target,
+                                            float z_target, int threads) {
   for (int i = threadIdx.x; i < a.top; i += threads) {
     const int c = t.column[i];
     if (c < 0) continue;
     float share = t.p[i];
-    if (named_elsewhere(t, a.top, c, i)) {
+    if (f.twice) {
       share = 0.f;
       bool first = true;
       for (int k = 0; k < a.top; ++k) {
@@ -365,7 +406,7 @@ __device__ __forceinline__ void write_named(const DistillArgs& a, T* grad, const
     }
     grad[c] = from_float<T>(gradient(g, t.z[i]) - soft_scale * share - (c == target ? hard_scale : 0.f));
   }
-  if (int(threadIdx.x) == threads - 1 && target >= 0 && !named_elsewhere(t, a.top, target, -1))
+  if (int(threadIdx.x) == threads - 1 && target >= 0 && !f.target_named)
     grad[target] = from_float<T>(gradient(g, z_target) - hard_scale);
 }
 
@@ -395,19 +436,16 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ float red[4][kRowThreads / 32];
-  __shared__ alignas(8) uint64_t full[kChunks], empty[kChunks];
+  __shared__ alignas(8) uint64_t full, empty[kChunks];
   __shared__ int abort_flag;
-  __shared__ float entropy_s[3];
-  __shared__ int live_s[3];
+  __shared__ TeacherFacts facts[3];
   const int threads = blockDim.x - 32, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slots = padded_slots(a.top);
   float* teachers = reinterpret_cast<float*>(shared + row_bytes);          // [3]
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int c = 0; c < kChunks; ++c) {
-      ptx::mbar_init(ptx::smem_u32(&full[c]), 1);
-      ptx::mbar_init(ptx::smem_u32(&empty[c]), warps);
-    }
+    ptx::mbar_init(ptx::smem_u32(&full), 1);
+    for (int c = 0; c < kChunks; ++c) ptx::mbar_init(ptx::smem_u32(&empty[c]), warps);
     ptx::fence_barrier_init();
   }
   __syncthreads();
@@ -421,26 +459,22 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
     bool ok = true;
     auto prepare = [&](int64_t row, bool again) {
       if (row < a.rows) {
-        float entropy;
-        const bool live = teacher_row(a, row, Teacher(teachers + set * 3 * slots, a.top), &entropy);
-        if (lane == 0) { entropy_s[set] = entropy; live_s[set] = live; }
+        const TeacherFacts f = teacher_row(a, row, Teacher(teachers + set * 3 * slots, a.top), target_of(a, row), true);
+        if (lane == 0) facts[set] = f;
         const T* in = row_of(row);
         const Cut<T> cut(in, a.vocab);
         const int first = cut.head > 0 ? 1 : 0, last = first + cut.packs;  // blocks that are whole
         const T* block0 = in + cut.head - first * VEC;
+        const uint32_t bar = ptx::smem_u32(&full);
         for (int c = 0; c < kChunks && c * chunk * 16 < row_bytes; ++c) {
           if (again)
             ok = ok && ptx::mbar_wait(ptx::smem_u32(&empty[c]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
           ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           if (lane == 0) {
-            const uint32_t bar = ptx::smem_u32(&full[c]);
+            if (c == 0) ptx::mbar_arrive_expect_tx(bar, uint32_t(cut.packs) * 16);
             const int from = max(first, c * chunk), to = min(last, (c + 1) * chunk);
-            if (ok && from < to) {
-              ptx::mbar_arrive_expect_tx(bar, uint32_t(to - from) * 16);
-              ptx::bulk_load(blocks + from * 16, block0 + from * VEC, uint32_t(to - from) * 16, bar);
-            } else {
-              ptx::mbar_arrive(bar);
-            }
+            if (from < to) ptx::bulk_load(blocks + from * 16, block0 + from * VEC, uint32_t(to - from) * 16, bar);
           }
           __syncwarp();
         }
@@ -466,17 +500,14 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
   __syncthreads();
   int set = 0;
   uint32_t phase = 0;
-  bool ok = true;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* in = row_of(row);
     const Cut<T> cut(in, a.vocab);
     const int first = cut.head > 0 ? 1 : 0, last = first + cut.packs;
     const T* copy = reinterpret_cast<const T*>(shared) + first * VEC - cut.head;         // where element 0 would lie
     const Teacher t(teachers + set * 3 * slots, a.top);
-    const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
-    const int target = wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
+    const int target = target_of(a, row);
     const bool two = target >= 0 && w.squares != 0;
-    const bool live = live_s[set] != 0;
     // The elements before the first and behind the last 16-byte boundary stay in memory: one thread's each.
     const int tail0 = a.vocab - cut.tail;
     const int mine = int(threadIdx.x) < cut.head ? int(threadIdx.x)
@@ -489,16 +520,13 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
       for (int i = first + threadIdx.x; i < last; i += threads) body(i);
     };
 
+    // One warp looks for the row's arrival; the others stand at the barrier, where they cost no issue slots.
+    if (warp == 0) ptx::mbar_wait(ptx::smem_u32(&full), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
+    group_sync();
+    const TeacherFacts f = facts[set];
+    const bool ok = *static_cast<volatile int*>(&abort_flag) == 0;
     float top = edge;
-    for (int c = 0; c < kChunks && c * chunk < last; ++c) {
-      ok = ok && ptx::mbar_wait(ptx::smem_u32(&full[c]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
-      const int to = min(last, (c + 1) * chunk);
-      if (ok) {
-#pragma unroll 4
-        for (int i = max(first, c * chunk) + threadIdx.x; i < to; i += threads)
-          top = fmaxf(top, pack_max<T>(load_shared(blocks + i * 16)));
-      }
-    }
+    if (ok) each([&](int i) { top = fmaxf(top, pack_max<T>(load_shared(blocks + i * 16))); });
     top = warp_max(top);
     if (lane == 0) red[0][warp] = top;
     group_sync();
@@ -546,45 +574,47 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
     }
     group_sync();
     float sum_soft = warp_sum(lane < warps ? red[1][lane] : 0.f);
+    const float all_cross = warp_sum(lane < warps ? red[3][lane] : 0.f);
     if (!two) sum_soft *= exp2_approx(-fmaf(base, w.k, -offset));
     const float sum_hard = two ? warp_sum(lane < warps ? red[2][lane] : 0.f) : sum_soft;
-    if (warp == 0) {
-      const float c = warp_sum(lane < warps ? red[3][lane] : 0.f);
-      if (lane == 0) {
-        float l = 0.f;
-        if (live) l = a.temperature * a.temperature * (entropy_s[set] - kLn2 * (c * w.k - __log2f(sum_soft)));
-        if (target >= 0) l += a.hard_weight * (kLn2 * __log2f(sum_hard) + (top - z_target));
-        *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(ok ? l : NAN, top, sum_soft, sum_hard);
-      }
+    if (threadIdx.x == 32 % threads) {
+      float l = 0.f;
+      if (f.live) l = a.temperature * a.temperature * (f.entropy - kLn2 * (all_cross * w.k - __log2f(sum_soft)));
+      if (target >= 0) l += a.hard_weight * (kLn2 * __log2f(sum_hard) + (top - z_target));
+      *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(ok ? l : NAN, top, sum_soft, sum_hard);
     }
-    const RowGrad g = row_grad(a, live, target >= 0, a.scale, top, sum_soft, sum_hard, w);
+    const RowGrad g = row_grad(a, f.live != 0, target >= 0, a.scale, top, sum_soft, sum_hard, w);
     T* out = grad + row * a.vocab;
     if (mine >= 0) out[mine] = from_float<T>(gradient(g, edge));
     T* block0 = out + cut.head - first * VEC;      // where block 0 would lie
     const bool aligned = reinterpret_cast<uintptr_t>(block0) % 16 == 0;
-    for (int c = 0; c < kChunks && c * chunk * 16 < row_bytes; ++c) {
-      const int to = min(last, (c + 1) * chunk);
-      if (ok) {
-#pragma unroll 2
-        for (int i = max(first, c * chunk) + threadIdx.x; i < to; i += threads) {
+    with_parts(g, [&](auto parts) {
+      uint4* to16 = reinterpret_cast<uint4*>(block0);
+      for (int c = 0; c < kChunks && c * chunk * 16 < row_bytes; ++c) {
+        const int to = ok ? min(last, (c + 1) * chunk) : 0, from = max(first, c * chunk) + int(threadIdx.x);
+        auto value = [&](int i) {
           float2 x[kPairs<T>];
           unpack<T>(load_shared(blocks + i * 16), x);
-          gradient(g, x);
-          const uint4 v = pack<T>(x);
-          if (aligned) {
-            *reinterpret_cast<uint4*>(block0 + i * VEC) = v;
-          } else {
+          gradient<decltype(parts)::value>(g, x);
+          return pack<T>(x);
+        };
+        if (aligned) {
+#pragma unroll 4
+          for (int i = from; i < to; i += threads) to16[i] = value(i);
+        } else {
+          for (int i = from; i < to; i += threads) {
+            const uint4 v = value(i);
             const T* one = reinterpret_cast<const T*>(&v);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) block0[i * VEC + k] = one[k];
           }
         }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&empty[c]));
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&empty[c]));
-    }
+    });
     __syncthreads();
-    write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, target, z_target, threads);
+    write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, f, target, z_target, threads);
     phase ^= 1u;
     set = set == 2 ? 0 : set + 1;
   }
@@ -594,17 +624,14 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads)
 distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
-  constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ float red[3 * kMaxThreads / 32];
-  __shared__ float entropy_s;
-  __shared__ int live_s;
+  __shared__ TeacherFacts facts;
   const int64_t row = blockIdx.x;
   const T* in = static_cast<const T*>(a.logits) + row * a.vocab;
   const Cut<T> cut(in, a.vocab);
   const Teacher t(shared, a.top);
-  const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
-  const int target = wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
+  const int target = target_of(a, row);
   const Powers w = powers(a);
   const bool two = target >= 0 && w.squares != 0;               // a second sum, at temperature one
   Online sums;
@@ -629,12 +656,12 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
     }
   }
   if (threadIdx.x < 32) {
-    float entropy;
-    const bool live = teacher_row(a, row, t, &entropy);
-    if (threadIdx.x == 0) { entropy_s = entropy; live_s = live; }
+    const TeacherFacts f = teacher_row(a, row, t, target, grad != nullptr);
+    if (threadIdx.x == 0) facts = f;
   }
   sums = block_sums(sums, w, two, red);
-  const bool live = live_s != 0;
+  const TeacherFacts f = facts;
+  const bool live = f.live != 0;
   const float log_soft = __log2f(sums.soft);
 
   // Loss, and the named columns' logits before the row may be overwritten.
@@ -652,7 +679,7 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
   if (threadIdx.x == 0) {
     float sum = 0.f;
     for (int k = 0; k < int(blockDim.x >> 5); ++k) sum += red[k];
-    float l = live ? a.temperature * a.temperature * (entropy_s - kLn2 * sum) : 0.f;
+    float l = live ? a.temperature * a.temperature * (f.entropy - kLn2 * sum) : 0.f;
     if (target >= 0) l += a.hard_weight * (kLn2 * __log2f(sums.hard) + (sums.m - z_target));
     *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(l, sums.m, sums.soft, sums.hard);
   }
@@ -661,7 +688,7 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
   const RowGrad g = row_grad(a, live, target >= 0, a.scale, sums.m, sums.soft, sums.hard, w);
   write_gradient(in, cut, out, a.vocab, g);
   __syncthreads();
-  write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, target, z_target, blockDim.x);
+  write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, f, target, z_target, blockDim.x);
 }
 
 template <typename T>
@@ -669,17 +696,15 @@ __global__ void __launch_bounds__(kMaxThreads)
 distill_bwd_kernel(const DistillArgs a, const float* __restrict__ stats, const float* __restrict__ grad_out,
                    T* __restrict__ grad) {
   extern __shared__ __align__(16) unsigned char shared[];
-  __shared__ int live_s;
+  __shared__ TeacherFacts facts;
   const int64_t row = blockIdx.x;
   const T* in = static_cast<const T*>(a.logits) + row * a.vocab;
   const Cut<T> cut(in, a.vocab);
   const Teacher t(shared, a.top);
-  const int64_t wanted = a.targets != nullptr ? a.targets[row] : -1;
-  const int target = wanted >= 0 && wanted < a.vocab ? int(wanted) : -1;
+  const int target = target_of(a, row);
   if (threadIdx.x < 32) {
-    float entropy;
-    const bool live = teacher_row(a, row, t, &entropy);
-    if (threadIdx.x == 0) live_s = live;
+    const TeacherFacts f = teacher_row(a, row, t, target, true);
+    if (threadIdx.x == 0) facts = f;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.top; i += blockDim.x)
@@ -687,11 +712,11 @@ distill_bwd_kernel(const DistillArgs a, const float* __restrict__ stats, const f
   const float z_target = target >= 0 ? to_float(in[target]) : 0.f;
   const float scale = a.scale * *grad_out;
   const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
-  const RowGrad g = row_grad(a, live_s != 0, target >= 0, scale, st.y, st.z, st.w, powers(a));
+  const RowGrad g = row_grad(a, facts.live != 0, target >= 0, scale, st.y, st.z, st.w, powers(a));
   T* out = grad + row * a.vocab;
   write_gradient(in, cut, out, a.vocab, g);
   __syncthreads();
-  write_named(a, out, g, a.temperature * scale, a.hard_weight * scale, t, target, z_target, blockDim.x);
+  write_named(a, out, g, a.temperature * scale, a.hard_weight * scale, t, facts, target, z_target, blockDim.x);
 }
 
 __global__ void __launch_bounds__(1024)
