@@ -27,6 +27,7 @@ DEFAULT_ACTIVATION_FN = partial(F.gelu, approximate='tanh')
 
 _MLP_TYPES = ('mlp', 'glu')
 _MLP_IMPLS = ('sparse', 'grouped')
+_ROUTER_SCORES = ('softmax', 'sigmoid')
 
 
 def _default_device() -> Union[int, torch.device]:
@@ -87,8 +88,20 @@ class Arguments:
     moe_zloss_weight: float = 0
     moe_zloss_in_fp32: bool = False
 
-    # Extension of this library (absent from the reference): route the
-    # expert-parallel exchange through the fused peer-memory kernels instead of
+    # Extensions of this library (absent from the reference): how experts are selected
+    # (``ops.select_experts``).  ``moe_router_score``: 'softmax' or 'sigmoid' scores; ``moe_router_groups``
+    # groups of experts of which the best ``moe_router_top_groups`` stay (``None``: all); the weights are
+    # multiplied by ``moe_router_scale``.  ``moe_router_bias``: a bias per expert that takes part in the
+    # choice only, kept as a buffer of the router and moved against the load by
+    # ``layers.router.balance_routers`` (the trainer does, see ``TrainerConfig.router_bias_rate``), so that
+    # ``moe_loss_weight`` can be 0.
+    moe_router_score: str = 'softmax'
+    moe_router_bias: bool = False
+    moe_router_groups: int = 1
+    moe_router_top_groups: Optional[int] = None
+    moe_router_scale: float = 1.0
+
+    # Route the expert-parallel exchange through the fused peer-memory kernels instead of
     # NCCL all-to-all.  ``None`` picks the fused path whenever a symmetric
     # workspace can be created for ``expert_parallel_group``.
     ep_fused_comm: Optional[bool] = None
@@ -108,6 +121,14 @@ class Arguments:
             raise ValueError(f'mlp_type must be one of {_MLP_TYPES}, got {self.mlp_type!r}')
         if self.mlp_impl not in _MLP_IMPLS:
             raise ValueError(f'mlp_impl must be one of {_MLP_IMPLS}, got {self.mlp_impl!r}')
+        if self.moe_router_score not in _ROUTER_SCORES:
+            raise ValueError(f'moe_router_score must be one of {_ROUTER_SCORES}, got {self.moe_router_score!r}')
+        if self.moe_router_groups < 1 or self.moe_num_experts % self.moe_router_groups:
+            raise ValueError(f'moe_router_groups must divide the {self.moe_num_experts} experts, got '
+                             f'{self.moe_router_groups}')
+        kept = self.moe_router_groups if self.moe_router_top_groups is None else self.moe_router_top_groups
+        if not 1 <= kept <= self.moe_router_groups:
+            raise ValueError(f'moe_router_top_groups must lie in [1, {self.moe_router_groups}], got {kept}')
         if self.shared_expert_hidden_size is None:
             self.shared_expert_hidden_size = self.ffn_hidden_size
 

@@ -407,6 +407,8 @@ class MoE(torch.nn.Module):
             scores, expert_weights, top_experts = self.router(x)
         with nvtx_range('moe.experts'):
             out = self.experts(x, scores, expert_weights, top_experts)
+        if self.training and getattr(self.router, 'expert_load', None) is not None:
+            self.router.count_load(self.experts.last_tokens_per_expert)
         if self.shared_expert is not None:
             out = self.shared_expert.add_experts_sharedexpert(self.shared_expert(x), out)
         return out

@@ -10,16 +10,21 @@ in a module-level list when the z-loss is enabled; the trainer reads them with
 
 On CUDA the softmax / top-k / normalisation chain and its backward run as one
 kernel each (``csrc/router.cu``); the logits GEMM is a plain library GEMM.
+
+Sigmoid scores, expert groups, a weight factor and a balancing bias (the ``moe_router_*`` arguments) go
+through :func:`megablocks_b200.ops.select_experts` instead; :func:`balance_routers` moves the biases.
 """
 
 import warnings
-from typing import Any
+from typing import Any, Iterable, Optional
 
 import torch
+import torch.distributed as dist
 
 from megablocks_b200._ext import ext
 from megablocks_b200.layers import common, expert_block
 from megablocks_b200.layers.arguments import Arguments
+from megablocks_b200.ops.select import select_experts
 
 _ROUTER_LOGITS = []
 
@@ -112,6 +117,26 @@ class LearnedRouter(torch.nn.Module):
             device=args.device,
         )
         args.init_method(self.layer.weight)
+        # The balancing bias and the tokens that each expert got since it was last moved.
+        def vector(dtype):
+            return torch.zeros(args.moe_num_experts, dtype=dtype, device=args.device) if args.moe_router_bias else None
+
+        self.register_buffer('expert_bias', vector(torch.float32))
+        self.register_buffer('expert_load', vector(torch.int64), persistent=False)
+        self._selects = (args.moe_router_bias or args.moe_router_score != 'softmax' or args.moe_router_groups > 1
+                         or args.moe_router_scale != 1.0)
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        # The bias moves in steps that 16 bits would swallow: it keeps 32 when the module is cast.
+        if self.expert_bias is not None and self.expert_bias.dtype != torch.float32:
+            self.expert_bias = self.expert_bias.float()
+        return self
+
+    def count_load(self, tokens_per_expert: torch.Tensor) -> None:
+        """Add one forward pass's tokens per expert to the load that :func:`balance_routers` goes by."""
+        if self.expert_load is not None:
+            self.expert_load.add_(tokens_per_expert.detach())
 
     def jitter(self, x: torch.Tensor) -> torch.Tensor:
         eps = self.args.moe_jitter_eps
@@ -126,6 +151,10 @@ class LearnedRouter(torch.nn.Module):
     def _select(self, logits: torch.Tensor):
         args = self.args
         norm_p = args.moe_normalize_expert_weights
+        if self._selects:
+            return select_experts(logits, args.moe_top_k, score=args.moe_router_score, bias=self.expert_bias,
+                                  groups=args.moe_router_groups, top_groups=args.moe_router_top_groups,
+                                  norm_p=norm_p, scale=args.moe_router_scale)
         fused_ok = (logits.is_cuda and logits.dtype in (torch.float16, torch.bfloat16, torch.float32)
                     and args.moe_num_experts <= 1024 and args.moe_top_k <= 8
                     and (not norm_p or float(norm_p) in (1.0, 2.0)))
@@ -146,3 +175,26 @@ class LearnedRouter(torch.nn.Module):
         if self.args.uniform_expert_assignment:
             experts = _uniform_expert_assignment(experts, self.args.moe_num_experts)
         return scores, weights, experts
+
+
+@torch.no_grad()
+def balance_routers(routers: Iterable[LearnedRouter], rate: float,
+                    group: Optional[dist.ProcessGroup] = None) -> None:
+    """Move the balancing biases of ``routers`` by ``rate`` against the load since the last call
+    (:func:`megablocks_b200.ops.update_expert_bias`), summed over ``group``, and start counting anew.
+    Routers without a bias are left alone; all ranks of the group call it with the same layers."""
+    routers = [r for r in routers if r.expert_load is not None]
+    if not routers or rate == 0:
+        return
+    # The layers' vectors side by side (they may differ in length): a few launches for all of them.
+    load = torch.cat([r.expert_load for r in routers])
+    if group is not None and dist.get_world_size(group) > 1:
+        dist.all_reduce(load, group=group)
+    parts = load.split([r.expert_load.numel() for r in routers])
+    if len({p.numel() for p in parts}) == 1:
+        wide = load.view(len(routers), -1).double()
+        steps = torch.sign(wide.sum(dim=1, keepdim=True) - wide.shape[1] * wide).float().unbind()
+    else:
+        steps = [torch.sign(p.double().sum() - p.numel() * p.double()).float() for p in parts]
+    torch._foreach_add_([r.expert_bias for r in routers], list(steps), alpha=rate)
+    torch._foreach_zero_([r.expert_load for r in routers])

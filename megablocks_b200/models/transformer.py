@@ -9,14 +9,18 @@ family natively so the library can be trained and benchmarked stand-alone:
 * ``mixtral`` flavour: RMSNorm, rotary positions, grouped-query attention,
   SwiGLU experts (``mlp_type='glu'``), untied LM head.
 
-Attention uses the library fused attention (``scaled_dot_product_attention``);
+Attention uses the library fused attention (``scaled_dot_product_attention``), or this library's windowed
+attention where ``attention_window`` or ``attention_sinks`` is set and wherever a key-value cache is;
 everything MoE runs this library's kernels.  Inputs are ``[batch, seq]`` token ids.
+
+Beside training (``loss``, ``distillation_loss``) a model answers: ``prefill`` fills a :class:`KVCache` from a
+batch of prompts, ``decode`` takes one token per sequence further, ``generate`` does both greedily.
 """
 
 import dataclasses
 import math
 from functools import partial
-from typing import Optional
+from typing import List, NamedTuple, Optional
 
 import torch
 import torch.nn as nn
@@ -28,6 +32,7 @@ from megablocks_b200.layers.dmoe import dMoE
 from megablocks_b200.layers.moe import MoE, batched_load_balancing_loss, clear_load_balancing_loss
 from megablocks_b200.layers.router import batched_router_zloss, clear_router_zloss
 from megablocks_b200.ops import fused
+from megablocks_b200.ops.attention import window_attention, window_attention_decode
 
 
 @dataclasses.dataclass
@@ -60,6 +65,16 @@ class TransformerConfig:
     # pipeline parallelism: this process builds stage `pipeline_stage` of `pipeline_stages`
     pipeline_stages: int = 1
     pipeline_stage: int = 0
+    # selection of the experts (see Arguments)
+    moe_router_score: str = 'softmax'
+    moe_router_bias: bool = False
+    moe_router_groups: int = 1
+    moe_router_top_groups: Optional[int] = None
+    moe_router_scale: float = 1.0
+    # attention: a token sees itself and the `attention_window` - 1 before it (None: all), and the first
+    # `attention_sinks` tokens
+    attention_window: Optional[int] = None
+    attention_sinks: int = 0
 
     @property
     def kv_heads(self) -> int:
@@ -95,6 +110,11 @@ class TransformerConfig:
             ep_fused_comm=self.ep_fused_comm,
             ep_inflight_microbatches=self.ep_inflight_microbatches,
             pipeline_model_parallel_size=self.pipeline_stages,
+            moe_router_score=self.moe_router_score,
+            moe_router_bias=self.moe_router_bias,
+            moe_router_groups=self.moe_router_groups,
+            moe_router_top_groups=self.moe_router_top_groups,
+            moe_router_scale=self.moe_router_scale,
         )
 
 
@@ -126,6 +146,28 @@ def preset(name: str, **overrides) -> TransformerConfig:
 RMSNorm = fused.RMSNorm
 
 
+class Teacher(NamedTuple):
+    """A teacher's kept logits of a batch, for :meth:`MoETransformer.distillation_loss`."""
+    logits: torch.Tensor                # [batch, seq, top]
+    ids: torch.Tensor                   # [batch, seq, top] int32 or int64; outside the vocabulary: unused
+    temperature: float = 1.0
+    hard_weight: float = 0.0            # of the targets' cross entropy
+
+
+@dataclasses.dataclass
+class KVCache:
+    """Keys and values of every layer, ``[batch, capacity, kv_heads, head_dim]`` each, and the valid tokens of
+    every sequence.  ``used`` is the longest sequence's length as far as the host knows it."""
+    keys: List[torch.Tensor]
+    values: List[torch.Tensor]
+    lengths: torch.Tensor               # int32 [batch]
+    used: int = 0
+
+    @property
+    def capacity(self) -> int:
+        return self.keys[0].shape[1]
+
+
 def _rope_tables(seq_len: int, head_dim: int, theta: float, device):
     inv = 1.0 / (theta**(torch.arange(0, head_dim, 2, device=device, dtype=torch.float32) / head_dim))
     ang = torch.outer(torch.arange(seq_len, device=device, dtype=torch.float32), inv)
@@ -149,18 +191,47 @@ class Attention(nn.Module):
             nn.init.zeros_(self.qkv.bias)
             nn.init.zeros_(self.proj.bias)
 
-    def forward(self, x: torch.Tensor, rope) -> torch.Tensor:
+    def _project(self, x: torch.Tensor, rope):
+        """Queries, keys and values ``[batch, seq, heads, head_dim]``, rotated."""
         b, s, _ = x.shape
         cfg = self.cfg
-        qkv = self.qkv(x)
         q_dim, kv_dim = cfg.num_heads * self.head_dim, cfg.kv_heads * self.head_dim
-        q, k, v = qkv.split([q_dim, kv_dim, kv_dim], dim=-1)
+        q, k, v = self.qkv(x).split([q_dim, kv_dim, kv_dim], dim=-1)
         q = q.view(b, s, cfg.num_heads, self.head_dim)
         k = k.view(b, s, cfg.kv_heads, self.head_dim)
         if rope is not None:     # rotate the [batch, seq, heads, dim] views of the fused projection in one pass each
             q, k = fused.rope(q, *rope), fused.rope(k, *rope)
-        q, k = q.transpose(1, 2), k.transpose(1, 2)
-        v = v.view(b, s, cfg.kv_heads, self.head_dim).transpose(1, 2)
+        return q, k, v.view(b, s, cfg.kv_heads, self.head_dim)
+
+    def prefill(self, x: torch.Tensor, rope, keys: torch.Tensor, values: torch.Tensor,
+                lengths: torch.Tensor) -> torch.Tensor:
+        """Whole prompts; their keys and values go to the start of the caches."""
+        b, s, _ = x.shape
+        q, k, v = self._project(x, rope)
+        keys[:, :s].copy_(k)
+        values[:, :s].copy_(v)
+        out = window_attention(q, k, v, self.cfg.attention_window, self.cfg.attention_sinks, lengths)
+        return self.proj(out.reshape(b, s, -1))
+
+    def decode(self, x: torch.Tensor, rope, keys: torch.Tensor, values: torch.Tensor, at: torch.Tensor,
+               lengths: torch.Tensor) -> torch.Tensor:
+        """One token per sequence (``x[1, batch, hidden]``, the batch in the place of the positions, as the
+        rotary tables have it) at position ``at[batch]`` of the caches, ``lengths`` with it."""
+        q, k, v = (t.squeeze(0) for t in self._project(x, rope))
+        rows = torch.arange(at.shape[0], device=at.device)
+        keys[rows, at] = k
+        values[rows, at] = v
+        out = window_attention_decode(q, keys, values, lengths, self.cfg.attention_window, self.cfg.attention_sinks)
+        return self.proj(out.reshape(1, at.shape[0], -1))
+
+    def forward(self, x: torch.Tensor, rope) -> torch.Tensor:
+        b, s, _ = x.shape
+        cfg = self.cfg
+        q, k, v = self._project(x, rope)
+        if cfg.attention_window is not None or cfg.attention_sinks:
+            out = window_attention(q, k, v, cfg.attention_window, cfg.attention_sinks)
+            return self.proj(out.reshape(b, s, -1))
+        q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=cfg.kv_heads != cfg.num_heads)
         return self.proj(out.transpose(1, 2).reshape(b, s, -1))
 
@@ -186,12 +257,12 @@ class Block(nn.Module):
         self.ln2 = norm(cfg.hidden_size, **kw)
         self.moe = (dMoE if cfg.dropless else MoE)(moe_args)
 
-    def forward(self, x: torch.Tensor, delta, delta_bias, rope):
-        """The residual stream arrives as ``x + delta + delta_bias`` (``delta`` may be ``None``;
+    def forward(self, x: torch.Tensor, delta, delta_bias, rope, attend=None):
+        """``attend`` (optional) takes the place of the attention layer's forward pass.  The residual stream arrives as ``x + delta + delta_bias`` (``delta`` may be ``None``;
         ``delta_bias`` is the previous MoE layer's output bias, one value per column, or ``None``)
         and leaves the same way, so every residual add rides in the following norm's kernels."""
         x, normed = _add_norm(self.ln1, x, delta, delta_bias)
-        x, normed = _add_norm(self.ln2, x, self.attn(normed, rope))
+        x, normed = _add_norm(self.ln2, x, self.attn(normed, rope) if attend is None else attend(self.attn, normed))
         # The MoE layer is token-wise: it flattens every leading dimension, so the
         # [batch, seq, hidden] activations go in as they are (no transpose copy).
         out = self.moe(normed)
@@ -248,11 +319,16 @@ class MoETransformer(nn.Module):
             x = x + self.wpe(torch.arange(tokens.shape[1], device=tokens.device))
         return x
 
-    def _run_blocks(self, x: torch.Tensor):
+    def _run_blocks(self, x: torch.Tensor, attend=None):
         """Residual stream through this process's blocks; returns ``(x, delta, delta_bias)`` with the
-        last block's output (and its bias vector, if any) still to be added."""
-        rope = self._rope_for(x.shape[1], x.device)
+        last block's output (and its bias vector, if any) still to be added.  ``attend(layer, attention,
+        normed)`` takes the place of the attention layers' forward pass."""
         delta = delta_bias = None
+        if attend is not None:
+            for i, block in enumerate(self.blocks):
+                x, delta, delta_bias = block(x, delta, delta_bias, None, partial(attend, i))
+            return x, delta, delta_bias
+        rope = self._rope_for(x.shape[1], x.device)
         for block in self.blocks:
             if self.cfg.activation_checkpointing and self.training:
                 x, delta, delta_bias = checkpoint(block, x, delta, delta_bias, rope, use_reentrant=False)
@@ -314,6 +390,103 @@ class MoETransformer(nn.Module):
         aux = self._aux_loss()
         total = lm if aux is None else lm + aux
         return total, lm.detach()
+
+    def distillation_loss(self, tokens: torch.Tensor, teacher: Teacher, targets: Optional[torch.Tensor] = None):
+        """The loss against a teacher's kept logits (:func:`fused.linear_distillation_loss`), with
+        ``teacher.hard_weight`` times the targets' cross entropy, plus the MoE auxiliary losses.
+
+        Returns ``(total, distillation loss)``.  Clears the per-step loss accumulators.
+        """
+        if self.cfg.pipeline_stages > 1:
+            raise RuntimeError('a pipeline stage is driven through stage_forward / stage_loss')
+        top = teacher.logits.shape[-1]
+        if teacher.logits.shape[:-1] != tokens.shape or teacher.ids.shape != teacher.logits.shape:
+            raise ValueError('a teacher has logits and ids [batch, seq, top] for tokens [batch, seq]')
+        hidden = self.hidden_states(tokens)
+        weight = self.lm_head.weight if self.lm_head is not None else self.wte.weight
+        loss = fused.linear_distillation_loss(
+            hidden.reshape(-1, hidden.shape[-1]), weight, teacher.logits.reshape(-1, top),
+            teacher.ids.reshape(-1, top), teacher.temperature, None if targets is None else targets.reshape(-1),
+            teacher.hard_weight)
+        aux = self._aux_loss()
+        return loss if aux is None else loss + aux, loss.detach()
+
+    # -- answering -----------------------------------------------------------------------
+    def new_cache(self, batch: int, capacity: int) -> KVCache:
+        """An empty key-value cache for ``batch`` sequences of up to ``capacity`` tokens."""
+        cfg = self.cfg
+        if cfg.pipeline_stages > 1:
+            raise RuntimeError('a pipeline stage does not answer by itself')
+        if batch < 1 or capacity < 1:
+            raise ValueError('a cache holds at least one sequence of one token')
+        if self.wpe is not None and capacity > cfg.max_seq_len:
+            raise ValueError(f'the model has {cfg.max_seq_len} positions, a cache of {capacity} does not fit')
+        weight = self.wte.weight
+        shape = (batch, capacity, cfg.kv_heads, cfg.hidden_size // cfg.num_heads)
+        buffers = [[torch.zeros(shape, dtype=weight.dtype, device=weight.device) for _ in self.blocks]
+                   for _ in range(2)]
+        return KVCache(*buffers, torch.zeros(batch, dtype=torch.int32, device=weight.device))
+
+    @torch.no_grad()
+    def prefill(self, tokens: torch.Tensor, cache: KVCache, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Fill the cache from prompts ``tokens[batch, seq]`` (``lengths[batch]`` valid tokens each, at least one;
+        ``None``: all); returns the logits ``[batch, vocab]`` behind each prompt's last token."""
+        b, s = tokens.shape
+        if b != cache.lengths.shape[0] or not 1 <= s <= cache.capacity:
+            raise ValueError(f'prompts of {s} tokens for {b} sequences do not fit a cache of {cache.capacity} tokens '
+                             f'for {cache.lengths.shape[0]}')
+        if lengths is None:
+            lengths = torch.full((b,), s, dtype=torch.int32, device=tokens.device)
+        elif lengths.shape != (b,):
+            raise ValueError('lengths must have one entry per sequence')
+        cache.lengths.copy_(lengths.clamp(1, s))
+        cache.used = s
+        rope = self._rope_for(s, tokens.device)
+        valid = cache.lengths.clone()
+
+        def attend(layer, attention, normed):
+            return attention.prefill(normed, rope, cache.keys[layer], cache.values[layer], valid)
+
+        x, delta, delta_bias = self._run_blocks(self._embed(tokens), attend)
+        hidden = _add_norm(self.ln_f, x, delta, delta_bias)[1]
+        last = (cache.lengths - 1).long()
+        return self.logits(hidden[torch.arange(b, device=tokens.device), last])
+
+    @torch.no_grad()
+    def decode(self, tokens: torch.Tensor, cache: KVCache) -> torch.Tensor:
+        """Take every sequence one token further: ``tokens[batch]`` go to the end of the cache; returns the logits
+        ``[batch, vocab]`` behind them."""
+        if tokens.shape != cache.lengths.shape:
+            raise ValueError('decode takes one token per sequence of the cache')
+        if not 1 <= cache.used < cache.capacity:
+            raise ValueError(f'the cache holds {cache.used} of {cache.capacity} tokens: it has to be filled first and '
+                             'have room for one more')
+        at = cache.lengths.long()
+        cache.lengths += 1
+        cache.used += 1
+        rope = self._rope_for(cache.capacity, tokens.device)
+        if rope is not None:
+            rope = tuple(t[at] for t in rope)       # each sequence at its own position
+
+        def attend(layer, attention, normed):
+            return attention.decode(normed, rope, cache.keys[layer], cache.values[layer], at, cache.lengths)
+
+        x = self.wte(tokens)
+        if self.wpe is not None:
+            x = x + self.wpe(at)
+        x, delta, delta_bias = self._run_blocks(x.unsqueeze(0), attend)
+        return self.logits(_add_norm(self.ln_f, x, delta, delta_bias)[1].squeeze(0))
+
+    @torch.no_grad()
+    def generate(self, tokens: torch.Tensor, steps: int, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``steps`` most likely tokens behind each prompt: ``[batch, steps]``."""
+        if steps < 1:
+            raise ValueError('generate takes at least one step')
+        cache = self.new_cache(tokens.shape[0], tokens.shape[1] + steps)
+        out = [self.prefill(tokens, cache, lengths).argmax(dim=-1)]
+        for _ in range(steps - 1):
+            out.append(self.decode(out[-1], cache).argmax(dim=-1))
+        return torch.stack(out, dim=1)
 
     def num_parameters(self, only_active: bool = False) -> int:
         total = 0

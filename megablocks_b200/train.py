@@ -70,6 +70,9 @@ class TrainerConfig:
     # produce them instead of reading the gradients back for it (one optimizer step per backward
     # pass only: no gradient accumulation, no pipeline).
     fuse_grad_norm: bool = True
+    # Step of the routers' balancing biases (``Arguments.moe_router_bias``) against the experts' load, once per
+    # optimizer step.  0: they stay.
+    router_bias_rate: float = 0.0
 
 
 class Trainer:
@@ -142,6 +145,8 @@ class Trainer:
                 and self.expert_params and max(1, int(cfg.grad_accum_steps)) == 1 and pipeline is None):
             from megablocks_b200.ops.gg import GradNormSink
             self._norm_sink = GradNormSink(self.device)
+        from megablocks_b200.layers.router import LearnedRouter
+        self._routers = [m for m in model.modules() if isinstance(m, LearnedRouter)]
         self._graph = None           # (CUDAGraph, tokens, targets, loss, kernel launches per replay)
         self._eager_steps = 0
 
@@ -213,26 +218,37 @@ class Trainer:
         for p in self.expert_params:
             p.grad = None
 
-    def _forward_backward(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-        """All micro-batches of one step; returns the mean language-model loss (device scalar)."""
+    def _loss(self, tokens, targets, teacher):
+        if teacher is None:
+            return self.model.loss(tokens, targets)
+        return self.model.distillation_loss(tokens, teacher, targets)
+
+    def _forward_backward(self, tokens: torch.Tensor, targets: torch.Tensor, teacher=None) -> torch.Tensor:
+        """All micro-batches of one step; returns the mean language-model (or distillation) loss (device scalar)."""
         n = max(1, int(self.cfg.grad_accum_steps))
         scale = (self.scaler.scale if self.scaler is not None else 1.0) / n
         if self.pipeline is not None:
+            if teacher is not None:
+                raise ValueError('a pipeline stage cannot be distilled')
             return self._pipeline_forward_backward(tokens, targets, n, scale)
         if n == 1:
             with nvtx_range('forward'):
-                total, lm = self.model.loss(tokens, targets)
+                total, lm = self._loss(tokens, targets, teacher)
             with nvtx_range('backward'):
                 (total if scale == 1.0 else total * scale).backward()
             return lm
         if tokens.shape[0] % n:
             raise ValueError(f'batch of {tokens.shape[0]} rows does not split into {n} micro-batches')
         lm_sum = None
+        teachers = [None] * n
+        if teacher is not None:
+            teachers = [teacher._replace(logits=a, ids=b)
+                        for a, b in zip(teacher.logits.chunk(n), teacher.ids.chunk(n))]
         for i, (tok, tgt) in enumerate(zip(tokens.chunk(n), targets.chunk(n))):
             if self.reducer is not None:
                 self.reducer.active = i == n - 1
             with nvtx_range('forward'):
-                total, lm = self.model.loss(tok, tgt)
+                total, lm = self._loss(tok, tgt, teachers[i])
             with nvtx_range('backward'):
                 (total * scale).backward()
             lm_sum = lm if lm_sum is None else lm_sum + lm
@@ -367,8 +383,13 @@ class Trainer:
         if isinstance(self.expert_opt, FusedAdam):
             self.expert_opt.hyper = None
 
-    def step(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-        """Forward, backward, gradient reduction, clipping and the optimizer update.
+    def step(self, tokens: torch.Tensor, targets: torch.Tensor, teacher=None) -> torch.Tensor:
+        """Forward, backward, gradient reduction, clipping, the optimizer update and the step of the
+        routers' balancing biases (``cfg.router_bias_rate``).
+
+        ``teacher`` (a :class:`megablocks_b200.models.transformer.Teacher` for the batch): the model is
+        distilled from its logits instead, and the loss returned is that of ``model.distillation_loss``;
+        such a step runs kernel by kernel.
 
         ``tokens`` / ``targets`` hold this rank's whole share of the step: ``grad_accum_steps``
         micro-batches stacked along dimension 0.  Returns the language-model loss as a device
@@ -378,6 +399,13 @@ class Trainer:
         one records the step in a CUDA graph, and every call from then on copies the batch into the
         graph's input buffers and replays it.
         """
+        loss = self._step_eager(tokens, targets, teacher=teacher) if teacher is not None else self._step(tokens, targets)
+        if self.cfg.router_bias_rate:        # outside the recorded step: the loads are summed over the ranks
+            from megablocks_b200.layers.router import balance_routers
+            balance_routers(self._routers, self.cfg.router_bias_rate, self.dp_group if self.world > 1 else None)
+        return loss
+
+    def _step(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         if self._graph_eligible():
             if self._graph is not None:
                 _, static_tokens, _, _, _ = self._graph
@@ -417,7 +445,8 @@ class Trainer:
             self.drop_graph()        # past the end of the schedule table: back to plain launches
         return self._step_eager(tokens, targets)
 
-    def _step_eager(self, tokens: torch.Tensor, targets: torch.Tensor, zero_grad: bool = True) -> torch.Tensor:
+    def _step_eager(self, tokens: torch.Tensor, targets: torch.Tensor, zero_grad: bool = True,
+                    teacher=None) -> torch.Tensor:
         cfg = self.cfg
         self.model.train()
         if zero_grad:
@@ -428,11 +457,11 @@ class Trainer:
             sink.begin()
             gg.set_grad_norm_sink(sink)
             try:
-                lm = self._forward_backward(tokens, targets)
+                lm = self._forward_backward(tokens, targets, teacher)
             finally:
                 gg.set_grad_norm_sink(None)
         else:
-            lm = self._forward_backward(tokens, targets)
+            lm = self._forward_backward(tokens, targets, teacher)
         with nvtx_range('grad_reduce_wait'):
             if self.reducer is not None:
                 self.reducer.finish()
@@ -639,6 +668,13 @@ def main(argv=None):
     ap.add_argument('--top-k', type=int, default=None)
     ap.add_argument('--loss-weight', type=float, default=0.1)
     ap.add_argument('--capacity-factor', type=int, default=None, help='token-dropping MoE with this capacity factor')
+    ap.add_argument('--router-score', choices=['softmax', 'sigmoid'], default='softmax')
+    ap.add_argument('--router-groups', type=int, default=1, help='groups of experts; tokens choose within the best')
+    ap.add_argument('--router-top-groups', type=int, default=None, help='groups a token chooses from (default: all)')
+    ap.add_argument('--router-bias-rate', type=float, default=0.0,
+                    help='balance the experts by a bias on the choice that moves this far per step')
+    ap.add_argument('--attention-window', type=int, default=None, help='sliding window of the attention, in tokens')
+    ap.add_argument('--attention-sinks', type=int, default=0, help='first tokens that every token sees')
     ap.add_argument('--mlp-impl', choices=['grouped', 'sparse'], default='grouped')
     ap.add_argument('--lr', type=float, default=6e-4)
     ap.add_argument('--min-lr', type=float, default=6e-5)
@@ -692,7 +728,10 @@ def main(argv=None):
                      ep_fused_comm={'auto': None, 'fused': True, 'nccl': False}[args.ep_comm],
                      dtype=(torch.float16 if args.precision == 'fp16' else torch.bfloat16) if use_cuda
                      else torch.float32,
-                     pipeline_stages=pp, pipeline_stage=stage_index)
+                     pipeline_stages=pp, pipeline_stage=stage_index,
+                     moe_router_score=args.router_score, moe_router_groups=args.router_groups,
+                     moe_router_top_groups=args.router_top_groups, moe_router_bias=args.router_bias_rate != 0,
+                     attention_window=args.attention_window, attention_sinks=args.attention_sinks)
     if args.init_std is not None:
         overrides['init_std'] = args.init_std
     accum = 1
@@ -718,7 +757,8 @@ def main(argv=None):
     trainer = Trainer(model, TrainerConfig(lr=args.lr, min_lr=args.min_lr, total_steps=args.steps, zero1=args.zero1,
                                            overlap_expert_update=args.defer_expert_update, dp_backend=args.dp_comm,
                                            grad_accum_steps=accum, optimizer=args.optimizer,
-                                           cuda_graph=args.cuda_graph),
+                                           cuda_graph=args.cuda_graph,
+                                           router_bias_rate=args.router_bias_rate),
                       dp_group=group, pipeline=stage)
     if args.load:
         state = checkpoint.load(args.load, rank, world, map_location=device)

@@ -1,0 +1,253 @@
+"""Expert selection, windowed attention, distillation and decoding as a model uses them together."""
+
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+from conftest import DEVICES
+
+from megablocks_b200 import Arguments, MoE, dMoE
+from megablocks_b200.layers import router as router_lib
+from megablocks_b200.models.transformer import MoETransformer, Teacher, preset
+from megablocks_b200.ops import select_experts
+from megablocks_b200.train import Trainer, TrainerConfig
+
+OPTIONS = dict(moe_router_score='sigmoid', moe_router_bias=True, moe_router_groups=2, moe_router_top_groups=1,
+               moe_router_scale=1.5, attention_window=9, attention_sinks=2, moe_num_experts=8, moe_loss_weight=0.0)
+
+
+def build(device, name='tiny-mixtral', **options):
+    dtype = torch.bfloat16 if device == 'cuda' else torch.float32
+    torch.manual_seed(7)
+    model = MoETransformer(preset(name, device=torch.device(device), dtype=dtype, **{**OPTIONS, **options}))
+    return model
+
+
+def teacher_for(cfg, batch, seq, device, top=5, hard=0.5):
+    logits = torch.randn(batch, seq, top, device=device) * 2
+    ids = torch.randint(0, cfg.vocab_size, (batch, seq, top), device=device, dtype=torch.int32)
+    ids[:, -3:] = -1                    # a padded tail
+    return Teacher(logits, ids, temperature=2.0, hard_weight=hard)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('layer', [dMoE, MoE])
+@pytest.mark.parametrize('norm', [None, 1])
+def test_layer_routes_by_select_experts(device, layer, norm):
+    args = Arguments(hidden_size=128, ffn_hidden_size=256, moe_num_experts=16, moe_top_k=3, moe_capacity_factor=8,
+                     moe_router_score='sigmoid', moe_router_bias=True, moe_router_groups=4, moe_router_top_groups=2,
+                     moe_router_scale=2.5, moe_normalize_expert_weights=norm, moe_loss_weight=0.1, bias=False,
+                     fp16=False, bf16=device == 'cuda', device=torch.device(device))
+    moe = layer(args).train()
+    moe.router.expert_bias.copy_(torch.randn(16) * 0.1)
+    x = torch.randn(40, 1, 128, device=device, dtype=moe.router.layer.weight.dtype, requires_grad=True)
+    scores, weights, experts = moe.router(x)
+    logits = moe.router.layer(x.reshape(-1, 128))
+    want = select_experts(logits, 3, score='sigmoid', bias=moe.router.expert_bias, groups=4, top_groups=2,
+                          norm_p=norm, scale=2.5)
+    for a, b in zip((scores, weights, experts), want):
+        assert torch.equal(a, b)
+    out = moe(x)
+    out = out[0] if isinstance(out, tuple) else out
+    assert torch.equal(moe.router.expert_load, moe.experts.last_tokens_per_expert.long())
+    assert int(moe.router.expert_load.sum()) == 120
+    out.float().square().sum().backward()
+    assert torch.isfinite(moe.router.layer.weight.grad).all() and moe.router.layer.weight.grad.any()
+    moe.eval()(x)
+    assert int(moe.router.expert_load.sum()) == 120        # only training counts
+
+
+def test_default_router_is_as_it_was():
+    args = Arguments(hidden_size=64, moe_num_experts=8, moe_top_k=2, fp16=False, device=torch.device('cpu'))
+    router = router_lib.LearnedRouter(args)
+    assert list(router.state_dict()) == ['layer.weight'] and not router._selects
+    for bad in (dict(moe_router_score='tanh'), dict(moe_router_groups=3), dict(moe_router_groups=0),
+                dict(moe_router_groups=2, moe_router_top_groups=3), dict(moe_router_top_groups=0)):
+        with pytest.raises(ValueError):
+            Arguments(moe_num_experts=8, **bad)
+
+
+def test_bias_keeps_32_bits_and_is_saved():
+    args = Arguments(hidden_size=64, moe_num_experts=8, moe_top_k=2, fp16=False, device=torch.device('cpu'),
+                     moe_router_bias=True)
+    router = router_lib.LearnedRouter(args).bfloat16()
+    assert router.layer.weight.dtype == torch.bfloat16 and router.expert_bias.dtype == torch.float32
+    assert sorted(router.state_dict()) == ['expert_bias', 'layer.weight']
+    router.count_load(torch.tensor([8, 0, 4, 4, 4, 4, 4, 4], dtype=torch.int32))
+    other = router_lib.LearnedRouter(Arguments(hidden_size=64, moe_num_experts=4, moe_top_k=2, fp16=False,
+                                               device=torch.device('cpu'), moe_router_bias=True))
+    other.count_load(torch.tensor([1, 2, 3, 2]))
+    router_lib.balance_routers([router, other], 0.25)
+    assert router.expert_bias.tolist() == [-0.25, 0.25, 0, 0, 0, 0, 0, 0]
+    assert other.expert_bias.tolist() == [0.25, 0, -0.25, 0]
+    assert not router.expert_load.any() and not other.expert_load.any()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('name', ['tiny', 'tiny-mixtral'])
+def test_a_distilled_step(device, name):
+    """Forward, backward and update with everything on: gradients arrive everywhere, biases move against the load."""
+    model = build(device, name)
+    cfg = model.cfg
+    trainer = Trainer(model, TrainerConfig(lr=1e-3, total_steps=10, router_bias_rate=0.01, grad_accum_steps=2))
+    tokens = torch.randint(0, cfg.vocab_size, (4, 33), device=device)
+    teacher = teacher_for(cfg, 4, 32, device)
+    before = [r.expert_bias.clone() for r in trainer._routers]
+    loss = trainer.step(tokens[:, :-1], tokens[:, 1:], teacher=teacher)
+    assert torch.isfinite(loss) and loss.dim() == 0
+    for p in model.parameters():
+        assert p.grad is None or torch.isfinite(p.grad).all()
+    for old, router in zip(before, trainer._routers):
+        moved = router.expert_bias - old
+        assert moved.any() and not router.expert_load.any()
+        assert all(abs(abs(v) - 0.01) < 1e-7 or v == 0 for v in moved.tolist())
+    loss = trainer.step(tokens[:, :-1], tokens[:, 1:])          # and an ordinary step
+    assert torch.isfinite(loss)
+
+
+def test_distillation_gradient_of_a_model_against_differences():
+    """fp32 on the CPU: the directional derivative of the total loss along the parameters of head, attention and
+    norms.  Central differences: cancellation 2^-23 x loss / step, truncation step^2; step 2^-6 of a unit
+    direction leaves both below 1e-3 of a gradient of size one."""
+    model = build('cpu', moe_router_bias=False)
+    with torch.no_grad():       # experts chosen by a wide margin: the choice does not flip within the step
+        for block in model.blocks:
+            block.moe.router.layer.weight.mul_(0)
+    tokens = torch.randint(0, 512, (2, 20))
+    teacher = teacher_for(model.cfg, 2, 20, 'cpu')
+    params = [p for n, p in model.named_parameters() if 'attn' in n or 'ln' in n or 'lm_head' in n]
+    total, _ = model.distillation_loss(tokens, teacher, tokens.roll(-1, 1))
+    grads = torch.autograd.grad(total, params)
+    way = [torch.randn_like(p) for p in params]
+    norm = math.sqrt(sum(float(w.square().sum()) for w in way))
+    way = [w / norm for w in way]
+    want = sum(float((g * w).double().sum()) for g, w in zip(grads, way))
+    size = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    ends = []
+    for sign in (1, -1):
+        with torch.no_grad():
+            for p, w in zip(params, way):
+                p.add_(w, alpha=sign * 2.0**-6)
+            ends.append(float(model.distillation_loss(tokens, teacher, tokens.roll(-1, 1))[0].double()))
+            for p, w in zip(params, way):
+                p.sub_(w, alpha=sign * 2.0**-6)
+    assert abs((ends[0] - ends[1]) / 2.0**-5 - want) <= 2e-3 * (1 + size)
+
+
+def fixed_choice(model):
+    """Every token takes the same experts, whatever its rounding: decoding and the whole sequence agree."""
+    with torch.no_grad():
+        for block in model.blocks:
+            block.moe.router.layer.weight.zero_()
+            block.moe.router.expert_bias.copy_(torch.linspace(0.5, -0.5, model.cfg.moe_num_experts))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('name', ['tiny', 'tiny-mixtral'])
+@pytest.mark.parametrize('window,sinks', [(9, 2), (None, 0), (1, 0)])
+def test_decoding_agrees_with_the_whole_sequence(device, name, window, sinks):
+    """Logits of a prompt and of each token decoded behind it against one pass over the whole sequence.
+
+    On the CPU in fp32 the two differ by sums of another order.  In bf16 each of the two layers rounds some ten
+    tensors by half a step, which norms pass on at about their size: twice 2 x 10 x 2^-8 of the largest logit.  A
+    token in a wrong place, or a key too many or too few, moves logits by their own size."""
+    model = build(device, name, attention_window=window, attention_sinks=sinks).eval()
+    fixed_choice(model)
+    batch, prompt, extra = 3, 21, 8
+    tokens = torch.randint(0, 512, (batch, prompt + extra), device=device)
+    lengths = torch.tensor([prompt, 13, 1], dtype=torch.int32, device=device)
+    cache = model.new_cache(batch, prompt + extra)
+    got = [model.prefill(tokens[:, :prompt], cache, lengths)]
+    for i in range(extra - 1):
+        step = tokens[torch.arange(batch), (lengths + i).long()]
+        got.append(model.decode(step, cache))
+    assert cache.lengths.tolist() == [n + extra - 1 for n in lengths.tolist()]
+    with torch.no_grad():
+        for b, n in enumerate(lengths.tolist()):
+            whole = model(tokens[b:b + 1, :n + extra - 1])[0].float()
+            size = whole.abs().max()
+            for i in range(extra):
+                bound = size * (2.0**-12 if device == 'cpu' else 40 * 2.0**-8)
+                assert (got[i][b].float() - whole[n - 1 + i]).abs().max() <= bound
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_generate_and_refusals(device):
+    model = build(device, 'tiny').eval()
+    tokens = torch.randint(0, 512, (2, 6), device=device)
+    out = model.generate(tokens, 5, torch.tensor([6, 2], device=device))
+    assert out.shape == (2, 5) and ((out >= 0) & (out < 512)).all()
+    with pytest.raises(ValueError):
+        model.generate(tokens, 0)
+    with pytest.raises(ValueError):
+        model.new_cache(2, 65)                  # the model has 64 positions
+    cache = model.new_cache(2, 7)
+    with pytest.raises(ValueError):
+        model.decode(tokens[:, 0], cache)       # nothing in it yet
+    with pytest.raises(ValueError):
+        model.prefill(tokens.repeat(1, 2), cache)
+    with pytest.raises(ValueError):
+        model.prefill(tokens[:1], cache)
+    model.prefill(tokens, cache)
+    model.decode(tokens[:, 0], cache)
+    with pytest.raises(ValueError):
+        model.decode(tokens[:, 0], cache)       # full
+    with pytest.raises(ValueError):
+        model.distillation_loss(tokens, Teacher(torch.zeros(2, 5, 3, device=device),
+                                                torch.zeros(2, 5, 3, device=device, dtype=torch.int64)))
+
+
+@pytest.mark.gpu
+def test_recorded_step_counts_and_balances_like_the_eager_one():
+    runs = []
+    for graph in (False, True):
+        model = build('cuda', 'tiny')
+        trainer = Trainer(model, TrainerConfig(lr=1e-3, total_steps=20, router_bias_rate=0.01, cuda_graph=graph,
+                                               graph_warmup_steps=2))
+        gen = torch.Generator(device='cuda').manual_seed(3)
+        for _ in range(6):
+            tokens = torch.randint(0, 512, (4, 65), device='cuda', generator=gen)
+            trainer.step(tokens[:, :-1], tokens[:, 1:])
+        assert (trainer._graph is not None) == graph
+        runs.append(torch.stack([r.expert_bias for r in trainer._routers]))
+    assert torch.equal(runs[0], runs[1]) and runs[0].any()
+
+
+_RANK = '''
+import sys, torch, torch.distributed as dist
+sys.path.insert(0, {root!r})
+from megablocks_b200 import Arguments
+from megablocks_b200.layers import router as R
+rank = int(sys.argv[1])
+dist.init_process_group('gloo', init_method='tcp://127.0.0.1:{port}', rank=rank, world_size=2)
+r = R.LearnedRouter(Arguments(hidden_size=8, moe_num_experts=4, moe_top_k=1, fp16=False, moe_router_bias=True,
+                              device=torch.device('cpu')))
+r.count_load(torch.tensor([[4, 0, 2, 2], [0, 1, 3, 4]][rank]))      # together 4, 1, 5, 6: mean 4
+R.balance_routers([r], 0.5, dist.group.WORLD)
+assert r.expert_bias.tolist() == [0.0, 0.5, -0.5, -0.5], r.expert_bias
+dist.destroy_process_group()
+'''
+
+
+def test_ranks_sum_their_loads():
+    import socket
+    with socket.socket() as s:
+        s.bind(('127.0.0.1', 0))
+        port = s.getsockname()[1]
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = _RANK.format(root=root, port=port)
+    procs = [subprocess.Popen([sys.executable, '-c', code, str(r)]) for r in range(2)]
+    assert [p.wait(timeout=120) for p in procs] == [0, 0]
+
+
+def test_command_line():
+    from megablocks_b200 import train
+    if torch.cuda.is_available():
+        pytest.skip('the CPU run of the command')
+    loss = train.main(['--preset', 'tiny', '--steps', '2', '--micro-batch', '2', '--router-score', 'sigmoid',
+                       '--router-groups', '2', '--router-top-groups', '1', '--router-bias-rate', '0.01',
+                       '--loss-weight', '0', '--attention-window', '16', '--attention-sinks', '2'])
+    assert torch.isfinite(loss)
