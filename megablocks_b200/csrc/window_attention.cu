@@ -10,7 +10,9 @@
 // for larger ones, whose keys and values are twice as many bytes a product, as one CTA that loads them once
 // for both.  The running maximum follows a row lazily: O is scaled again only when
 // the maximum has grown by 2^8, which leaves probabilities at most 256 times their value and sums in 32 bits.
-// Tiles that no query of a group sees are not loaded, and only tiles on the window's edges are masked.
+// Tiles that no query of a group sees are not loaded.  Within a tile a warp takes 32 keys at a time: those that
+// none of its queries sees cost it nothing, and only those on an edge are masked.  The product with V starts
+// on the first half of a tile's probabilities while the second half is taken.
 #include "window_attention.cuh"
 
 namespace mb {
@@ -54,33 +56,16 @@ struct Tiles {
   __device__ __forceinline__ bool wanted(int g, int j) const { return j <= hi[g] && (j >= lo[g] || j < sink_tiles); }
 };
 
-// Scores of a row's tile into probabilities, in place.  `m` is the reference of the exponent, `sum` the sum of
-// the probabilities; `to` the row's sum in tensor memory, which is scaled when the reference moves.
-template <typename T, int D, bool EDGE>
-__device__ __forceinline__ void row_tile(uint32_t ts, uint32_t to, float scale, int from, int upto, int keep, bool first,
-                                         float& m, float& sum) {
-  uint32_t s[kTile];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, chunk_of(s, c));
-  tmem_ld_wait();
-  if constexpr (EDGE) {
-#pragma unroll
-    for (int k = 0; k < kTile; ++k)
-      if (!(k <= upto && (k >= from || k < keep))) s[k] = 0xff800000u;        // -infinity
-  }
-  float top4[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) top4[c] = __uint_as_float(s[c]);
-#pragma unroll
-  for (int k = 4; k < kTile; k += 4)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) top4[c] = fmaxf(top4[c], __uint_as_float(s[k + c]));
-  const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale;
-  // The sum of the tile before is complete: its MMAs precede the ones that made these scores.
-  const bool grow = top > m + kLazy;
-  const float factor = grow ? exp2_approx(m - top) : 1.f;
-  if (grow) { m = top; sum *= factor; }
-  if (!first && __any_sync(0xffffffffu, grow)) {
+// Running reference of a row's exponent (scaled) and sum of its probabilities.  The sum in tensor memory, `to`,
+// is scaled when the reference moves; it is complete, its MMAs precede the ones that made the scores at hand.
+struct RowState {
+  float m = -INFINITY, sum = 0.f;
+  template <int D>
+  __device__ __forceinline__ void follow(float top, uint32_t to, bool first) {
+    const bool grow = top > m + kLazy;
+    const float factor = grow ? exp2_approx(m - top) : 1.f;
+    if (grow) { m = top; sum *= factor; }
+    if (first || !__any_sync(0xffffffffu, grow)) return;
 #pragma unroll 1
     for (int c = 0; c < D / 16; ++c) {
       uint32_t raw[16];
@@ -91,22 +76,103 @@ __device__ __forceinline__ void row_tile(uint32_t ts, uint32_t to, float scale, 
       tmem_st_32x16(to + c * 16, raw);
     }
   }
-  const float2 scale2 = splat2(scale), base2 = splat2(m == -INFINITY ? 0.f : -m);
+};
+
+__device__ __forceinline__ float chunk_max(const uint32_t (&s)[32]) {
+  float top[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) top[x] = __uint_as_float(s[x]);
+#pragma unroll
+  for (int k = 4; k < 32; k += 4)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], __uint_as_float(s[k + x]));
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// Probabilities of 32 scores, rounded over them to 8 or 11 bits for the product; the sum takes them whole.
+template <typename T>
+__device__ __forceinline__ void chunk_exp(const uint32_t (&s)[32], uint32_t out, float2 scale2, float2 base2,
+                                          float2 (&part)[2]) {
+  uint32_t packed[16];
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const float2 e = exp2_pair(__ffma2_rn(pair_of(s[2 * x], s[2 * x + 1]), scale2, base2));
+    part[x & 1] = __fadd2_rn(part[x & 1], e);
+    packed[x] = pack2<T>(e.x, e.y);
+  }
+  tmem_st_32x16(out, packed);
+}
+
+__device__ __forceinline__ void arrive_stored(uint32_t bar, int lane) {
+  tmem_st_wait();
+  tcgen05_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+// Scores of a row's tile into probabilities, in place; `half_done` and `done` get the warp's arrivals.
+template <typename T, int D>
+__device__ __forceinline__ void row_tile(uint32_t ts, uint32_t to, float scale, int lane, bool first, RowState& row,
+                                         uint32_t half_done, uint32_t done) {
+  uint32_t s[kTile];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, chunk_of(s, c));
+  tmem_ld_wait();
+  const float top = fmaxf(fmaxf(chunk_max(chunk_of(s, 0)), chunk_max(chunk_of(s, 1))),
+                          fmaxf(chunk_max(chunk_of(s, 2)), chunk_max(chunk_of(s, 3))));
+  row.follow<D>(top * scale, to, first);
+  const float2 scale2 = splat2(scale), base2 = splat2(row.m == -INFINITY ? 0.f : -row.m);
   float2 part[2] = {splat2(0.f), splat2(0.f)};
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint32_t packed[16];
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      const float2 e = exp2_pair(__ffma2_rn(pair_of(s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]), scale2, base2));
-      part[x & 1] = __fadd2_rn(part[x & 1], e);
-      packed[x] = pack2<T>(e.x, e.y);  // 8 or 11 bits for the product; the sum takes them whole
-    }
-    tmem_st_32x16(ts + c * 16, packed);                // over scores that this thread has read
+    chunk_exp<T>(chunk_of(s, c), ts + c * 16, scale2, base2, part);
+    if (c & 1) arrive_stored(c == 1 ? half_done : done, lane);
   }
   part[0] = __fadd2_rn(part[0], part[1]);
-  sum += part[0].x + part[0].y;
-  tmem_st_wait();
+  row.sum += part[0].x + part[0].y;
+}
+
+// The same for a tile on an edge: 32 keys at a time, those left out that none of the warp's queries (`i0` and 31
+// more) sees of the keys from `k0` on.  The scores are read twice instead of being kept.
+template <typename T, int D>
+__device__ __forceinline__ void row_edge_tile(uint32_t ts, uint32_t to, float scale, int i0, int k0, const Params& p,
+                                              int lane, bool first, RowState& row, uint32_t half_done, uint32_t done) {
+  const int upto = i0 + lane - k0, from = upto - p.window + 1, keep = p.sinks - k0;
+  uint32_t s[32];
+  auto load = [&](int c, Sight seen) {
+    tmem_ld_32x32(ts + c * 32, s);
+    tmem_ld_wait();
+    if (seen == kAll) return;
+    const int to_c = upto - c * 32, from_c = from - c * 32, keep_c = keep - c * 32;
+#pragma unroll
+    for (int k = 0; k < 32; ++k)
+      if (!(k <= to_c && (k >= from_c || k < keep_c))) s[k] = 0xff800000u;    // -infinity
+  };
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const Sight seen = sight(i0, k0 + c * 32, p.window, p.sinks);
+    if (seen == kNone) continue;
+    load(c, seen);
+    top = fmaxf(top, chunk_max(s));
+  }
+  row.follow<D>(top * scale, to, first);
+  const float2 scale2 = splat2(scale), base2 = splat2(row.m == -INFINITY ? 0.f : -row.m);
+  float2 part[2] = {splat2(0.f), splat2(0.f)};
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const Sight seen = sight(i0, k0 + c * 32, p.window, p.sinks);
+    if (seen == kNone) {
+      const uint32_t zeros[16] = {};
+      tmem_st_32x16(ts + c * 16, zeros);
+    } else {
+      load(c, seen);
+      chunk_exp<T>(s, ts + c * 16, scale2, base2, part);
+    }
+    if (c & 1) arrive_stored(c == 1 ? half_done : done, lane);
+  }
+  part[0] = __fadd2_rn(part[0], part[1]);
+  row.sum += part[0].x + part[0].y;
 }
 
 template <typename T, int D>
@@ -125,7 +191,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* empty = bars + kStages;
   uint64_t* q_full = bars + 2 * kStages;           // [G]
   uint64_t* s_full = q_full + G;                   // [G] scores of a group are in tensor memory
-  uint64_t* p_full = s_full + G;                   // [G] its probabilities are
+  uint64_t* p_half = s_full + G;                   // [G] half its probabilities are
+  uint64_t* p_full = p_half + G;                   // [G] all are
   uint64_t* o_full = p_full + G;                   // [G] its sum is complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + G);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -145,6 +212,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (int g = 0; g < G; ++g) {
       mbar_init(smem_u32(&q_full[g]), 1);
       mbar_init(smem_u32(&s_full[g]), 1);
+      mbar_init(smem_u32(&p_half[g]), 4);
       mbar_init(smem_u32(&p_full[g]), 4);
       mbar_init(smem_u32(&o_full[g]), 1);
     }
@@ -191,16 +259,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     constexpr uint32_t idesc_o = instr_desc_f16(kIsBf16<T>, false, true, kTile, D);
     const uint32_t q_base = uniform(smem_u32(tile_q)), ring_base = uniform(smem_u32(ring)), ts = uniform(tmem_s),
                    to = uniform(tmem_o);
+    const uint32_t bar0 = uniform(smem_u32(bars));                          // full[], empty[], then the groups'
+    auto bar_of = [&](const uint64_t* bar) { return bar0 + uint32_t(bar - bars) * 8; };
+    IssueWait wait{abort_flag, p.status, false};
     int stage = 0;
-    uint32_t phase = 0, p_phase[G] = {};
-    bool started[G] = {}, ok = true;
+    uint32_t phase = 0, p_phase = 0;                                        // p_phase: a bit a group
+    bool started[G] = {};
     auto next = [&] {
       if (++stage == kStages) { stage = 0; phase ^= 1u; }
-    };
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && mbar_wait(smem_u32(bar), parity, abort_flag, p.status, kErrMma, kWaitNs);
-      ok = __all_sync(0xffffffffu, ok);
-      tcgen05_fence_after();
     };
     auto scores = [&](int g) {         // S_g = Q_g K^T with K in the current stage
       if (elect_one()) {
@@ -208,56 +274,60 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
           umma_f16(ts + g * kTile, desc_along_dim<kTile>(q, i), desc_along_dim<kTile>(k, i), idesc_s, i != 0);
-        umma_commit(smem_u32(&s_full[g]));
+        umma_commit(bar_of(&s_full[g]));
       }
       __syncwarp();
     };
     if (tiles.count > 0) {
-      wait(&full[stage], phase);
+      wait(bar_of(&full[stage]), phase);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        if (!ok || !tiles.wanted(g, tiles.at(0))) continue;
-        wait(&q_full[g], 0);
-        if (ok) scores(g);
+        if (!tiles.wanted(g, tiles.at(0))) continue;
+        wait(bar_of(&q_full[g]), 0);
+        scores(g);
       }
-      if (ok && elect_one()) umma_commit(smem_u32(&empty[stage]));
+      if (elect_one()) umma_commit(bar_of(&empty[stage]));
       __syncwarp();
       next();
     }
-    for (int t = 0; t < tiles.count && ok; ++t) {
-      const int j = tiles.at(t);
+    for (int t = 0; t < tiles.count; ++t) {
+      const int j = tiles.at(t), j_next = tiles.at(t + 1);
       const int v_stage = stage;
-      wait(&full[v_stage], phase);
-      if (!ok) break;
+      const bool more = t + 1 < tiles.count;
+      wait(bar_of(&full[v_stage]), phase);
       if ((j + 1) * kTile > len)
         zero_rows<kTile, D>(ring + v_stage * kTileBytes, len - j * kTile, lane);
       next();
-      const bool more = t + 1 < tiles.count;
-      if (more) wait(&full[stage], phase);
+      const uint32_t v = ring_base + v_stage * kTileBytes;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        if (ok && tiles.wanted(g, j)) {
-          wait(&p_full[g], p_phase[g]);
-          p_phase[g] ^= 1u;
-          if (ok && elect_one()) {
-            const uint32_t v = ring_base + v_stage * kTileBytes;
+        if (tiles.wanted(g, j)) {
+          auto product = [&](int from) {
 #pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)
-              umma_f16_ta(to + g * D, ts + g * kTile + i * 8, desc_along_rows<kTile>(v, i), idesc_o,
-                          started[g] || i != 0);
-            if (j == tiles.hi[g]) umma_commit(smem_u32(&o_full[g]));
+            for (int i = from; i < from + kTile / 32; ++i)
+              umma_f16_ta(to + g * D, ts + g * kTile + i * 8, desc_along_rows<kTile>(v, i), idesc_o, started[g] || i != 0);
+          };
+          wait(bar_of(&p_half[g]), (p_phase >> g) & 1u);
+          if (elect_one()) product(0);
+          __syncwarp();
+          wait(bar_of(&p_full[g]), (p_phase >> g) & 1u);
+          if (elect_one()) {
+            product(kTile / 32);
+            if (j == tiles.hi[g]) umma_commit(bar_of(&o_full[g]));
           }
           __syncwarp();
+          p_phase ^= 1u << g;
           started[g] = true;
         }
-        if (ok && more && tiles.wanted(g, tiles.at(t + 1))) {
-          if (!started[g]) wait(&q_full[g], 0);
-          if (ok) scores(g);
+        if (more && tiles.wanted(g, j_next)) {
+          if (!started[g]) wait(bar_of(&q_full[g]), 0);
+          wait(bar_of(&full[stage]), phase);           // passes at once for the second group
+          scores(g);
         }
       }
-      if (ok && elect_one()) {
-        umma_commit(smem_u32(&empty[v_stage]));
-        if (more) umma_commit(smem_u32(&empty[stage]));
+      if (elect_one()) {
+        umma_commit(bar_of(&empty[v_stage]));
+        if (more) umma_commit(bar_of(&empty[stage]));
       }
       __syncwarp();
       if (more) next();
@@ -269,7 +339,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t ts = tmem_s + g * kTile + lanes, to = tmem_o + g * D + lanes;
     const float scale = p.scale * kLog2e;
-    float m = -INFINITY, sum = 0.f;    // reference of the exponent (scaled), sum of the probabilities
+    RowState row;
     uint32_t s_phase = 0;
     bool ok = true, first = true;
     const int lo = G > 1 && g > 0 ? tiles.lo[G - 1] : tiles.lo[0], hi = G > 1 && g > 0 ? tiles.hi[G - 1] : tiles.hi[0];
@@ -282,16 +352,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!ok) break;
       s_phase ^= 1u;
       tcgen05_fence_after();
-      // Visible keys of this row in the tile: from the window's first to its own, and the first tokens.
-      const int k0 = j * kTile, upto = i - k0, from = upto - p.window + 1, keep = p.sinks - k0;
-      if (k0 + kTile - 1 > g0 || g0 + kTile - 1 - k0 >= p.window)
-        row_tile<T, D, true>(ts, to, scale, from, upto, keep, first, m, sum);
+      const int i0 = g0 + quarter * 32, k0 = j * kTile;
+      const uint32_t half_done = smem_u32(&p_half[g]), done = smem_u32(&p_full[g]);
+      if (k0 + kTile - 1 <= i0 && k0 > i0 + 31 - p.window)         // the whole tile in the window
+        row_tile<T, D>(ts, to, scale, lane, first, row, half_done, done);
       else
-        row_tile<T, D, false>(ts, to, scale, from, upto, keep, first, m, sum);
+        row_edge_tile<T, D>(ts, to, scale, i0, k0, p, lane, first, row, half_done, done);
       first = false;
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&p_full[g]));
     }
     if (rows && ok) {
       ok = mbar_wait(smem_u32(&o_full[g]), 0, abort_flag, p.status, kErrRows, kWaitNs);
@@ -299,38 +366,45 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       tcgen05_fence_after();
     }
     const bool live = rows && i < len && ok;
-    const float inv = live ? 1.f / sum : 0.f;
+    const float inv = live ? 1.f / row.sum : 0.f;
     if (p.neg_lse != nullptr && i < p.seq_pad)
-      p.neg_lse[(int64_t(b) * p.heads + head) * p.seq_pad + i] = live ? -(m + __log2f(sum)) : -INFINITY;
-    // The result, and for a backward pass what its rounding left (the row sums delta want it), one after the
-    // other through the queries' tile, which has been used.
+      p.neg_lse[(int64_t(b) * p.heads + head) * p.seq_pad + i] = live ? -(row.m + __log2f(row.sum)) : -INFINITY;
+    // The result goes out through the queries' tile, which has been used.  What its rounding left, which the
+    // backward pass wants for its row sums, goes through the ring where it is free (one group has no other to
+    // wait for), else through the same tile afterwards.
     uint8_t* staged = tile_q + g * kTileBytes;
-    for (int part = 0; part < (p.out_low != nullptr ? 2 : 1); ++part) {
+    const bool low = p.out_low != nullptr;
+    constexpr int kPasses = G == 1 ? 1 : 2;
+    for (int pass = 0; pass < (low ? kPasses : 1); ++pass) {
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
-        uint32_t raw[32];
+        uint32_t raw[32], rest[32];
         if (rows && ok) {
           tmem_ld_32x32(to + c * 32, raw);
           tmem_ld_wait();
         }
 #pragma unroll
         for (int x = 0; x < 32; ++x) {                // zeros behind the end, whatever was computed there
-          float o = live ? __uint_as_float(raw[x]) * inv : 0.f;
-          if (part == 1) o -= to_float(from_float<T>(o));
+          const float o = live ? __uint_as_float(raw[x]) * inv : 0.f;
           raw[x] = __float_as_uint(o);
+          rest[x] = __float_as_uint(o - to_float(from_float<T>(o)));
         }
-        stage_row<T>(staged, r, c, raw, 1.f);
+        if (pass == 0) stage_row<T>(staged, r, c, raw, 1.f);
+        if (low && pass == kPasses - 1) stage_row<T>(G == 1 ? ring : staged, r, c, rest, 1.f);
       }
       fence_proxy_async_smem();
       group_barrier(1 + g);
       if (quarter == 0 && lane == 0 && g0 < p.seq) {
-        for (int box = 0; box < D / 64; ++box)
-          if (box * 64 < p.dim)
-            tma_store_4d(part == 0 ? &map_o : &map_low, smem_u32(staged + box * (kTile * 128)), box * 64, g0, head, b);
+        for (int box = 0; box < D / 64; ++box) {
+          if (box * 64 >= p.dim) continue;
+          if (pass == 0) tma_store_4d(&map_o, smem_u32(staged + box * (kTile * 128)), box * 64, g0, head, b);
+          if (low && pass == kPasses - 1)
+            tma_store_4d(&map_low, smem_u32((G == 1 ? ring : staged) + box * (kTile * 128)), box * 64, g0, head, b);
+        }
         bulk_commit_group();
         bulk_wait_read_all();
       }
-      group_barrier(1 + g);
+      if (G > 1) group_barrier(1 + g);
     }
   }
   tcgen05_fence_before();

@@ -97,6 +97,26 @@ __device__ __forceinline__ void group_barrier(int id) {        // the 128 thread
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
 
+// Waits of the warp that issues MMAs.  A wait that runs out is recorded; from then on none waits, the loops run
+// to their end on whatever is there, in bounds, and the result is not valid.
+struct IssueWait {
+  volatile int* abort_flag;
+  int* status;
+  bool dead;
+  __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) {
+    if (!dead && !mbar_try_wait(bar, parity))
+      dead = !mbar_wait(bar, parity, abort_flag, status, kErrMma, kWaitNs);
+    tcgen05_fence_after();
+  }
+};
+
+// How much of the 32 keys from `k0` on the 32 queries from `i0` on see.
+enum Sight { kNone, kSome, kAll };
+__device__ __forceinline__ Sight sight(int i0, int k0, int window, int sinks) {
+  if (k0 > i0 + 31 || (k0 + 31 <= i0 - window && k0 >= sinks)) return kNone;
+  return k0 + 31 <= i0 && (k0 > i0 + 31 - window || k0 + 31 < sinks) ? kAll : kSome;
+}
+
 // A wait that ran out leaves copies and MMAs in flight: give them time before tensor memory is freed.
 __device__ __forceinline__ void settle(const volatile int* abort_flag) {
   if (*abort_flag == 0) return;
