@@ -63,9 +63,11 @@ struct RowState {
   template <int D>
   __device__ __forceinline__ void follow(float top, uint32_t to, bool first) {
     const bool grow = top > m + kLazy;
-    const float factor = grow ? exp2_approx(m - top) : 1.f;
-    if (grow) { m = top; sum *= factor; }
-    if (first || !__any_sync(0xffffffffu, grow)) return;
+    const bool scale = grow && m != -INFINITY;         // without a key so far the sums are zero
+    const float factor = scale ? exp2_approx(m - top) : 1.f;
+    if (grow) m = top;
+    sum *= factor;
+    if (first || !__any_sync(0xffffffffu, scale)) return;
 #pragma unroll 1
     for (int c = 0; c < D / 16; ++c) {
       uint32_t raw[16];
@@ -143,10 +145,10 @@ __device__ __forceinline__ void row_edge_tile(uint32_t ts, uint32_t to, float sc
     tmem_ld_32x32(ts + c * 32, s);
     tmem_ld_wait();
     if (seen == kAll) return;
-    const int to_c = upto - c * 32, from_c = from - c * 32, keep_c = keep - c * 32;
+    const uint32_t bits = seen_bits(from - c * 32, upto - c * 32, keep - c * 32);
 #pragma unroll
     for (int k = 0; k < 32; ++k)
-      if (!(k <= to_c && (k >= from_c || k < keep_c))) s[k] = 0xff800000u;    // -infinity
+      if (!(bits & (1u << k))) s[k] = 0xff800000u;    // -infinity
   };
   float top = -INFINITY;
 #pragma unroll 1

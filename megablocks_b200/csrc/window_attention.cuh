@@ -117,6 +117,12 @@ __device__ __forceinline__ Sight sight(int i0, int k0, int window, int sinks) {
   return k0 + 31 <= i0 && (k0 > i0 + 31 - window || k0 + 31 < sinks) ? kAll : kSome;
 }
 
+// The keys (bits) of 32 that a row sees: [from, to], and those below `keep` up to `to`.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+__device__ __forceinline__ uint32_t seen_bits(int from, int to, int keep) {
+  return bits_below(to + 1) & (~bits_below(from) | bits_below(keep));
+}
+
 // A wait that ran out leaves copies and MMAs in flight: give them time before tensor memory is freed.
 __device__ __forceinline__ void settle(const volatile int* abort_flag) {
   if (*abort_flag == 0) return;

@@ -47,11 +47,10 @@ struct Stream {
   }
 };
 
-// Whether pair k of a row's 64 is visible: [from, to), and in the queries' kernel also [0, keep) below `to`.
+// Visible pairs of a row's 64, as bits.
 struct Seen {
-  int from, to, keep;
-  template <bool KEYS>
-  __device__ __forceinline__ bool at(int k) const { return k < to && (k >= from || (!KEYS && k < keep)); }
+  uint32_t half[2];
+  __device__ __forceinline__ bool at(int k) const { return half[k >> 5] >> (k & 31) & 1u; }
 };
 
 // Exponentials of a row's 64 scores; in the keys' kernel also rounded over the scores.  The statistics are the
@@ -75,8 +74,8 @@ __device__ __forceinline__ void row_exp(const uint32_t (&s)[64], uint32_t ts, fl
         const int k = c * 32 + 2 * (x + u);
         float2 e = exp2_pair(__ffma2_rn(pair_of(s[k], s[k + 1]), scale2, l[u]));
         if constexpr (EDGE) {
-          if (!seen.at<KEYS>(k)) e.x = 0.f;
-          if (!seen.at<KEYS>(k + 1)) e.y = 0.f;
+          if (!seen.at(k)) e.x = 0.f;
+          if (!seen.at(k + 1)) e.y = 0.f;
         }
         pr[c * 16 + x + u] = e;
         if constexpr (KEYS) packed[x + u] = pack2<T>(e.x, e.y);
@@ -109,8 +108,8 @@ __device__ __forceinline__ void row_ds(uint32_t td, const float* col, float row,
         const int k = c * 32 + 2 * (x + u);
         float2 ds = __fmul2_rn(pr[c * 16 + x + u], __fadd2_rn(pair_of(d[k], d[k + 1]), l[u]));
         if constexpr (EDGE) {
-          if (!seen.at<KEYS>(k)) ds.x = 0.f;
-          if (!seen.at<KEYS>(k + 1)) ds.y = 0.f;
+          if (!seen.at(k)) ds.x = 0.f;
+          if (!seen.at(k + 1)) ds.y = 0.f;
         }
         packed[x + u] = pack2<T>(ds.x, ds.y);
       }
@@ -247,18 +246,14 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
     const uint32_t ts = uniform(tmem), td = ts + R, ta = ts + 2 * R;
     // P and dS of 64 columns take the first 32 of the columns that their products took.
     auto at = [](int i) { return (i / 4) * 64 + (i % 4) * 8; };
-    bool ok = true;
+    const uint32_t bar0 = uniform(smem_u32(bars));
+    auto bar_of = [&](const uint64_t* bar) { return bar0 + uint32_t(bar - bars) * 8; };
+    IssueWait wait{abort_flag, p.status, false};
     int stage = 0, next = 0;           // stages of pair t and of pair t + 1
     uint32_t next_phase = 0;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && mbar_wait(smem_u32(bar), parity, abort_flag, p.status, kErrMma, kWaitNs);
-      ok = __all_sync(0xffffffffu, ok);
-      tcgen05_fence_after();
-    };
     // Products of the resident tiles with the streamed ones of stage `next`.
     auto scores = [&](int t) {
-      wait(&full[next], next_phase);
-      if (!ok) return;
+      wait(bar_of(&full[next]), next_phase);
       const int left = len - st.tile(t, KEYS) * R;
       if (left < R) {
         uint8_t* y = ring + next * 2 * kStream;
@@ -270,7 +265,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
           umma_f16(ts, desc_along_dim<kTile>(x0, i), desc_along_dim<R>(y0, i), idesc_s, i != 0);
-        umma_commit(smem_u32(s_full));
+        umma_commit(bar_of(s_full));
       }
       __syncwarp();
     };
@@ -280,21 +275,20 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
           umma_f16(td, desc_along_dim<kTile>(x1, i), desc_along_dim<R>(y1, i), idesc_s, i != 0);
-        umma_commit(smem_u32(d_full));
+        umma_commit(bar_of(d_full));
       }
       __syncwarp();
     };
     if (st.count > 0) {
-      wait(x_full, 0);
-      if (ok) scores(0);
-      if (ok) other();
+      wait(bar_of(x_full), 0);
+      scores(0);
+      other();
     }
-    for (int t = 0; t < st.count && ok; ++t) {
+    for (int t = 0; t < st.count; ++t) {
       const bool more = t + 1 < st.count;
       if (more && ++next == kStages) { next = 0; next_phase ^= 1u; }
       const uint32_t y0 = y_base + stage * 2 * kStream, y1 = y0 + kStream;
-      wait(p_done, t & 1);
-      if (!ok) break;
+      wait(bar_of(p_done), t & 1);
       if constexpr (KEYS) {
         if (elect_one()) {
 #pragma unroll
@@ -304,15 +298,13 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
         __syncwarp();
       }
       if (more) scores(t + 1);
-      if (!ok) break;
-      wait(ds_done, t & 1);
-      if (!ok) break;
+      wait(bar_of(ds_done), t & 1);
       if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < R / 16; ++i)
           umma_f16_ta(ta + (KEYS ? D : 0), td + at(i), desc_along_rows<R>(y0, i), idesc_a, t > 0 || i != 0);
-        umma_commit(smem_u32(&empty[stage]));
-        if (!more) umma_commit(smem_u32(acc_full));
+        umma_commit(bar_of(&empty[stage]));
+        if (!more) umma_commit(bar_of(acc_full));
       }
       __syncwarp();
       if (more) other();
@@ -337,19 +329,20 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
       const int y_tile = st.tile(t, KEYS) * R, y_row = y_tile + half * 64;
       // Keys' kernel: queries i = y_row + column see this key when key <= i < key + window, or from the key on
       // for a first token; behind the end none does.  Queries' kernel: keys of the window, and first tokens.
-      Seen seen{0, 64, 0};
+      int from, to, keep = 0;          // [from, to], and [0, keep) where it is not above `to`
       bool edge;
       if constexpr (KEYS) {
-        seen.from = mine - y_row;
-        seen.to = mine < p.sinks ? 64 : int(min(int64_t(64), int64_t(mine) + p.window - y_row));
-        seen.to = min(seen.to, len - y_row);
+        from = mine - y_row;
+        to = mine < p.sinks ? 63 : int(min(int64_t(63), int64_t(mine) + p.window - 1 - y_row));
+        to = min(to, len - 1 - y_row);
         edge = x_row + kTile - 1 > y_tile || (y_tile + R - 1) - x_row >= p.window || y_tile + R > len;
       } else {
-        seen.from = mine - p.window + 1 - y_row;
-        seen.to = min(64, mine + 1 - y_row);
-        seen.keep = p.sinks - y_row;
+        from = mine - p.window + 1 - y_row;
+        to = mine - y_row;
+        keep = p.sinks - y_row;
         edge = y_tile + R - 1 > x_row || (x_row + kTile - 1) - y_tile >= p.window;
       }
+      const Seen seen{{seen_bits(from, to, keep), seen_bits(from - 32, to - 32, keep - 32)}};
       const float* col = stats + stage * 2 * R + half * 64;
       ok = mbar_wait(smem_u32(s_full), t & 1, abort_flag, p.status, kErrRows, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
