@@ -20,7 +20,7 @@ namespace mb {
 namespace {
 
 constexpr int kChunks = 8;                        // most chunks of a row in shared memory
-constexpr int kMaxThreads = 512;
+constexpr int kMaxThreads = 256;
 constexpr int kRowThreads = 768;                  // most threads that work on a row in shared memory
 constexpr int kSharedBytes = 226 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;

@@ -422,7 +422,8 @@ template <typename T, int D>
 cudaError_t launch_forward(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& out,
                            const CUtensorMap& low, const Params& p, cudaStream_t stream) {
   auto kernel = window_fwd_kernel<T, D>;
-  const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes);
+  static std::atomic<bool> allowed[64];
+  const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes, allowed);
   if (rc != cudaSuccess) return rc;
   constexpr int rows = Layout<D>::kGroups * kTile;
   const dim3 grid((p.seq + rows - 1) / rows, p.heads, p.batch);

@@ -496,7 +496,8 @@ template <typename T, int D, bool KEYS>
 cudaError_t launch_backward(const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& y0, const CUtensorMap& y1,
                             const CUtensorMap& o0, const CUtensorMap& o1, const Params& p, cudaStream_t stream) {
   auto kernel = window_bwd_kernel<T, D, KEYS>;
-  const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes);
+  static std::atomic<bool> allowed[64];
+  const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes, allowed);
   if (rc != cudaSuccess) return rc;
   const int far = KEYS ? p.far_splits * ((p.sinks + kTile - 1) / kTile) : 0;
   const dim3 grid((KEYS ? p.kv_heads : p.heads) * p.batch, far + (p.seq + kTile - 1) / kTile);

@@ -9,6 +9,8 @@
 // memory and CTAs over the cluster's shared memory, in a fixed order: one launch, no workspace.  The products
 // run on warp-level MMAs: 16 rows would leave the 128-row tensor-memory ones seven eighths empty, and the
 // memory sets the pace.
+#include <cstdint>
+
 #include "window_attention.cuh"
 
 namespace mb {
@@ -16,19 +18,22 @@ namespace attn {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kStages = 3;
+constexpr int kStages = 3;             // steps of a warp's ring
 constexpr int kKeys = 16;              // keys of a warp's step
 constexpr int kRows = 16;              // query heads of a CTA
+constexpr int kMaxSplits = 8;          // CTAs of a cluster; 16 of them start 2 us later
 
-template <int D>
+// A step of 16 keys takes a warp a microsecond, most of it latency, and eight warps' rings fill an SM: two CTAs
+// of four, or one of eight for few sequences, whose CTAs do not fill the SMs.
+template <int D, int kWarps>
 struct DecodeLayout {
   static constexpr int kPitch = D * 2 + 16;                        // bytes; keeps matrix loads off one another's banks
   static constexpr int kStageBytes = 2 * kKeys * kPitch;           // K, V
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kJoinBytes = kRows * D * 4 + 2 * kRows * 4; // output, maximum, sum of the CTA
   static constexpr int kBytes = kRingBytes + kJoinBytes;
-  static_assert(kWarps * (kRows * D * 4 + 2 * kRows * 4) <= kRingBytes, "the warps' results fit the ring");
+  static_assert(kWarps * (kRows * D * 4 + 2 * kRows * 4) <= kRingBytes && 2 * kMaxSplits * kRows * 4 <= kRingBytes,
+                "the warps' results, and later the parts' weights, fit the ring");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
@@ -54,17 +59,17 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 
 __device__ __forceinline__ float remote_float(const float* p, uint32_t rank) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_u32(p), rank)) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_u32(p), rank)));
   return v;
 }
 
 // Weight of a part whose maximum is m beside the joint one; parts without a key have m = -inf.
 __device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.f : exp2_approx(m - top); }
 
-template <typename T, int D>
+template <typename T, int D, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32)
 window_decode_kernel(const DecodeParams p) {
-  using L = DecodeLayout<D>;
+  using L = DecodeLayout<D, kWarps>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = gridDim.x, split = blockIdx.x;               // a cluster spans x
@@ -82,20 +87,36 @@ window_decode_kernel(const DecodeParams p) {
   const T* kbase = static_cast<const T*>(p.k) + b * p.k_batch + kv_head * p.k_head;
   const T* vbase = static_cast<const T*>(p.v) + b * p.v_batch + kv_head * p.v_head;
   uint8_t* ring = smem + warp * (kStages * L::kStageBytes);
-  constexpr int kChunks = D / 8;                                  // 16-byte pieces of a key
+  constexpr int kChunks = D / 8, kAbreast = 32 / kChunks;         // 16-byte pieces of a key; keys a warp copies at once
+  const int piece = lane % kChunks, key0 = lane / kChunks;
+  const bool inside = piece * 8 < p.dim;
+  // Where this lane's piece of visible key 0 would lie, if it were among the last keys.
+  const T* kwin = kbase + int64_t(lo - first) * p.k_row + (inside ? piece * 8 : 0);
+  const T* vwin = vbase + int64_t(lo - first) * p.v_row + (inside ? piece * 8 : 0);
   auto load = [&](int step) {
     if (step < end) {
-      uint8_t* stage = ring + (step - begin) % kStages * L::kStageBytes;
       const int base = (step * kWarps + warp) * kKeys;
+      const uint32_t dst = smem_u32(ring + (step - begin) % kStages * L::kStageBytes) + key0 * L::kPitch + piece * 16;
+      if (base >= first && base + kKeys <= visible) {             // 16 keys in a row, but for few steps
+        const T* ks = kwin + int64_t(base + key0) * p.k_row;
+        const T* vs = vwin + int64_t(base + key0) * p.v_row;
+        const int bytes = inside ? 16 : 0;
 #pragma unroll
-      for (int x = lane; x < kKeys * kChunks; x += 32) {
-        const int key = x / kChunks, c = x % kChunks, at = base + key;
-        const bool there = at < visible && c * 8 < p.dim;
-        const int64_t row = there ? (at < first ? at : lo + at - first) : 0;
-        const uint32_t dst = smem_u32(stage) + key * L::kPitch + c * 16;
-        const int bytes = there ? 16 : 0;                         // else zeros, and nothing is read
-        copy16(dst, kbase + row * p.k_row + (there ? c * 8 : 0), bytes);
-        copy16(dst + kKeys * L::kPitch, vbase + row * p.v_row + (there ? c * 8 : 0), bytes);
+        for (int i = 0; i < kKeys / kAbreast; ++i) {
+          copy16(dst + i * kAbreast * L::kPitch, ks, bytes);
+          copy16(dst + (kKeys + i * kAbreast) * L::kPitch, vs, bytes);
+          ks += kAbreast * p.k_row;
+          vs += kAbreast * p.v_row;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kKeys / kAbreast; ++i) {
+          const int at = base + key0 + i * kAbreast;
+          const bool there = at < visible && inside;
+          const int64_t row = there ? at + (at < first ? first - lo : 0) : first - lo;       // else zeros, nothing is read
+          copy16(dst + i * kAbreast * L::kPitch, kwin + row * p.k_row, there ? 16 : 0);
+          copy16(dst + (kKeys + i * kAbreast) * L::kPitch, vwin + row * p.v_row, there ? 16 : 0);
+        }
       }
     }
     copy_commit();
@@ -223,57 +244,82 @@ window_decode_kernel(const DecodeParams p) {
     if (d == 0) { joint_m[r] = top; joint_sum[r] = total; }
   }
   cluster_sync_all();
+  // Every CTA reads all parts' maxima and sums at once (a remote read takes as long as a few keys), then its share
+  // of the outputs.
+  float* weight = reinterpret_cast<float*>(smem);                  // [split][rows]; the warps' parts have been read
+  float* sums = weight + kMaxSplits * kRows;
+  for (int x = threadIdx.x; x < splits * rows; x += kWarps * 32) {
+    const int s = x / rows, r = x % rows;
+    weight[s * kRows + r] = remote_float(joint_m + r, s);
+    sums[s * kRows + r] = remote_float(joint_sum + r, s);
+  }
+  __syncthreads();
+  if (int(threadIdx.x) < rows) {
+    const int r = threadIdx.x;
+    float top = -INFINITY, total = 0.f;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, weight[s * kRows + r]);
+    for (int s = 0; s < splits; ++s) total += join_weight(weight[s * kRows + r], top) * sums[s * kRows + r];
+    const float inv = total == 0.f ? 0.f : 1.f / total;            // an idle slot: zeros
+    for (int s = 0; s < splits; ++s) weight[s * kRows + r] = join_weight(weight[s * kRows + r], top) * inv;
+  }
+  __syncthreads();
   T* out = static_cast<T*>(p.out) + (int64_t(b) * p.heads + head0) * p.dim;
   for (int x = split * (kWarps * 32) + threadIdx.x; x < rows * D; x += splits * (kWarps * 32)) {
     const int r = x / D, d = x % D;
     if (d >= p.dim) continue;
-    float top = -INFINITY, total = 0.f, value = 0.f;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, remote_float(joint_m + r, s));
-    for (int s = 0; s < splits; ++s) {
-      const float weight = join_weight(remote_float(joint_m + r, s), top);
-      total += weight * remote_float(joint_sum + r, s);
-      value += weight * remote_float(joint + x, s);
-    }
-    out[r * p.dim + d] = from_float<T>(total == 0.f ? 0.f : value / total);       // an idle slot: zeros
+    float value = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) value = fmaf(weight[s * kRows + r], remote_float(joint + x, s), value);
+    out[r * p.dim + d] = from_float<T>(value);
   }
   cluster_sync_all();                  // no CTA leaves while another reads its shared memory
 }
 
-template <typename T, int D>
-cudaError_t launch_decode(const DecodeParams& p, int sms, cudaStream_t stream) {
-  auto kernel = window_decode_kernel<T, D>;
-  cudaError_t rc = allow_shared(kernel, DecodeLayout<D>::kBytes);
+template <typename T, int D, int kWarps>
+cudaError_t launch_decode(const DecodeParams& p, dim3 grid, cudaStream_t stream) {
+  auto kernel = window_decode_kernel<T, D, kWarps>;
+  constexpr int bytes = DecodeLayout<D, kWarps>::kBytes;
+  static std::atomic<bool> allowed[64];
+  const cudaError_t rc = allow_shared(kernel, bytes, allowed);
   if (rc != cudaSuccess) return rc;
-  const int ratio = p.heads / p.kv_heads, blocks = (ratio + kRows - 1) / kRows;
-  const int64_t units = int64_t(p.batch) * p.kv_heads * blocks;
-  // Two CTAs fit an SM.  Few sequences are split until every SM has its two; many until there are several
-  // waves to even out ragged lengths, as long as a CTA keeps 1024 keys.
-  const int64_t keys = int64_t(p.window < p.capacity ? p.window : p.capacity) + p.sinks;
-  int splits = 1;
-  while (splits < 8 && keys > splits * kWarps * kKeys &&
-         (units * splits < 2 * sms || (units * splits < 8 * sms && keys > splits * 1024)))
-    splits *= 2;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(splits, p.kv_heads * blocks, p.batch);
+  config.gridDim = grid;
   config.blockDim = dim3(kWarps * 32);
-  config.dynamicSmemBytes = DecodeLayout<D>::kBytes;
+  config.dynamicSmemBytes = bytes;
   config.stream = stream;
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = splits;
+  cluster.val.clusterDim.x = grid.x;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
   config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, kernel, p);
 }
 
+template <typename T>
+cudaError_t launch_decode(const DecodeParams& p, int sms, cudaStream_t stream) {
+  const int ratio = p.heads / p.kv_heads, blocks = (ratio + kRows - 1) / kRows;
+  const int64_t units = int64_t(p.batch) * p.kv_heads * blocks;
+  // The split that ends first: waves of CTAs, each as long as its keys and a start and end that take about as
+  // long as 192 keys; no CTA with less than a step of four warps.
+  const int64_t keys = int64_t(p.window < p.capacity ? p.window : p.capacity) + p.sinks;
+  int splits = 1;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= kMaxSplits && (s == 1 || keys > (s / 2) * 4 * kKeys); s *= 2) {
+    const int64_t cost = (units * s + 2 * sms - 1) / (2 * sms) * (keys / s + 192);
+    if (cost < best) { best = cost; splits = s; }
+  }
+  const dim3 grid(splits, p.kv_heads * blocks, p.batch);
+  const bool few = units * splits <= sms && keys > splits * 4 * kKeys;
+  if (p.dim <= 64) return few ? launch_decode<T, 64, 8>(p, grid, stream) : launch_decode<T, 64, 4>(p, grid, stream);
+  return few ? launch_decode<T, 128, 8>(p, grid, stream) : launch_decode<T, 128, 4>(p, grid, stream);
+}
+
 }  // namespace
 
 cudaError_t decode(bool bf16, const DecodeParams& p, int sms, cudaStream_t stream) {
   if (p.batch == 0) return cudaSuccess;
-  if (p.dim <= 64)
-    return bf16 ? launch_decode<__nv_bfloat16, 64>(p, sms, stream) : launch_decode<__half, 64>(p, sms, stream);
-  return bf16 ? launch_decode<__nv_bfloat16, 128>(p, sms, stream) : launch_decode<__half, 128>(p, sms, stream);
+  return bf16 ? launch_decode<__nv_bfloat16>(p, sms, stream) : launch_decode<__half>(p, sms, stream);
 }
 
 }  // namespace attn
