@@ -136,10 +136,13 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
     dv = at::empty({p.batch, p.seq, p.kv_heads, p.dim}, q.options());
     if (p.sinks > 0) {
       // Every query sees the first tokens: their tile's stream is as long as the sequence, the others' a
-      // window.  What exceeds that is split into parts of a window's length.
+      // window.  It starts first; where it would still end last, what exceeds a window is split into parts of a
+      // window's length (and at least 1024 rows).  An SM runs one CTA of large heads, two of small ones.
       const int usual = (p.window + attn::kTile + rows - 1) / rows;
       const int far_tiles = std::max(0, (p.seq + rows - 1) / rows - usual);
-      if (far_tiles > usual / 2) {
+      const int64_t streams = int64_t(p.batch) * p.kv_heads * ((p.seq + attn::kTile - 1) / attn::kTile);
+      const int64_t share = streams * usual / (int64_t(sm_count()) * (p.dim > 64 ? 1 : 2));
+      if (far_tiles > 0 && usual + far_tiles > std::max<int64_t>(usual + usual / 2, share * 3 / 4)) {
         p.far_tiles = std::max({usual, 1024 / rows, (far_tiles + 63) / 64});
         p.far_splits = (far_tiles + p.far_tiles - 1) / p.far_tiles;
         far = at::empty({p.far_splits + 1, p.batch, p.kv_heads, 2, p.sinks, p.dim}, lse.options());

@@ -447,26 +447,29 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
 }
 
 // delta_i = dO_i O_i with O as it was before its rounding (P (dP - delta) cancels where few keys are visible:
-// with the rounded O the gradients of q and k were off by half as much again), 16 lanes a row of one head; zero behind a sequence's end, whatever lies there.
-template <typename T>
+// with the rounded O the gradients of q and k were off by half as much again), LANES lanes of 16 bytes a row of one
+// head; zero behind a sequence's end, whatever lies there.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
 row_sums_kernel(const T* __restrict__ out, const T* __restrict__ low, const T* __restrict__ dout,
                 const Params p) {
-  const int lane = threadIdx.x & 15, h = blockIdx.y, b = blockIdx.z;
-  const int i = blockIdx.x * 16 + (threadIdx.x >> 4);
+  // Rows in the order of memory: all heads of a token, then the next token.
+  const int lane = threadIdx.x % LANES, b = blockIdx.y;
+  const int64_t n = int64_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  const int i = int(n / p.heads), h = int(n - int64_t(i) * p.heads);
   float sum = 0.f;
   if (i < length_of(p, b) && lane * 8 < p.dim) {
-    const int64_t at = ((int64_t(b) * p.seq + i) * p.heads + h) * p.dim + lane * 8;
+    const int64_t at = (int64_t(b) * p.seq * p.heads + n) * p.dim + lane * 8;
     const uint4 x = *reinterpret_cast<const uint4*>(out + at), y = *reinterpret_cast<const uint4*>(dout + at);
     const uint4 z = *reinterpret_cast<const uint4*>(low + at);
-    const T* zs = reinterpret_cast<const T*>(&z);
     const T* xs = reinterpret_cast<const T*>(&x);
     const T* ys = reinterpret_cast<const T*>(&y);
+    const T* zs = reinterpret_cast<const T*>(&z);
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum = fmaf(to_float(xs[k]) + to_float(zs[k]), to_float(ys[k]), sum);
   }
 #pragma unroll
-  for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  for (int d = LANES / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) p.neg_delta[(int64_t(b) * p.heads + h) * p.seq_pad + i] = -sum;
 }
 
@@ -519,14 +522,19 @@ cudaError_t backward(bool bf16, const CUtensorMap& x0, const CUtensorMap& x1, co
 }  // namespace
 
 cudaError_t row_sums(bool bf16, const void* out, const void* dout, const Params& p, cudaStream_t stream) {
-  const dim3 grid(p.seq_pad / 16, p.heads, p.batch);
-  auto launch = [&](auto* x) {
+  auto launch = [&](auto* x, auto lanes) {
     using T = std::remove_pointer_t<decltype(x)>;
-    row_sums_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(out), static_cast<const T*>(p.out_low),
-                                                 static_cast<const T*>(dout), p);
+    constexpr int kLanes = decltype(lanes)::value;
+    const dim3 grid(p.seq_pad / (256 / kLanes) * p.heads, p.batch);              // seq_pad is a multiple of 256
+    row_sums_kernel<T, kLanes><<<grid, 256, 0, stream>>>(static_cast<const T*>(out), static_cast<const T*>(p.out_low),
+                                                         static_cast<const T*>(dout), p);
   };
-  if (bf16) launch(static_cast<__nv_bfloat16*>(nullptr));
-  else launch(static_cast<__half*>(nullptr));
+  auto typed = [&](auto* x) {
+    if (p.dim <= 64) launch(x, std::integral_constant<int, 8>{});
+    else launch(x, std::integral_constant<int, 16>{});
+  };
+  if (bf16) typed(static_cast<__nv_bfloat16*>(nullptr));
+  else typed(static_cast<__half*>(nullptr));
   return cudaGetLastError();
 }
 
