@@ -143,6 +143,7 @@ struct Params {
   float* neg_delta;
   void* out_low;                       // nullable: what the rounding of `out` left, [batch, seq, heads, dim]
   int seq_pad;
+  bool split;                          // backward pass: P and dS as two 16-bit numbers each
   // Backward pass over the keys: queries a window away from the first tokens are split into `far_splits`
   // parts of `far_tiles` tiles, whose shares of the first tokens' gradients are summed afterwards.
   int far_splits, far_tiles;

@@ -53,15 +53,22 @@ struct Seen {
   __device__ __forceinline__ bool at(int k) const { return half[k >> 5] >> (k & 31) & 1u; }
 };
 
+// What the rounding of a pair left, as a pair.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_rest(float2 v, uint32_t rounded) {
+  const T* r = reinterpret_cast<const T*>(&rounded);
+  return pack2<T>(v.x - to_float(r[0]), v.y - to_float(r[1]));
+}
+
 // Exponentials of a row's 64 scores; in the keys' kernel also rounded over the scores.  The statistics are the
 // columns' in the keys' kernel (in shared memory), the row's in the queries'.
-template <typename T, bool KEYS, bool EDGE>
+template <typename T, bool KEYS, bool EDGE, bool SPLIT>
 __device__ __forceinline__ void row_exp(const uint32_t (&s)[64], uint32_t ts, float scale, const float* col, float row,
                                         const Seen& seen, float2 (&pr)[32]) {
   const float2 scale2 = splat2(scale);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t packed[16];
+    uint32_t packed[16], rest[16];
 #pragma unroll
     for (int x = 0; x < 16; x += 2) {
       float2 l[2] = {splat2(row), splat2(row)};
@@ -79,14 +86,16 @@ __device__ __forceinline__ void row_exp(const uint32_t (&s)[64], uint32_t ts, fl
         }
         pr[c * 16 + x + u] = e;
         if constexpr (KEYS) packed[x + u] = pack2<T>(e.x, e.y);
+        if constexpr (KEYS && SPLIT) rest[x + u] = pack_rest<T>(e, packed[x + u]);
       }
     }
     if constexpr (KEYS) tmem_st_32x16(ts + c * 16, packed);
+    if constexpr (KEYS && SPLIT) tmem_st_32x16(ts + 32 + c * 16, rest);
   }
 }
 
 // dS over the other product.  P = 0 does not do for hidden pairs, whose product may be infinite or NaN.
-template <typename T, bool KEYS, bool EDGE>
+template <typename T, bool KEYS, bool EDGE, bool SPLIT>
 __device__ __forceinline__ void row_ds(uint32_t td, const float* col, float row, const Seen& seen,
                                        const float2 (&pr)[32]) {
   uint32_t d[64];
@@ -95,7 +104,7 @@ __device__ __forceinline__ void row_ds(uint32_t td, const float* col, float row,
   tmem_ld_wait();
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t packed[16];
+    uint32_t packed[16], rest[16];
 #pragma unroll
     for (int x = 0; x < 16; x += 2) {
       float2 l[2] = {splat2(row), splat2(row)};
@@ -112,13 +121,15 @@ __device__ __forceinline__ void row_ds(uint32_t td, const float* col, float row,
           if (!seen.at(k + 1)) ds.y = 0.f;
         }
         packed[x + u] = pack2<T>(ds.x, ds.y);
+        if constexpr (SPLIT) rest[x + u] = pack_rest<T>(ds, packed[x + u]);
       }
     }
     tmem_st_32x16(td + c * 16, packed);
+    if constexpr (SPLIT) tmem_st_32x16(td + 32 + c * 16, rest);
   }
 }
 
-template <typename T, int D, bool KEYS>
+template <typename T, int D, bool KEYS, bool SPLIT>
 __global__ void __launch_bounds__(Layout<D>::kThreads, Layout<D>::kResident)
 window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_constant__ CUtensorMap map_x1,
                   const __grid_constant__ CUtensorMap map_y0, const __grid_constant__ CUtensorMap map_y1,
@@ -294,6 +305,10 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
 #pragma unroll
           for (int i = 0; i < R / 16; ++i)
             umma_f16_ta(ta, ts + at(i), desc_along_rows<R>(y1, i), idesc_a, t > 0 || i != 0);
+          if constexpr (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < R / 16; ++i) umma_f16_ta(ta, ts + 32 + at(i), desc_along_rows<R>(y1, i), idesc_a, 1);
+          }
         }
         __syncwarp();
       }
@@ -303,6 +318,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
 #pragma unroll
         for (int i = 0; i < R / 16; ++i)
           umma_f16_ta(ta + (KEYS ? D : 0), td + at(i), desc_along_rows<R>(y0, i), idesc_a, t > 0 || i != 0);
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int i = 0; i < R / 16; ++i)
+            umma_f16_ta(ta + (KEYS ? D : 0), td + 32 + at(i), desc_along_rows<R>(y0, i), idesc_a, 1);
+        }
         umma_commit(bar_of(&empty[stage]));
         if (!more) umma_commit(bar_of(acc_full));
       }
@@ -359,8 +379,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(p_done));
         }
-        if (edge) row_exp<T, KEYS, true>(s, ts, scale, col, row_lse, seen, pr);
-        else row_exp<T, KEYS, false>(s, ts, scale, col, row_lse, seen, pr);
+        if (edge) row_exp<T, KEYS, true, SPLIT>(s, ts, scale, col, row_lse, seen, pr);
+        else row_exp<T, KEYS, false, SPLIT>(s, ts, scale, col, row_lse, seen, pr);
       }
       if constexpr (KEYS) {
         tmem_st_wait();
@@ -372,8 +392,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
-      if (edge) row_ds<T, KEYS, true>(td, col + R, row_delta, seen, pr);
-      else row_ds<T, KEYS, false>(td, col + R, row_delta, seen, pr);
+      if (edge) row_ds<T, KEYS, true, SPLIT>(td, col + R, row_delta, seen, pr);
+      else row_ds<T, KEYS, false, SPLIT>(td, col + R, row_delta, seen, pr);
       tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
@@ -495,10 +515,10 @@ sum_far_kernel(T* __restrict__ dk, T* __restrict__ dv, const Params p) {
   out[((int64_t(b) * p.seq + row) * p.kv_heads + h) * p.dim + d] = from_float<T>(sum);
 }
 
-template <typename T, int D, bool KEYS>
+template <typename T, int D, bool KEYS, bool SPLIT>
 cudaError_t launch_backward(const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& y0, const CUtensorMap& y1,
                             const CUtensorMap& o0, const CUtensorMap& o1, const Params& p, cudaStream_t stream) {
-  auto kernel = window_bwd_kernel<T, D, KEYS>;
+  auto kernel = window_bwd_kernel<T, D, KEYS, SPLIT>;
   static std::atomic<bool> allowed[64];
   const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes, allowed);
   if (rc != cudaSuccess) return rc;
@@ -512,11 +532,15 @@ template <bool KEYS>
 cudaError_t backward(bool bf16, const CUtensorMap& x0, const CUtensorMap& x1, const CUtensorMap& y0,
                      const CUtensorMap& y1, const CUtensorMap& o0, const CUtensorMap& o1, const Params& p,
                      cudaStream_t stream) {
-  if (p.dim <= 64)
-    return bf16 ? launch_backward<__nv_bfloat16, 64, KEYS>(x0, x1, y0, y1, o0, o1, p, stream)
-                : launch_backward<__half, 64, KEYS>(x0, x1, y0, y1, o0, o1, p, stream);
-  return bf16 ? launch_backward<__nv_bfloat16, 128, KEYS>(x0, x1, y0, y1, o0, o1, p, stream)
-              : launch_backward<__half, 128, KEYS>(x0, x1, y0, y1, o0, o1, p, stream);
+  auto typed = [&](auto* x) {
+    using T = std::remove_pointer_t<decltype(x)>;
+    if (p.dim <= 64)
+      return p.split ? launch_backward<T, 64, KEYS, true>(x0, x1, y0, y1, o0, o1, p, stream)
+                     : launch_backward<T, 64, KEYS, false>(x0, x1, y0, y1, o0, o1, p, stream);
+    return p.split ? launch_backward<T, 128, KEYS, true>(x0, x1, y0, y1, o0, o1, p, stream)
+                   : launch_backward<T, 128, KEYS, false>(x0, x1, y0, y1, o0, o1, p, stream);
+  };
+  return bf16 ? typed(static_cast<__nv_bfloat16*>(nullptr)) : typed(static_cast<__half*>(nullptr));
 }
 
 }  // namespace
