@@ -337,6 +337,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t ts = tmem + lanes + half * 64, td = tmem_d + lanes + half * 64;
     const float scale = p.scale * kLog2e;
+    const bool one_key = p.window == 1 && p.sinks == 0;           // for every query
     float row_lse = 0.f, row_delta = 0.f;
     if constexpr (!KEYS) {
       const int64_t at = (int64_t(b) * p.heads + own_head) * p.seq_pad + mine;
@@ -362,7 +363,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
         keep = p.sinks - y_row;
         edge = y_tile + R - 1 > x_row || (x_row + kTile - 1) - y_tile >= p.window;
       }
-      const Seen seen{{seen_bits(from, to, keep), seen_bits(from - 32, to - 32, keep - 32)}};
+      Seen seen{{seen_bits(from, to, keep), seen_bits(from - 32, to - 32, keep - 32)}};
       const float* col = stats + stage * 2 * R + half * 64;
       ok = mbar_wait(smem_u32(s_full), t & 1, abort_flag, p.status, kErrRows, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
@@ -392,6 +393,10 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
+      // A query that sees one key has P = 1 and dS = 0 whatever the inputs are; computed, dP - delta would be what
+      // its two orders of summation leave.  Such queries lie in edge tiles.
+      if (one_key || (!KEYS && mine == 0)) seen.half[0] = seen.half[1] = 0u;
+      else if (KEYS && y_row == 0) seen.half[0] &= ~1u;
       if (edge) row_ds<T, KEYS, true, SPLIT>(td, col + R, row_delta, seen, pr);
       else row_ds<T, KEYS, false, SPLIT>(td, col + R, row_delta, seen, pr);
       tmem_st_wait();
