@@ -389,7 +389,8 @@ class Trainer:
 
         ``teacher`` (a :class:`megablocks_b200.models.transformer.Teacher` for the batch): the model is
         distilled from its logits instead, and the loss returned is that of ``model.distillation_loss``;
-        such a step runs kernel by kernel.
+        such a step runs kernel by kernel, and a recorded step is forgotten (it keeps the place in the schedule on
+        the device).
 
         ``tokens`` / ``targets`` hold this rank's whole share of the step: ``grad_accum_steps``
         micro-batches stacked along dimension 0.  Returns the language-model loss as a device
@@ -399,7 +400,12 @@ class Trainer:
         one records the step in a CUDA graph, and every call from then on copies the batch into the
         graph's input buffers and replays it.
         """
-        loss = self._step_eager(tokens, targets, teacher=teacher) if teacher is not None else self._step(tokens, targets)
+        if teacher is None:
+            loss = self._step(tokens, targets)
+        else:
+            if self._graph is not None:
+                self.drop_graph()
+            loss = self._step_eager(tokens, targets, teacher=teacher)
         if self.cfg.router_bias_rate:        # outside the recorded step: the loads are summed over the ranks
             from megablocks_b200.layers.router import balance_routers
             balance_routers(self._routers, self.cfg.router_bias_rate, self.dp_group if self.world > 1 else None)
