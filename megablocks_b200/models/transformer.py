@@ -17,6 +17,7 @@ Beside training (``loss``, ``distillation_loss``) a model answers: ``prefill`` f
 batch of prompts, ``decode`` takes one token per sequence further, ``generate`` does both greedily.
 """
 
+import contextlib
 import dataclasses
 import math
 from functools import partial
@@ -427,10 +428,27 @@ class MoETransformer(nn.Module):
                    for _ in range(2)]
         return KVCache(*buffers, torch.zeros(batch, dtype=torch.int32, device=weight.device))
 
-    @torch.no_grad()
+    @contextlib.contextmanager
+    def _answering(self):
+        """Without gradients and, whatever mode the model is in, without what only training does: the layers'
+        loss accumulators and load counts, jitter."""
+        training = [m for m in self.modules() if m.training] if self.training else []
+        for m in training:
+            m.training = False
+        try:
+            with torch.no_grad():
+                yield
+        finally:
+            for m in training:
+                m.training = True
+
     def prefill(self, tokens: torch.Tensor, cache: KVCache, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Fill the cache from prompts ``tokens[batch, seq]`` (``lengths[batch]`` valid tokens each, at least one;
         ``None``: all); returns the logits ``[batch, vocab]`` behind each prompt's last token."""
+        with self._answering():
+            return self._prefill(tokens, cache, lengths)
+
+    def _prefill(self, tokens, cache, lengths):
         b, s = tokens.shape
         if b != cache.lengths.shape[0] or not 1 <= s <= cache.capacity:
             raise ValueError(f'prompts of {s} tokens for {b} sequences do not fit a cache of {cache.capacity} tokens '
@@ -452,17 +470,24 @@ class MoETransformer(nn.Module):
         last = (cache.lengths - 1).long()
         return self.logits(hidden[torch.arange(b, device=tokens.device), last])
 
-    @torch.no_grad()
     def decode(self, tokens: torch.Tensor, cache: KVCache) -> torch.Tensor:
         """Take every sequence one token further: ``tokens[batch]`` go to the end of the cache; returns the logits
-        ``[batch, vocab]`` behind them."""
+        ``[batch, vocab]`` behind them.
+
+        A recorded call may be replayed: lengths advance on the device, and a token for which a sequence has no
+        room takes the place of its last one."""
+        with self._answering():
+            return self._decode(tokens, cache)
+
+    def _decode(self, tokens, cache):
         if tokens.shape != cache.lengths.shape:
             raise ValueError('decode takes one token per sequence of the cache')
         if not 1 <= cache.used < cache.capacity:
             raise ValueError(f'the cache holds {cache.used} of {cache.capacity} tokens: it has to be filled first and '
                              'have room for one more')
-        at = cache.lengths.long()
-        cache.lengths += 1
+        # `used` says nothing of replays of a recorded call, which must not write behind the cache.
+        at = cache.lengths.long().clamp_(0, cache.capacity - 1)
+        torch.add(at, 1, out=cache.lengths)
         cache.used += 1
         rope = self._rope_for(cache.capacity, tokens.device)
         if rope is not None:
@@ -477,7 +502,6 @@ class MoETransformer(nn.Module):
         x, delta, delta_bias = self._run_blocks(x.unsqueeze(0), attend)
         return self.logits(_add_norm(self.ln_f, x, delta, delta_bias)[1].squeeze(0))
 
-    @torch.no_grad()
     def generate(self, tokens: torch.Tensor, steps: int, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``steps`` most likely tokens behind each prompt: ``[batch, steps]``."""
         if steps < 1:
