@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "kernels.h"
@@ -51,11 +52,16 @@ attn::Params make_params(const at::Tensor& q, const at::Tensor& k, int64_t windo
                          const OptTensor& lengths, double scale) {
   TORCH_CHECK(in_place(q) && in_place(k), "window_attention expects 16-bit CUDA tensors [batch, seq, heads, dim] with "
               "aligned rows");
-  TORCH_CHECK(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3) && k.size(2) >= 1 &&
-                  q.size(2) % k.size(2) == 0 && q.size(1) >= 1 && q.size(1) < (int64_t(1) << 22) &&
-                  q.size(0) * q.size(2) < (int64_t(1) << 16) && q.size(0) >= 1 && q.size(2) >= 1,
-              "window_attention: sizes do not match or are too large");
-  TORCH_CHECK(window >= 1 && sinks >= 0 && scale > 0, "window_attention: bad window, sinks or scale");
+  TORCH_CHECK_VALUE(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3) && k.size(2) >= 1 &&
+                        q.size(2) % k.size(2) == 0 && q.size(0) >= 1 && q.size(1) >= 1 && q.size(2) >= 1,
+                    "window_attention: sizes do not match");
+  // Tiles, heads and sequences are the dimensions of a grid (65535 of the last two; heads and sequences share one
+  // in the backward pass), rows and heads numbers of 32 bits.
+  TORCH_CHECK_VALUE(q.size(0) < (int64_t(1) << 16) && q.size(1) < (int64_t(1) << 22) && q.size(2) < (int64_t(1) << 16) &&
+                        q.size(0) * q.size(2) < (int64_t(1) << 31),
+                    "window_attention takes fewer than 65536 sequences and heads and 4194304 tokens");
+  TORCH_CHECK_VALUE(window >= 1 && sinks >= 0 && float(scale) > 0 && std::isfinite(float(scale)),
+                    "window_attention: bad window, sinks or scale");
   if (lengths.has_value())
     TORCH_CHECK(lengths->device() == q.device() && lengths->is_contiguous() && lengths->scalar_type() == at::kInt &&
                     lengths->dim() == 1 && lengths->size(0) == q.size(0),
@@ -142,12 +148,13 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
     if (p.sinks > 0) {
       // Every query sees the first tokens: their tile's stream is as long as the sequence, the others' a
       // window.  It starts first; where it would still end last, what exceeds a window is split into parts of a
-      // window's length (and at least 1024 rows).  An SM runs one CTA of large heads, two of small ones.
+      // window's length (and at least 1024 rows).  An SM runs one CTA of large heads, two of small ones.  More
+      // first tokens than a tile make long streams enough to fill the SMs, and the parts' workspace grows with them.
       const int usual = (p.window + attn::kTile + rows - 1) / rows;
       const int far_tiles = std::max(0, (p.seq + rows - 1) / rows - usual);
       const int64_t streams = int64_t(p.batch) * p.kv_heads * ((p.seq + attn::kTile - 1) / attn::kTile);
       const int64_t share = streams * usual / (int64_t(sm_count()) * (p.dim > 64 ? 1 : 2));
-      if (far_tiles > 0 && usual + far_tiles > std::max<int64_t>(usual + usual / 2, share * 3 / 4)) {
+      if (p.sinks <= attn::kTile && far_tiles > 0 && usual + far_tiles > std::max<int64_t>(usual + usual / 2, share * 3 / 4)) {
         p.far_tiles = std::max({usual, 1024 / rows, (far_tiles + 63) / 64});
         p.far_splits = (far_tiles + p.far_tiles - 1) / p.far_tiles;
         far = at::empty({p.far_splits + 1, p.batch, p.kv_heads, 2, p.sinks, p.dim}, lse.options());
@@ -197,12 +204,13 @@ struct Window : torch::autograd::Function<Window> {
     out[0] = g[0];
     if (need_k) out[1] = g[1];
     if (need_v) out[2] = g[2];
-    return out;
+    return once_differentiable(out, "window_attention");
   }
 };
 
-OptTensor int32(const OptTensor& t) {
-  return t.has_value() ? OptTensor(t->to(at::kInt).contiguous()) : OptTensor();
+// 64-bit lengths are clamped before they lose their upper half.
+at::Tensor int32(const at::Tensor& t, int64_t most) {
+  return (t.scalar_type() == at::kInt ? t : t.clamp(0, most).to(at::kInt)).contiguous();
 }
 
 }  // namespace
@@ -213,14 +221,14 @@ at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::
                             int64_t sinks, const OptTensor& lengths, double scale) {
   auto ready = [](const at::Tensor& t) { return in_place(t) ? t : t.clone(at::MemoryFormat::Contiguous); };
   const at::Tensor qr = ready(q), kr = ready(k), vr = ready(v);
+  const OptTensor dense = lengths.has_value() ? OptTensor(int32(*lengths, q.size(1))) : OptTensor();
   if (at::GradMode::is_enabled() && (qr.requires_grad() || kr.requires_grad() || vr.requires_grad()))
-    return Window::apply(qr, kr, vr, window, sinks, int32(lengths), scale);
-  return window_forward(qr, kr, vr, window, sinks, int32(lengths), scale, false)[0];
+    return Window::apply(qr, kr, vr, window, sinks, dense, scale);
+  return window_forward(qr, kr, vr, window, sinks, dense, scale, false)[0];
 }
 
 at::Tensor window_attention_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                    const at::Tensor& lengths_in, int64_t window, int64_t sinks, double scale) {
-  const at::Tensor lengths = lengths_in.to(at::kInt).contiguous();
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.is_contiguous() && reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 == 0 &&
                   in_place(k) && in_place(v) && q.device() == k.device() && k.device() == v.device() &&
                   q.scalar_type() == k.scalar_type() && k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() &&
@@ -228,11 +236,12 @@ at::Tensor window_attention_decode(const at::Tensor& q, const at::Tensor& k, con
                   k.size(1) < (int64_t(1) << 30) && q.size(0) < (int64_t(1) << 16) && q.size(1) < (int64_t(1) << 16),
               "window_attention_decode expects 16-bit CUDA q[batch, heads, dim] and caches [batch, capacity, kv_heads, "
               "dim] with aligned rows");
-  TORCH_CHECK(lengths.device() == q.device() && lengths.is_contiguous() && lengths.scalar_type() == at::kInt &&
-                  lengths.dim() == 1 && lengths.size(0) == q.size(0),
-              "window_attention_decode: lengths must be int32 [batch]");
-  TORCH_CHECK(window >= 1 && sinks >= 0 && scale > 0, "window_attention_decode: bad window, sinks or scale");
+  TORCH_CHECK(lengths_in.device() == q.device() && lengths_in.dim() == 1 && lengths_in.size(0) == q.size(0),
+              "window_attention_decode: lengths must be [batch]");
+  TORCH_CHECK_VALUE(window >= 1 && sinks >= 0 && float(scale) > 0 && std::isfinite(float(scale)),
+                    "window_attention_decode: bad window, sinks or scale");
   c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor lengths = int32(lengths_in, k.size(1));
   at::Tensor out = at::empty_like(q);
   if (q.size(0) == 0) return out;
   attn::DecodeParams p{};

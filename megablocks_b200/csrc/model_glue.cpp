@@ -118,7 +118,7 @@ struct Select : torch::autograd::Function<Select> {
     const SelectArgs a = select_args(saved[0], saved[1].size(1), how[0] != 0, 1, 1, how[1],
                                      ctx->saved_data["scale"].toDouble());
     out[0] = select_backward(saved[0], a, saved[1], grads[0], grads[1]);
-    return out;
+    return once_differentiable(out, "select_experts");
   }
 };
 
@@ -226,7 +226,7 @@ struct Distill : torch::autograd::Function<Distill> {
       C10_CUDA_CHECK(scale_unless_one(float_code(out[0].scalar_type()), out[0].data_ptr(), out[0].numel(),
                                       scale.data_ptr<float>(), sm_count(), stream()));
       count_launches(1);
-      return out;
+      return once_differentiable(out, "distillation_loss");
     }
     const auto saved = ctx->get_saved_variables();
     const auto how = ctx->saved_data["how"].toDoubleVector();
@@ -238,7 +238,7 @@ struct Distill : torch::autograd::Function<Distill> {
     C10_CUDA_CHECK(distill_bwd(float_code(saved[0].scalar_type()), a, saved[4].data_ptr<float>(),
                                scale.data_ptr<float>(), out[0].data_ptr(), stream()));
     count_launches(1);
-    return out;
+    return once_differentiable(out, "distillation_loss");
   }
 };
 

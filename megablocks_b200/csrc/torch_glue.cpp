@@ -3,6 +3,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -578,7 +579,16 @@ at::Tensor& status_word(const at::Device& device) {
   // the teardown of the CUDA context.
   static auto* words = new std::vector<at::Tensor>(64);
   const int idx = device.index();
-  if (!(*words)[idx].defined()) (*words)[idx] = at::zeros({4}, at::TensorOptions().device(device).dtype(at::kInt));
+  if (!(*words)[idx].defined()) {
+    // On a stream of its own: were the first use inside a recording, zeroing it would be recorded, and repeated by
+    // every replay, instead of done.
+    c10::cuda::CUDAGuard guard(device);
+    c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    const auto side = c10::cuda::getStreamFromPool(false, idx);
+    c10::cuda::CUDAStreamGuard on_side(side);
+    (*words)[idx] = at::zeros({4}, at::TensorOptions().device(device).dtype(at::kInt));
+    side.synchronize();
+  }
   return (*words)[idx];
 }
 

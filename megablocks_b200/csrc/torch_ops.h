@@ -3,8 +3,11 @@
 #pragma once
 
 #include <cuda.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <memory>
+#include <string>
 #include <vector>
 
 namespace mb {
@@ -30,6 +33,26 @@ at::Tensor binned_scatter_wgrad(const at::Tensor& x, const at::Tensor& grad, con
                                 const at::Tensor& bins, int64_t top_k);
 at::Tensor column_sum_op(const at::Tensor& x);
 // The device's status word, which kernels that give up a wait write, and the count of launched kernels.
+// Gradients of a pass that has no gradient itself: where one is asked for (create_graph), taking it is an error
+// rather than zero.
+inline torch::autograd::variable_list once_differentiable(torch::autograd::variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list inputs;
+  for (at::Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach().requires_grad_(true);
+    inputs.push_back(g);
+  }
+  if (inputs.empty()) return grads;
+  auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " is differentiable once: its gradient has none", int64_t(inputs.size()));
+  inputs = (*refuse)(std::move(inputs));
+  size_t i = 0;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = inputs[i++];
+  return grads;
+}
+
 int* device_status(const at::Device& device);
 void count_launches(int64_t n);
 // Tensor map of a 16-bit tensor (innermost dimension dense, `strides` in bytes of the others), 128-byte swizzle.

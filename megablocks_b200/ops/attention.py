@@ -54,7 +54,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
     ``lengths[batch]``: valid tokens of each sequence of a padded batch (clamped to ``[0, seq]``); rows behind
     them are zero, have no gradient, and are not looked at.  ``scale`` is by default ``dim ** -0.5``.  Any
-    strides; views of a fused projection with 16-byte aligned rows are read in place, others are copied."""
+    strides; views of a fused projection with 16-byte aligned rows are read in place, others are copied.  On CUDA
+    fewer than 65536 sequences and heads and 2^22 tokens, and differentiable once."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or q.shape[:2] != k.shape[:2]:
         raise ValueError('window_attention expects q[batch, seq, heads, dim] and k, v[batch, seq, kv_heads, dim]')
     scale = q.shape[-1]**-0.5 if scale is None else float(scale)

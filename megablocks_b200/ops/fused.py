@@ -30,6 +30,7 @@ from typing import Any
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from megablocks_b200._ext import ext
 
@@ -105,6 +106,7 @@ class _LinearDistillation(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx: Any, grad_out: torch.Tensor):
         hidden, weight, dlogits = ctx.saved_tensors
         scale = grad_out.detach().float()

@@ -272,3 +272,18 @@ def test_refusals(device):
     for change in bad:
         with pytest.raises(ValueError):
             fused.distillation_loss(**{**good, **change})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16])
+def test_differentiable_once(dtype):
+    logits = torch.randn(9, 300, device='cuda').to(dtype).requires_grad_(True)
+    values, ids = torch.randn(9, 4, device='cuda'), torch.randint(0, 300, (9, 4), device='cuda')
+    again, = torch.autograd.grad(fused.distillation_loss(logits, values, ids), logits, create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        again.sum().backward()
+    hidden = torch.randn(9, 64, device='cuda', requires_grad=True)
+    weight = torch.randn(300, 64, device='cuda')
+    again, = torch.autograd.grad(fused.linear_distillation_loss(hidden, weight, values, ids), hidden, create_graph=True)
+    with pytest.raises(RuntimeError):
+        again.sum().backward()

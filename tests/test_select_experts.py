@@ -311,3 +311,15 @@ def test_refusals(device):
                  (torch.randn(2, 64, device=device), 33), (torch.randn(2, 0, device=device), 1)):
         with pytest.raises(ValueError):
             ops.select_experts(x, k)
+
+
+@pytest.mark.gpu
+def test_differentiable_once():
+    logits = torch.randn(9, 16, device='cuda', requires_grad=True)
+    scores, weights, _ = ops.select_experts(logits, 3, score='sigmoid', norm_p=1)
+    loss = scores.square().sum() + weights.square().sum()
+    first, = torch.autograd.grad(loss, logits, retain_graph=True)
+    again, = torch.autograd.grad(loss, logits, create_graph=True)
+    assert torch.equal(first, again)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        again.sum().backward()

@@ -1,6 +1,9 @@
 """Windowed attention with first tokens that stay visible, against its definition in 64 bits."""
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -418,3 +421,72 @@ def test_refusals(device):
                      ((one[:, :3], k, v, lengths), {}), ((one.detach().requires_grad_(True), k, v, lengths), {})):
         with pytest.raises(ValueError):
             ops.window_attention_decode(*args, **kw)
+
+
+@pytest.mark.gpu
+def test_more_sequences_times_heads_than_a_grid_dimension():
+    """80000 short sequences of heads: as two halves."""
+    q, k, v = (t.requires_grad_(True) for t in inputs(5000, 3, 16, 8, 32, BF16, 'cuda', fused=False))
+    dout = torch.randn(q.shape, device='cuda').to(BF16)
+
+    def step(rows):
+        out = ops.window_attention(q[rows], k[rows], v[rows], 2, 1)
+        return [out, *(g[rows] for g in torch.autograd.grad(out, (q, k, v), dout[rows]))]
+
+    for whole, a, b in zip(step(slice(None)), step(slice(0, 2500)), step(slice(2500, None))):
+        assert torch.equal(whole, torch.cat([a, b]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(65536, 1, 1, 8), (1, 1 << 22, 1, 8), (1, 1, 65536, 8)])
+def test_sizes_that_are_refused(shape):
+    q = torch.zeros(shape, dtype=BF16, device='cuda')
+    with pytest.raises(ValueError):
+        ops.window_attention(q, q, q, 4)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_lengths_beyond_32_bits_are_clamped(device):
+    q, k, v = inputs(3, 20, 4, 2, 64, BF16, device, fused=False)
+    far = torch.tensor([1 << 40, -(1 << 40) + 5, (1 << 32) + 7], device=device)
+    near = torch.tensor([20, 0, 20], dtype=torch.int32, device=device)
+    assert torch.equal(ops.window_attention(q, k, v, 6, 1, far), ops.window_attention(q, k, v, 6, 1, near))
+    one = q[:, 0]
+    assert torch.equal(ops.window_attention_decode(one, k, v, far, 6), ops.window_attention_decode(one, k, v, near, 6))
+
+
+@pytest.mark.gpu
+def test_differentiable_once():
+    q, k, v = (t.requires_grad_(True) for t in inputs(1, 20, 4, 2, 64, BF16, 'cuda', fused=False))
+    out = ops.window_attention(q, k, v, 6, 1)
+    first = torch.autograd.grad(out.float().square().sum(), (q, k, v), retain_graph=True)
+    again = torch.autograd.grad(out.float().square().sum(), (q, k, v), create_graph=True)
+    for a, b in zip(first, again):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        again[0].float().sum().backward()
+
+
+_FIRST_IN_A_GRAPH = """
+import sys, torch
+sys.path.insert(0, {root!r})
+from megablocks_b200 import ops
+from megablocks_b200.utils.status import read as read_status
+q = torch.randn(1, 40, 2, 64, device='cuda').bfloat16()
+fill = torch.full((1 << 20,), -1, dtype=torch.int32, device='cuda')
+del fill
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = ops.window_attention(q, q, q, 8, 2)
+assert read_status(False) == 0
+graph.replay()
+assert torch.equal(out, ops.window_attention(q, q, q, 8, 2)) and read_status(False) == 0
+"""
+
+
+@pytest.mark.gpu
+def test_the_first_call_of_a_process_may_be_recorded():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, '-c', _FIRST_IN_A_GRAPH.format(root=root)], capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
