@@ -7,14 +7,19 @@
 //
 // One warp owns a token and holds its experts in registers, PL consecutive ones a lane, fetched V at a time.
 // A lane with up to eight sorts them once, as keys whose last three bits are the place, and a round of the
-// choice is one reduction of the lanes' heads; it is bound by instructions (1678 a token with the places
-// compared anew in every round: 80 us for 32768 x 256).  FULL: the experts fill all places of all lanes.
+// choice is one reduction of the lanes' heads (1678 instructions a token with the places compared anew in every
+// round).  FULL: the experts fill all places of all lanes.
 //
 // The order of the experts is exact: equal values go to the lowest id, and values that 32 bits cannot tell
 // apart are ordered by their 64-bit ones.  Without a bias the scores have the order of the logits, which are
 // compared as they are.  Each comparison that decides (neighbours in the chosen order, the last chosen one
-// and the next, the last group that stays and the next) is checked against a bound of the arithmetic's
-// error; a token with a closer pair, a few in a thousand, is chosen again from scores in 64 bits.
+// and the next, the last group that stays and the next) is checked against a bound of the arithmetic's error; in a
+// token with a closer pair, a few in a thousand, what is in question is ordered in 64 bits.  That path is kept
+// short, as the last token's latency is the launch's: with all of the choice redone a launch of 37 us ended 13 us
+// later for five tokens with close groups.
+//
+// 32768 x 256 bf16 in 8 groups, sigmoid and bias: 40 us (36 MB, 0.14 of the copy bandwidth), bound by
+// instructions, 874 a token at 3.1 a cycle and SM; backward 12 us at 0.6 of it.
 #include "common.cuh"
 
 namespace mb {
@@ -136,8 +141,9 @@ __device__ __forceinline__ float score_at(float x, const RowStat& r, bool use_si
 // ---- the choice in 64 bits: lane i returns the i-th expert ---------------------------------------------
 __device__ __forceinline__ double key64(double v) { return v != v ? INFINITY : v; }
 
+// What a choice goes by, in 64 bits, into c.
 template <typename T>
-__device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, double* c, int lane) {
+__device__ __forceinline__ void choice_wide(const T* row, const SelectArgs& a, double* c, int lane) {
   const int E = a.experts;
   double top = -INFINITY, sum = 0.;
   if (!a.use_sigmoid) {
@@ -145,6 +151,7 @@ __device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, doubl
     for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
     if (top == -INFINITY) top = 0.;
   }
+#pragma unroll 4
   for (int e = lane; e < E; e += 32) {
     const double x = to_float(row[e]);
     c[e] = a.use_sigmoid ? 1. / (1. + exp(-x)) : exp(x - top);
@@ -156,6 +163,39 @@ __device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, doubl
     c[e] = key64(a.bias != nullptr ? s + double(a.bias[e]) : s);
   }
   __syncwarp();
+}
+
+// The groups that stay, as choose_groups returns them.
+template <typename T>
+__device__ __noinline__ unsigned groups_wide(const T* row, const SelectArgs& a, double* c, int shift, int lane) {
+  choice_wide(row, a, c, lane);
+  const int g = lane >> shift, size = a.group_size;
+  double b1 = -INFINITY, b2 = -INFINITY;
+  if (g < a.groups) {
+    for (int i = lane & ((1 << shift) - 1); i < size; i += 1 << shift) {
+      const double v = c[g * size + i];
+      b2 = fmax(b2, fmin(b1, v));
+      b1 = fmax(b1, v);
+    }
+  }
+  for (int d = 1 << shift >> 1; d > 0; d >>= 1) {
+    const double o1 = __shfl_xor_sync(0xffffffffu, b1, d), o2 = __shfl_xor_sync(0xffffffffu, b2, d);
+    b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+    b1 = fmax(b1, o1);
+  }
+  const double value = size > 1 ? b1 + b2 : b1;
+  int rank = 0;
+  for (int h = 0; h < a.groups; ++h) {
+    const double o = __shfl_sync(0xffffffffu, value, h << shift);
+    rank += o > value || (o == value && h < g);
+  }
+  return __ballot_sync(0xffffffffu, g < a.groups && rank < a.top_groups);
+}
+
+template <typename T>
+__device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, double* c, int lane) {
+  const int E = a.experts;
+  choice_wide(row, a, c, lane);
   unsigned kept = 0xffffffffu;
   const int size = a.group_size;
   if (a.top_groups < a.groups) {
@@ -196,6 +236,38 @@ __device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, doubl
     if (lane == i) mine = at;
   }
   return mine;
+}
+
+// The order in 64 bits of the n experts that lanes hold, no others being in question: lane i returns the i-th.  Takes
+// a tenth of the time of the choice from all, which at the end of a launch every SM waits for.
+template <typename T>
+__device__ __noinline__ int order_wide(const T* row, const SelectArgs& a, float top, int mine, int n, int lane) {
+  double sum = 0.;
+  if (a.bias != nullptr && !a.use_sigmoid) {
+    for (int e = lane; e < a.experts; e += 32) sum += exp(double(to_float(row[e])) - double(top));
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  }
+  double c = -INFINITY;
+  if (lane < n) {
+    c = to_float(row[mine]);
+    if (a.bias != nullptr) {
+      if (a.use_sigmoid) c = 1. / (1. + exp(-c));
+      else c = sum == 0. ? 0. : exp(c - double(top)) / sum;
+      c += double(a.bias[mine]);
+    }
+    c = key64(c);
+  }
+  int rank = 0, sorted = 0;
+  for (int i = 0; i < n; ++i) {
+    const double o = __shfl_sync(0xffffffffu, c, i);
+    const int e = __shfl_sync(0xffffffffu, mine, i);
+    rank += o > c || (o == c && e < mine);
+  }
+  for (int i = 0; i < n; ++i) {
+    const int at = __shfl_sync(0xffffffffu, rank, i), e = __shfl_sync(0xffffffffu, mine, i);
+    if (at == lane) sorted = e;
+  }
+  return sorted;
 }
 
 __host__ __device__ constexpr int padded_slot(int e) { return e + (e >> 5) * 4; }
@@ -311,7 +383,8 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
         }
       }
       join_best(b1, b2, a.aligned_shift);
-      const unsigned stays = choose_groups(b1, b2, a.aligned_shift, a, lane, margin, doubt);
+      unsigned stays = choose_groups(b1, b2, a.aligned_shift, a, lane, margin, doubt);
+      if (doubt) stays = groups_wide<T>(row, a, shared + warp * E, a.aligned_shift, lane);
       if (!(stays >> (lane >> a.aligned_shift << a.aligned_shift) & 1u)) {
 #pragma unroll
         for (int j = 0; j < PL; ++j) key[j] = 0u;
@@ -327,7 +400,11 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
         }
       }
       join_best(b1, b2, shift);
-      const unsigned stays = choose_groups(b1, b2, shift, a, lane, margin, doubt);
+      unsigned stays = choose_groups(b1, b2, shift, a, lane, margin, doubt);
+      if (doubt) {
+        __syncwarp();                                     // the values in 32 bits have been read
+        stays = groups_wide<T>(row, a, shared + warp * E, shift, lane);
+      }
       const float inv_size = 1.f / float(a.group_size);
 #pragma unroll
       for (int j = 0; j < PL; ++j) {
@@ -343,9 +420,9 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
   // the next.
   const bool inexact = biased || (kSorted && sizeof(T) == 4);
   const int rounds = a.top_k + (inexact ? 1 : 0);
-  int mine = 0;                        // this lane's choice and its key; the key after all choices
-  unsigned mine_key = 0u, next_key = 0u;
-  for (int i = 0; i < rounds; ++i) {
+  int mine = 0;                        // lane i: the i-th choice and its key
+  unsigned mine_key = 0u, next_key = 0u;                  // the last key taken
+  auto take = [&](int i) {
     unsigned head;
     int at;
     if constexpr (kSorted) {
@@ -358,11 +435,11 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
       for (int j = 0; j < PL; ++j)
         if (key[j] > head) { head = key[j]; at = expert_of<PL>(j, lane); }
     }
-    const unsigned top = __reduce_max_sync(0xffffffffu, head);
-    const int from = __ffs(__ballot_sync(0xffffffffu, head == top)) - 1;      // the lowest lane has the lowest id
+    const unsigned best = __reduce_max_sync(0xffffffffu, head);
+    const int from = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;     // the lowest lane has the lowest id
     const int e = __shfl_sync(0xffffffffu, at, from);
-    if (lane == i && i < a.top_k) { mine = e; mine_key = top; }
-    next_key = top;
+    if (lane == i) { mine = e; mine_key = best; }
+    next_key = best;
     if (lane == from) {
       if constexpr (kSorted) {
 #pragma unroll
@@ -374,15 +451,18 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
           if (expert_of<PL>(j, lane) == e) key[j] = 0u;
       }
     }
-  }
+  };
+  for (int i = 0; i < rounds; ++i) take(i);
+  bool crowd = false;                                     // more than 31 experts come into question
   if (inexact) {                                          // all neighbours at once; a key of 0: no expert was left
+    auto close_keys = [&](unsigned k, unsigned next) {
+      if (!biased) return k == next;
+      const float c = from_ordered(k), d = from_ordered(next);
+      return !(c - d > margin + 0x1p-20f * fmaxf(fabsf(c), fabsf(d)));
+    };
     const bool last = lane == a.top_k - 1;
     const unsigned down = __shfl_down_sync(0xffffffffu, mine_key, 1), next = last ? next_key : down;
-    bool close = false;
-    if (lane < a.top_k && next != 0u) {
-      const float c = from_ordered(mine_key), d = from_ordered(next);
-      close = biased ? !(c - d > margin + 0x1p-20f * fmaxf(fabsf(c), fabsf(d))) : mine_key == next;
-    }
+    bool close = lane < a.top_k && next != 0u && close_keys(mine_key, next);
     if (__any_sync(0xffffffffu, close)) {
       // Experts that are alike in logit and bias are equal.  Not so behind the last choice, where others that are
       // as close may follow.
@@ -390,10 +470,18 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
       if (close && !last)
         close = !(ordered(to_float(row[mine])) == ordered(to_float(row[other])) &&
                   (!biased || a.bias[mine] == a.bias[other]));
-      if (__any_sync(0xffffffffu, close)) doubt = true;
+      if (__any_sync(0xffffffffu, close)) {
+        // Those behind the last choice that are as close to it come into question too; others do not, as they
+        // are further from all choices.
+        const unsigned end = __shfl_sync(0xffffffffu, mine_key, a.top_k - 1);
+        int n = a.top_k;
+        while (n < 32 && next_key != 0u && close_keys(end, next_key)) take(++n);
+        if (n < 32) mine = order_wide<T>(row, a, r.top, mine, n, lane);
+        else crowd = true;
+      }
     }
   }
-  if (doubt) {
+  if (crowd) {
     __syncwarp();
     mine = choose_wide<T>(row, a, shared + warp * E, lane);
   }

@@ -133,6 +133,25 @@ def test_neighbouring_values(device, experts, top_k):
 
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('experts,groups,top_groups', [(256, 8, 4), (60, 5, 2), (700, 1, 1)])
+def test_some_close_values_among_others(device, score, experts, groups, top_groups):
+    """A few of the chosen experts, of those behind them and of the groups are as good as equal, the others not."""
+    gen = torch.Generator().manual_seed(5)
+    logits = torch.randn(300, experts, generator=gen)
+    order = logits.argsort(dim=-1, descending=True)
+    for first, count in ((1, 2), (4, 5)):               # of six: the second and third; the fifth to the ninth
+        at = order[:, first:first + count]
+        near = logits.gather(1, at[:, :1]).expand(-1, count).contiguous().view(torch.int32)
+        logits.scatter_(1, at, (near + torch.randint(0, 3, near.shape, generator=gen, dtype=torch.int32)).view(FP32))
+    logits = logits.to(device)
+    bias = torch.randint(0, 3, (experts,), generator=gen).to(device) * 2.0**-26
+    for b in (None, bias):
+        got, want = both(logits, top_k=6, score=score, bias=b, groups=groups, top_groups=top_groups, norm_p=1)
+        assert torch.equal(got[2].cpu(), want[2])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
 @pytest.mark.parametrize('bias', [None, 0.0, 0.25])
 @pytest.mark.parametrize('dtype', [BF16, FP32])
 def test_ties_go_to_the_lowest_id(device, score, bias, dtype):
