@@ -200,7 +200,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int q0 = blockIdx.x * G * kTile, head = blockIdx.y, b = blockIdx.z;
+  // Heads fastest and the last queries, which see the most keys, first, so that short CTAs end the launch.
+  const int head = blockIdx.x % p.heads, b = blockIdx.x / p.heads;
+  const int q0 = int(gridDim.y - 1 - blockIdx.y) * G * kTile;
   const int kv_head = head / (p.heads / p.kv_heads);
   const int len = length_of(p, b);
   const Tiles<G> tiles(p, q0, len);
@@ -426,7 +428,7 @@ cudaError_t launch_forward(const CUtensorMap& q, const CUtensorMap& k, const CUt
   const cudaError_t rc = allow_shared(kernel, Layout<D>::kBytes, allowed);
   if (rc != cudaSuccess) return rc;
   constexpr int rows = Layout<D>::kGroups * kTile;
-  const dim3 grid((p.seq + rows - 1) / rows, p.heads, p.batch);
+  const dim3 grid(p.heads * p.batch, (p.seq + rows - 1) / rows);
   kernel<<<grid, Layout<D>::kThreads, Layout<D>::kBytes, stream>>>(q, k, v, out, low, p);
   return cudaGetLastError();
 }

@@ -156,14 +156,15 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // Keys' kernel: heads fastest, so that the tiles of the first tokens, which have the longest streams, start
-  // first.  `part` > 0: queries far from the first tokens.
+  // Heads fastest, tiles in the order of their streams' lengths, so that short CTAs end the launch: the first keys
+  // first, which most queries see, or the last queries, which see the most keys.  `part` > 0: queries far from the first tokens.
   const int ratio = p.heads / p.kv_heads;
   const int heads_here = KEYS ? p.kv_heads : p.heads;
   const int own_head = blockIdx.x % heads_here, b = blockIdx.x / heads_here;
   const int far_blocks = KEYS ? p.far_splits * ((p.sinks + kTile - 1) / kTile) : 0;
   const int part = KEYS && int(blockIdx.y) < far_blocks ? 1 + int(blockIdx.y) % p.far_splits : 0;
-  const int x_tile = part > 0 ? int(blockIdx.y) / p.far_splits : int(blockIdx.y) - far_blocks;
+  const int y = int(blockIdx.y);
+  const int x_tile = part > 0 ? y / p.far_splits : KEYS ? y - far_blocks : int(gridDim.y) - 1 - y;
   const int x_row = x_tile * kTile;
   const int len = length_of(p, b);
 
