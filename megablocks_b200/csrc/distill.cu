@@ -6,12 +6,16 @@
 //
 // Bound by memory: a logit is read once and its gradient written once.  Where a row fits shared memory, CTAs
 // stay and walk the rows.  A row is fetched by bulk copies, in chunks, and worked on in three passes over shared
-// memory (maximum; sums; gradient, stored straight to memory); the last pass hands its chunks back, and a warp
-// of its own fetches the next row's into them and prepares the next row's teacher.  Two CTAs share an SM where
-// two rows fit, so that one takes exponentials, of which there are two a logit, while the other waits for a
-// sum or a copy.  Longer rows, and passes without a gradient, stream the row from memory with a running maximum;
-// a gradient then reads it again, from L2.  The few columns that the teacher or the target names are written
-// again, with their whole value and one rounding, after the row.
+// memory (maximum, as the chunks arrive; sums; gradient, stored straight to memory); the last pass hands its chunks
+// back, and a warp of its own fetches the next row's into them and prepares the next row's teacher.  Two CTAs share
+// an SM where two rows fit, so that one takes exponentials, of which there are two a logit, while the other waits for a
+// sum or a copy.  Maximum and sums in one pass, with a maximum per thread, took 20 % longer.  Longer rows, and passes
+// without a gradient, stream the row from memory with a running maximum; a gradient then reads it again, from
+// L2.  The few columns that the teacher or the target names are written again, with their whole value and one
+// rounding, after the row.
+//
+// 8192 rows of 51200 bf16 logits, 64 of the teacher: 332 us (1.68 GB, 0.78 of the copy bandwidth), 347 with the mean
+// and the backward pass's factor; half of the exponentials' rate, half of the issue slots.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -19,12 +23,13 @@ namespace mb {
 
 namespace {
 
-constexpr int kChunks = 8;                        // most chunks of a row in shared memory
+constexpr int kChunks = 4;                        // most chunks of a row in shared memory; with 8: 357 us of kernel
 constexpr int kMaxThreads = 256;
-constexpr int kRowThreads = 768;                  // most threads that work on a row in shared memory
+constexpr int kRowThreads = 768;                  // of an SM that work on rows; 640: 363 us, 512: 368, 896: 416
 constexpr int kSharedBytes = 226 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kMost = 0x1p30f;                  // of an offset: its rounding, 2^6 at most, is an exponent
 
 // 16 bytes of logits as pairs of fp32 values, on which the arithmetic runs two to an instruction.
 template <typename T>
@@ -299,7 +304,8 @@ struct RowGrad {
 
 enum Parts { kNothing, kOne, kBoth };                // to learn from a row; whatever its logits where nothing
 __device__ __forceinline__ Parts parts_of(const RowGrad& g) {
-  return g.soft == 0.f && g.hard == 0.f ? kNothing : (g.hard == 0.f ? kOne : kBoth);
+  if (g.soft == 0.f && g.hard == 0.f) return kNothing;
+  return g.hard == 0.f && fabsf(g.offset) <= kMost ? kOne : kBoth;
 }
 
 template <Parts P, int N>
@@ -349,7 +355,7 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, bool live, boo
     g.hard = 0.f;
   }
   g.offset = max * w.k;
-  if (g.hard == 0.f && g.soft != 0.f) g.soft *= exp2_approx(-fmaf(max, w.k, -g.offset));
+  if (parts_of(g) == kOne) g.soft *= exp2_approx(-fmaf(max, w.k, -g.offset));
   return g;
 }
 
@@ -436,7 +442,7 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ float red[4][kRowThreads / 32];
-  __shared__ alignas(8) uint64_t full, empty[kChunks];
+  __shared__ alignas(8) uint64_t full[kChunks], empty[kChunks];
   __shared__ int abort_flag;
   __shared__ TeacherFacts facts[3];
   const int threads = blockDim.x - 32, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -444,8 +450,10 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
   float* teachers = reinterpret_cast<float*>(shared + row_bytes);          // [3]
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    ptx::mbar_init(ptx::smem_u32(&full), 1);
-    for (int c = 0; c < kChunks; ++c) ptx::mbar_init(ptx::smem_u32(&empty[c]), warps);
+    for (int c = 0; c < kChunks; ++c) {
+      ptx::mbar_init(ptx::smem_u32(&full[c]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty[c]), warps);
+    }
     ptx::fence_barrier_init();
   }
   __syncthreads();
@@ -465,15 +473,15 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
         const Cut<T> cut(in, a.vocab);
         const int first = cut.head > 0 ? 1 : 0, last = first + cut.packs;  // blocks that are whole
         const T* block0 = in + cut.head - first * VEC;
-        const uint32_t bar = ptx::smem_u32(&full);
         for (int c = 0; c < kChunks && c * chunk * 16 < row_bytes; ++c) {
           if (again)
             ok = ok && ptx::mbar_wait(ptx::smem_u32(&empty[c]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (lane == 0) {
-            if (c == 0) ptx::mbar_arrive_expect_tx(bar, uint32_t(cut.packs) * 16);
+            const uint32_t bar = ptx::smem_u32(&full[c]);
             const int from = max(first, c * chunk), to = min(last, (c + 1) * chunk);
+            ptx::mbar_arrive_expect_tx(bar, uint32_t(max(0, to - from)) * 16);
             if (from < to) ptx::bulk_load(blocks + from * 16, block0 + from * VEC, uint32_t(to - from) * 16, bar);
           }
           __syncwarp();
@@ -514,27 +522,33 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
                      : int(threadIdx.x) - cut.head < cut.tail ? tail0 + int(threadIdx.x) - cut.head : -1;
     const float edge = mine >= 0 ? to_float(in[mine]) : -INFINITY;
     auto value_at = [&](int c) { return to_float(c < cut.head || c >= tail0 ? in[c] : copy[c]); };
-    // The whole blocks of a chunk, a thread's share of them.
+    // The row's whole blocks, a thread's share of them.
     auto each = [&](auto&& body) {
 #pragma unroll 4
       for (int i = first + threadIdx.x; i < last; i += threads) body(i);
     };
 
-    // One warp looks for the row's arrival; the others stand at the barrier, where they cost no issue slots.
-    if (warp == 0) ptx::mbar_wait(ptx::smem_u32(&full), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs);
-    group_sync();
-    const TeacherFacts f = facts[set];
-    const bool ok = *static_cast<volatile int*>(&abort_flag) == 0;
+    // The maximum, chunk by chunk as they arrive.
     float top = edge;
-    if (ok) each([&](int i) { top = fmaxf(top, pack_max<T>(load_shared(blocks + i * 16))); });
+    for (int c = 0; c < kChunks && c * chunk * 16 < row_bytes; ++c) {
+      if (!ptx::mbar_wait(ptx::smem_u32(&full[c]), phase, &abort_flag, a.status, kDistillTimeout, kWaitNs)) break;
+      const int to = min(last, (c + 1) * chunk);
+#pragma unroll 4
+      for (int i = max(first, c * chunk) + int(threadIdx.x); i < to; i += threads)
+        top = fmaxf(top, pack_max<T>(load_shared(blocks + i * 16)));
+    }
+    const TeacherFacts f = facts[set];
     top = warp_max(top);
     if (lane == 0) red[0][warp] = top;
     group_sync();
     top = warp_max(lane < warps ? red[0][lane] : -INFINITY);
+    const bool ok = *static_cast<volatile int*>(&abort_flag) == 0;
     const float base = top == -INFINITY ? 0.f : top;
 
-    // 2^(z k - offset) is e^((z - max) / T) up to the rounding of the offset, which all of the row share.
+    // 2^(z k - offset) is e^((z - max) / T) up to the rounding of the offset, which all of the row share.  Where that
+    // is too large (a row of the type's lowest value), or the hard part wants them, differences come first.
     const float offset = base * w.k;
+    const bool differ = two || !(fabsf(offset) <= kMost);
     float2 soft = splat2(0.f), hard = soft;
     float cross = 0.f;
     for (int i = threadIdx.x; i < a.top; i += threads) {
@@ -544,10 +558,10 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
     }
     const float z_target = target >= 0 ? value_at(target) : 0.f;
     if (mine >= 0) {
-      soft.x = two ? exp2_approx((edge - base) * w.k) : exp2_approx(fmaf(edge, w.k, -offset));
+      soft.x = differ ? exp2_approx((edge - base) * w.k) : exp2_approx(fmaf(edge, w.k, -offset));
       if (two) hard.x = w.second(soft.x, edge - base);
     }
-    const float2 minus = splat2(two ? -base : -offset), k2 = splat2(w.k);
+    const float2 minus = splat2(differ ? -base : -offset), k2 = splat2(w.k);
     auto add = [&](auto with_hard) {
       each([&](int i) {
         float2 x[kPairs<T>];
@@ -565,7 +579,7 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
       });
     };
     if (ok) {
-      if (two) add(std::true_type{});
+      if (differ) add(std::true_type{});
       else add(std::false_type{});
     }
     {
@@ -575,7 +589,7 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
     group_sync();
     float sum_soft = warp_sum(lane < warps ? red[1][lane] : 0.f);
     const float all_cross = warp_sum(lane < warps ? red[3][lane] : 0.f);
-    if (!two) sum_soft *= exp2_approx(-fmaf(base, w.k, -offset));
+    if (!differ) sum_soft *= exp2_approx(-fmaf(base, w.k, -offset));
     const float sum_hard = two ? warp_sum(lane < warps ? red[2][lane] : 0.f) : sum_soft;
     if (threadIdx.x == 32 % threads) {
       float l = 0.f;

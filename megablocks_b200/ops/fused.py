@@ -164,8 +164,13 @@ def _composed_distillation(logits, teacher_logits, teacher_ids, temperature, tar
     z = logits if logits.dtype == torch.float64 else logits.float()
     ids = teacher_ids.long()
     used = (ids >= 0) & (ids < vocab)
-    values = (teacher_logits.detach().to(z.dtype) / temperature).masked_fill(~used, -math.inf)
+    def shifted(x):                                 # by the maximum, before a small temperature overflows
+        top = x.detach().amax(dim=-1, keepdim=True)
+        return (x - top.masked_fill(top == -math.inf, 0.0)) / temperature
+
+    values = teacher_logits.detach().to(z.dtype).masked_fill(~used, -math.inf)
     used = used & (values != -math.inf)
+    values = shifted(values)
     live = used.any(dim=-1)
     logp = values.masked_fill(~live.unsqueeze(1), 0.0).log_softmax(dim=-1).masked_fill(~used, 0.0)
     p = logp.exp() * used
@@ -174,7 +179,7 @@ def _composed_distillation(logits, teacher_logits, teacher_ids, temperature, tar
     if targets is not None and hard_weight:
         hard = (targets >= 0) & (targets < vocab)
     z = z.masked_fill(~(live | hard).unsqueeze(1), 0.0)
-    logq = (z / temperature).log_softmax(dim=-1).gather(1, ids.masked_fill(~used, 0))
+    logq = shifted(z).log_softmax(dim=-1).gather(1, ids.masked_fill(~used, 0))
     loss = temperature**2 * torch.where(used & live.unsqueeze(1), p * (logp - logq), 0.0).sum()
     if targets is not None and hard_weight:
         ce = -z.log_softmax(dim=-1).gather(1, targets.masked_fill(~hard, 0).unsqueeze(1)).squeeze(1)

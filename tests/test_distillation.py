@@ -162,6 +162,21 @@ def test_masked_columns_and_masked_teacher_slots(device, dtype):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('vocab', [40, 3001])
+@pytest.mark.parametrize('temperature,hard', [(1.0, 0.0), (1.0, 0.5), (0.5, 0.5), (3.0, 0.0)])
+def test_rows_masked_by_the_lowest_value(device, dtype, vocab, temperature, hard):
+    """All of a row, all but the columns that are named, and long stretches."""
+    logits, values, ids, targets = batch(5, vocab, 5, dtype, device)
+    low = torch.finfo(dtype).min
+    logits[0] = low
+    for r, columns in ((1, range(vocab)), (2, range(vocab // 2)), (3, range(vocab // 3, vocab))):
+        logits[r, [c for c in columns if c not in ids[r].tolist() and c != int(targets[r])]] = low
+    got = check(logits, values, ids, temperature, targets, hard)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
 def test_logits_far_from_zero(device):
     """A constant on all logits changes nothing, also where it is large."""
     logits, values, ids, targets = batch(6, 500, 8, FP32, device)
