@@ -71,6 +71,19 @@ def main():
     logits = torch.randn(T, E, device=dev, dtype=bf)
     add('router softmax + top-k forward', lambda: ext().router_topk_forward(logits, 2, 0.0), nbytes=2 * T * E * 2)
 
+    wide = torch.randn(32768, 256, device=dev, dtype=bf, requires_grad=True)
+    lift = torch.randn(256, device=dev) * 0.03
+
+    def select():
+        return ops.select_experts(wide, 8, score='sigmoid', bias=lift, groups=8, top_groups=4, norm_p=1, scale=2.5)
+
+    add('expert selection forward (256 experts in 8 groups)', select, nbytes=2 * wide.numel() * 2 + 32768 * 8 * 10)
+    if args.only is None or args.only in 'expert selection backward':
+        picked = select()[1]
+        gp = torch.randn_like(picked)
+        add('expert selection backward', lambda: torch.autograd.grad(picked, wide, gp, retain_graph=True),
+            nbytes=wide.numel() * 2)
+
     # ---- row-wise model kernels -----------------------------------------------------------
     ln = fused.LayerNorm(H).to(device=dev, dtype=bf)
     rn = fused.RMSNorm(H).to(device=dev, dtype=bf)
@@ -90,7 +103,24 @@ def main():
     one = torch.ones(1, device=dev)
     add('cross-entropy backward (in place)', lambda: ext().cross_entropy_backward_(lg, tg, lse, one, 1.0 / R),
         nbytes=2 * R * V * 2)
+    lt = lg.clone().requires_grad_(True)
+    tv, ti = torch.randn(R, 64, device=dev), torch.randint(0, V, (R, 64), device=dev)
+    add('distillation loss with gradient (64 teacher logits)', lambda: fused.distillation_loss(lt, tv, ti, 2.0),
+        nbytes=2 * R * V * 2)
     q = torch.randn(8, 4096, 32, 128, device=dev, dtype=bf)
+    heads = [torch.randn(2, 8192, n, 128, device=dev, dtype=bf, requires_grad=True) for n in (32, 8, 8)]
+    pairs = 2 * 32 * (8192 * 1024 - 1024 * 1023 // 2 + 4 * (8192 - 1024))      # the first tokens' about
+    add('windowed attention forward (window 1024, 4 first tokens)',
+        lambda: ops.window_attention(*(t.detach() for t in heads), 1024, 4), flops=4.0 * 128 * pairs)
+    if args.only is None or args.only in 'windowed attention backward':
+        seen = ops.window_attention(*heads, 1024, 4)
+        gs = torch.randn_like(seen)
+        add('windowed attention backward', lambda: torch.autograd.grad(seen, heads, gs, retain_graph=True),
+            flops=10.0 * 128 * pairs)
+    caches = [torch.randn(32, 4096, 8, 128, device=dev, dtype=bf) for _ in range(2)]
+    full = torch.full((32,), 4096, device=dev, dtype=torch.int32)
+    add('windowed attention of one token (4096 keys, 32 sequences)',
+        lambda: ops.window_attention_decode(q[0, :32], *caches, full), nbytes=2 * caches[0].numel() * 2)
     inv = 1.0 / (10000.0**(torch.arange(0, 128, 2, device=dev).float() / 128))
     ang = torch.outer(torch.arange(4096, device=dev).float(), inv)
     cos, sin = ang.cos().contiguous(), ang.sin().contiguous()

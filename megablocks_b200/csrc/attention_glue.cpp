@@ -232,10 +232,11 @@ at::Tensor window_attention_decode(const at::Tensor& q, const at::Tensor& k, con
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.is_contiguous() && reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 == 0 &&
                   in_place(k) && in_place(v) && q.device() == k.device() && k.device() == v.device() &&
                   q.scalar_type() == k.scalar_type() && k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() &&
-                  q.size(0) == k.size(0) && q.size(2) == k.size(3) && q.size(1) % k.size(2) == 0 &&
-                  k.size(1) < (int64_t(1) << 30) && q.size(0) < (int64_t(1) << 16) && q.size(1) < (int64_t(1) << 16),
+                  q.size(0) == k.size(0) && q.size(2) == k.size(3) && q.size(1) % k.size(2) == 0,
               "window_attention_decode expects 16-bit CUDA q[batch, heads, dim] and caches [batch, capacity, kv_heads, "
               "dim] with aligned rows");
+  TORCH_CHECK_VALUE(k.size(1) < (int64_t(1) << 30) && q.size(0) < (int64_t(1) << 16) && q.size(1) < (int64_t(1) << 16),
+                    "window_attention_decode takes fewer than 65536 sequences and heads and 2^30 tokens");
   TORCH_CHECK(lengths_in.device() == q.device() && lengths_in.dim() == 1 && lengths_in.size(0) == q.size(0),
               "window_attention_decode: lengths must be [batch]");
   TORCH_CHECK_VALUE(window >= 1 && sinks >= 0 && float(scale) > 0 && std::isfinite(float(scale)),

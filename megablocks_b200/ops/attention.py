@@ -102,7 +102,8 @@ def window_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
 
     ``lengths[batch]``: valid tokens, the new one included (clamped to ``[0, capacity]``); an idle slot of length
     0 gives zeros.  Only visible keys are read.  The caches may have any strides; where their rows do not start
-    on 16 bytes the visible ones are gathered by PyTorch ops.  Not differentiable."""
+    on 16 bytes the visible ones are gathered by PyTorch ops.  On CUDA fewer than 65536 sequences and heads and
+    2^30 tokens.  Not differentiable."""
     if q.dim() != 3 or k.dim() != 4 or v.dim() != 4 or q.shape[0] != k.shape[0]:
         raise ValueError('window_attention_decode expects q[batch, heads, dim] and k, v[batch, capacity, kv_heads, dim]')
     if lengths is None:

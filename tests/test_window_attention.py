@@ -445,6 +445,15 @@ def test_sizes_that_are_refused(shape):
         ops.window_attention(q, q, q, 4)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('batch,heads', [(65536, 1), (1, 65536)])
+def test_decode_sizes_that_are_refused(batch, heads):
+    q = torch.zeros(batch, heads, 8, dtype=BF16, device='cuda')
+    k = torch.zeros(batch, 1, 1, 8, dtype=BF16, device='cuda')
+    with pytest.raises(ValueError):
+        ops.window_attention_decode(q, k, k, torch.ones(batch, dtype=torch.int32, device='cuda'), 4)
+
+
 @pytest.mark.parametrize('device', DEVICES)
 def test_lengths_beyond_32_bits_are_clamped(device):
     q, k, v = inputs(3, 20, 4, 2, 64, BF16, device, fused=False)
