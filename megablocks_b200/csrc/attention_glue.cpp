@@ -150,13 +150,14 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
       // window.  It starts first; where it would still end last, what exceeds a window is split into parts of a
       // window's length (and at least 1024 rows).  An SM runs one CTA of large heads, two of small ones.  More
       // first tokens than a tile make long streams enough to fill the SMs, and the parts' workspace grows with them.
-      const int usual = (p.window + attn::kTile + rows - 1) / rows;
+      const int usual = attn::near_tiles(0, p.window, rows);
       const int far_tiles = std::max(0, (p.seq + rows - 1) / rows - usual);
       const int64_t streams = int64_t(p.batch) * p.kv_heads * ((p.seq + attn::kTile - 1) / attn::kTile);
       const int64_t share = streams * usual / (int64_t(sm_count()) * (p.dim > 64 ? 1 : 2));
       if (p.sinks <= attn::kTile && far_tiles > 0 && usual + far_tiles > std::max<int64_t>(usual + usual / 2, share * 3 / 4)) {
         p.far_tiles = std::max({usual, 1024 / rows, (far_tiles + 63) / 64});
         p.far_splits = (far_tiles + p.far_tiles - 1) / p.far_tiles;
+        p.far_first = usual;
         far = at::empty({p.far_splits + 1, p.batch, p.kv_heads, 2, p.sinks, p.dim}, lse.options());
         p.far = far.data_ptr<float>();
       }

@@ -129,6 +129,11 @@ namespace attn {
 constexpr int kTile = 128;             // rows of a resident tile, keys of a streamed one in the forward pass
 // Rows of a streamed tile in the backward pass.
 constexpr int streamed_rows(int dim) { return dim > 64 ? 128 : 64; }
+// Tiles of `rows` queries, from the first on, that hold a query whose window (no longer than a sequence) reaches the
+// keys of the tile from `x_row` on.
+__host__ __device__ constexpr int near_tiles(int x_row, int window, int rows) {
+  return int((int64_t(x_row) + kTile + window - 2) / rows) + 1;
+}
 constexpr int kPadRows = 256;          // per-row statistics are padded to a multiple of this
 constexpr int kErrLoad = 48, kErrMma = 49, kErrRows = 50;
 
@@ -144,9 +149,10 @@ struct Params {
   void* out_low;                       // nullable: what the rounding of `out` left, [batch, seq, heads, dim]
   int seq_pad;
   bool split;                          // backward pass: P and dS as two 16-bit numbers each
-  // Backward pass over the keys: queries a window away from the first tokens are split into `far_splits`
-  // parts of `far_tiles` tiles, whose shares of the first tokens' gradients are summed afterwards.
-  int far_splits, far_tiles;
+  // Backward pass over the keys: queries a window away from the first tokens, from query tile `far_first` on, are
+  // split into `far_splits` parts of `far_tiles` tiles, whose shares of the first tokens' gradients are summed
+  // afterwards.
+  int far_splits, far_tiles, far_first;
   float* far;                          // [far_splits + 1][batch, kv_heads][2][sinks][dim]
   int* status;
 };

@@ -181,13 +181,12 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_const
     const int tiles = (len + R - 1) / R;
     if constexpr (KEYS) {
       // Queries from the tile's own on; up to a window behind its last key, or all for first tokens.
-      const int near = int(min(int64_t(tiles), (int64_t(x_row) + kTile + p.window - 2) / R + 1));
       st.lo = x_row / R;
-      int hi = near;
+      int hi = min(tiles, near_tiles(x_row, p.window, R));
       if (x_row < p.sinks) {
         if (p.far_splits == 0) hi = tiles;
         if (part > 0) {
-          st.lo = near + (part - 1) * p.far_tiles;
+          st.lo = p.far_first + (part - 1) * p.far_tiles;
           hi = min(tiles, st.lo + p.far_tiles);
         }
       }

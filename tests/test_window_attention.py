@@ -499,3 +499,32 @@ def test_the_first_call_of_a_process_may_be_recorded():
     done = subprocess.run([sys.executable, '-c', _FIRST_IN_A_GRAPH.format(root=root)], capture_output=True, text=True,
                           timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# Far queries that are split, where the last part's tiles end with the sequence: with windows that end one row into a
+# tile, and others.
+FAR = [(1400, 8, 128, 129), (1472, 4, 64, 257), (1153, 4, 64, 1), (2300, 2, 64, 65), (1300, 1, 96, 129), (1408, 2, 128, 130),
+       (1472, 1, 64, 256), (2178, 1, 32, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('ratio,lengths', [(1, None), (2, None), (1, [0, 64, 65])])
+@pytest.mark.parametrize('seq,hk,d,window', FAR)
+def test_every_far_query_has_a_share_in_the_first_tokens(seq, hk, d, window, ratio, lengths):
+    """Gradients that arrive at single queries, those at the end of a stream among them: what the first tokens get
+    of each is there once."""
+    b = 1 if lengths is None else 3
+    if lengths is not None:
+        lengths = torch.tensor([seq - n for n in lengths], dtype=torch.int32, device='cuda')
+    q, k, v = (t.requires_grad_(True) for t in inputs(b, seq, hk * ratio, hk, d, BF16, 'cuda', fused=False))
+    out = ops.window_attention(q, k, v, window, 4, lengths)
+    half = torch.finfo(BF16).eps / 2
+    for at in (range(seq - 130, seq, 64), range(140, seq, 256)):
+        dout = torch.zeros_like(out)
+        rows = list(at) + [seq - 1]
+        dout[:, rows] = torch.randn(b, len(rows), hk * ratio, d, device='cuda').to(BF16)
+        grads = torch.autograd.grad(out, (k, v), dout, retain_graph=True)
+        _, _, exact, mags = plain(q, k, v, window, 4, lengths, dout=dout)
+        for got, want, mag in zip(grads, exact[1:], mags[1:]):
+            assert_rounded(got, want, 0.0, mag * (2 * half + 2.0**-15))
+            assert got[0, :4].any(-1).all()
