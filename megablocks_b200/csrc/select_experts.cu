@@ -44,6 +44,8 @@ __device__ __forceinline__ unsigned ordered(float v) {
 __device__ __forceinline__ float from_ordered(unsigned k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+// The value of a key that has lost its last bits: without them that of -infinity, 0x007fffff, is a NaN's.
+__device__ __forceinline__ float value_of(unsigned key) { return from_ordered(max(key, 0x007fffffu)); }
 
 // Experts of a lane: PL consecutive ones, so that a lower lane has lower ids.
 template <int PL>
@@ -317,7 +319,8 @@ __device__ __forceinline__ unsigned choose_groups(float b1, float b2, int shift,
   const bool stays = there && rank < a.top_groups;
   const float last = from_ordered(__reduce_min_sync(0xffffffffu, stays ? value : 0xffffffffu));
   const float next = from_ordered(__reduce_max_sync(0xffffffffu, stays ? 0u : value));
-  doubt = !(last - next > 2.f * margin + 0x1p-19f * fmaxf(fabsf(last), fabsf(next)));
+  const float gap = last - next;
+  doubt = !(gap > 2.f * margin + 0x1p-19f * fmaxf(fabsf(last), fabsf(next)) || gap == INFINITY);
   return __ballot_sync(0xffffffffu, stays);
 }
 
@@ -372,8 +375,8 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
     float b1 = -INFINITY, b2 = -INFINITY;
     if (a.aligned_shift >= 0) {                           // groups of whole lanes, a power of two of them
       if (kSorted && biased) {                            // the places' bits are within what `doubt` allows
-        b1 = key[0] != 0u ? from_ordered(key[0] & ~kPlace) : -INFINITY;
-        if (PL > 1) b2 = key[PL > 1 ? 1 : 0] != 0u ? from_ordered(key[PL > 1 ? 1 : 0] & ~kPlace) : -INFINITY;
+        b1 = value_of(key[0] & ~kPlace);
+        if (PL > 1) b2 = value_of(key[PL > 1 ? 1 : 0] & ~kPlace);
       } else {
 #pragma unroll
         for (int j = 0; j < PL; ++j) {
@@ -457,8 +460,8 @@ select_fwd_kernel(const T* __restrict__ logits, const SelectArgs a, T* __restric
   if (inexact) {                                          // all neighbours at once; a key of 0: no expert was left
     auto close_keys = [&](unsigned k, unsigned next) {
       if (!biased) return k == next;
-      const float c = from_ordered(k), d = from_ordered(next);
-      return !(c - d > margin + 0x1p-20f * fmaxf(fabsf(c), fabsf(d)));
+      const float c = value_of(k), d = value_of(next), gap = c - d;
+      return !(gap > margin + 0x1p-20f * fmaxf(fabsf(c), fabsf(d)) || gap == INFINITY);
     };
     const bool last = lane == a.top_k - 1;
     const unsigned down = __shfl_down_sync(0xffffffffu, mine_key, 1), next = last ? next_key : down;

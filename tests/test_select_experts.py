@@ -342,3 +342,41 @@ def test_differentiable_once():
     assert torch.equal(first, again)
     with pytest.raises(RuntimeError, match='differentiable once'):
         again.sum().backward()
+
+
+def banned(experts, groups, which):
+    """Biases that take experts out: single ones, 8 consecutive ones, whole groups, all but one or two of a group."""
+    size = experts // groups
+    bias = torch.randn(experts, generator=torch.Generator().manual_seed(11)) * 0.05
+    if which == 'one':
+        bias[size // 2] = bias[-1] = -math.inf
+    elif which == 'eight':
+        bias[:min(8, size)] = -math.inf
+        bias[size * (groups // 2):][:min(8, size)] = -math.inf
+    elif which == 'group':
+        bias[size:2 * size] = -math.inf
+    elif which == 'groups':
+        for g in range(0, groups, 3):
+            bias[g * size:(g + 1) * size] = -math.inf
+    elif which == 'most':
+        bias[1:size] = -math.inf                # one is left: the sum of the two largest is -inf
+        bias[size + 2:2 * size] = -math.inf     # two
+    elif which == 'preferred':
+        bias[size * (groups - 1)] = math.inf
+    return bias
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [BF16, FP32])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('experts,groups,top_groups,top_k', [(256, 8, 4, 8), (256, 8, 1, 4), (64, 8, 3, 6), (128, 4, 2, 8),
+                                                             (60, 5, 2, 4), (512, 8, 4, 8), (96, 1, 1, 6)])
+@pytest.mark.parametrize('which', ['one', 'eight', 'group', 'groups', 'most', 'preferred'])
+def test_banned_and_preferred_experts(device, dtype, score, experts, groups, top_groups, top_k, which):
+    if groups == 1 and which != 'one':
+        which = 'eight' if which == 'eight' else 'preferred'
+    bias = banned(experts, groups, which).to(device)
+    logits = torch.randn(120, experts).to(dtype).to(device)
+    got, want = both(logits, top_k=top_k, score=score, bias=bias, groups=groups, top_groups=top_groups, norm_p=1)
+    assert torch.equal(got[2].cpu(), want[2])
+    assert_rounded(got[1], want[1], REL)
