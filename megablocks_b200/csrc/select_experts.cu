@@ -303,7 +303,8 @@ __device__ __forceinline__ void join_best(float& b1, float& b2, int shift) {
 
 // Whether groups stay, as lane bits: bit g << shift.  `b1`, `b2`: the largest values of group lane >> shift.  The
 // lanes of a group share its comparisons.  Sets `doubt` when the last group that stays and the next are closer
-// than the arithmetic tells apart.
+// than the arithmetic tells apart: the errors of two scores each, and of what makes up a sum, whose parts may be
+// larger than the sum, 1.13 x 2^-19 of the largest (2^-20 x 0.88 for the keys' bits, 2^-24 for each rounding).
 __device__ __forceinline__ unsigned choose_groups(float b1, float b2, int shift, const SelectArgs& a, int lane,
                                                   float margin, bool& doubt) {
   const int g = lane >> shift;
@@ -319,8 +320,10 @@ __device__ __forceinline__ unsigned choose_groups(float b1, float b2, int shift,
   const bool stays = there && rank < a.top_groups;
   const float last = from_ordered(__reduce_min_sync(0xffffffffu, stays ? value : 0xffffffffu));
   const float next = from_ordered(__reduce_max_sync(0xffffffffu, stays ? 0u : value));
+  const float part = fmaxf(fabsf(b1) < INFINITY ? fabsf(b1) : 0.f, fabsf(b2) < INFINITY ? fabsf(b2) : 0.f);
+  const float largest = __uint_as_float(__reduce_max_sync(0xffffffffu, there ? __float_as_uint(part) : 0u));
   const float gap = last - next;
-  doubt = !(gap > 2.f * margin + 0x1p-19f * fmaxf(fabsf(last), fabsf(next)) || gap == INFINITY);
+  doubt = !(gap > 2.f * margin + 0x1p-18f * largest || gap == INFINITY);
   return __ballot_sync(0xffffffffu, stays);
 }
 

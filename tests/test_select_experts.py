@@ -380,3 +380,15 @@ def test_banned_and_preferred_experts(device, dtype, score, experts, groups, top
     got, want = both(logits, top_k=top_k, score=score, bias=bias, groups=groups, top_groups=top_groups, norm_p=1)
     assert torch.equal(got[2].cpu(), want[2])
     assert_rounded(got[1], want[1], REL)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('experts,groups,top_groups', [(256, 8, 4), (60, 5, 2), (512, 8, 4)])
+@pytest.mark.parametrize('size', [30.0, 1e3, 1e4, 1e6])
+def test_large_biases_of_both_signs(device, experts, groups, top_groups, size):
+    """A group's two largest values nearly cancel: what a key leaves out of them is more than their sum."""
+    bias = torch.full((experts,), -size, device=device)
+    bias[::experts // groups] = size
+    logits = torch.randn(2000, experts, device=device)
+    got, want = both(logits, top_k=4, score='sigmoid', bias=bias, groups=groups, top_groups=top_groups)
+    assert torch.equal(got[2].cpu(), want[2])
