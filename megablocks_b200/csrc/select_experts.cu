@@ -185,7 +185,7 @@ __device__ __noinline__ unsigned groups_wide(const T* row, const SelectArgs& a, 
     b2 = fmax(fmin(b1, o1), fmax(b2, o2));
     b1 = fmax(b1, o1);
   }
-  const double value = size > 1 ? b1 + b2 : b1;
+  const double value = key64(size > 1 ? b1 + b2 : b1);
   int rank = 0;
   for (int h = 0; h < a.groups; ++h) {
     const double o = __shfl_sync(0xffffffffu, value, h << shift);
@@ -208,7 +208,7 @@ __device__ __noinline__ int choose_wide(const T* row, const SelectArgs& a, doubl
         const double v = c[lane * size + i];
         if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) { b2 = v; }
       }
-      value = size > 1 ? b1 + b2 : b1;
+      value = key64(size > 1 ? b1 + b2 : b1);
     }
     int rank = 0;
     for (int h = 0; h < a.groups; ++h) {

@@ -14,6 +14,9 @@ the scores have.  The bias has a part in the choice only: no gradient reaches it
 of the unbiased scores.  It is moved by :func:`update_expert_bias`, against the load, so that a layer is
 balanced without an auxiliary loss.
 
+A bias of -inf takes an expert out, one of +inf puts it before all others; a group with both as its largest is
+worth +inf, and one with a single expert that is not taken out -inf.
+
 A token whose logits hold NaN (softmax: or +inf) gets distinct valid ids and NaN weights.  An expert with
 a logit of -inf has score 0; where every chosen score is 0, so are the weights.
 
@@ -92,6 +95,7 @@ def _composed(logits, top_k, score, bias, groups, top_groups, norm_p, scale):
         if top_groups < groups:
             size = logits.shape[1] // groups
             value = choice.view(-1, groups, size).topk(min(2, size), dim=-1).values.sum(dim=-1)
+            value = value.masked_fill(value.isnan(), math.inf)
             kept = value.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
             out = torch.ones_like(value, dtype=torch.bool).scatter_(1, kept, False).repeat_interleave(size, dim=1)
         # Experts of other groups behind all others, also behind those that are worth -inf.

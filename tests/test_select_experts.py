@@ -392,3 +392,27 @@ def test_large_biases_of_both_signs(device, experts, groups, top_groups, size):
     logits = torch.randn(2000, experts, device=device)
     got, want = both(logits, top_k=4, score='sigmoid', bias=bias, groups=groups, top_groups=top_groups)
     assert torch.equal(got[2].cpu(), want[2])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('experts,groups', [(256, 8), (16, 8), (60, 5), (1024, 32)])
+def test_a_preferred_expert_among_banned_ones(device, experts, groups):
+    """Its group is worth +inf - inf, which counts as +inf, as often as there is one: the lowest ids stay."""
+    size = experts // groups
+    logits = torch.randn(50, experts, device=device)
+    logits[7] = math.nan
+    bias = torch.randn(experts, device=device) * 0.1
+    want = []
+    for g in range(1, groups, 2):
+        bias[g * size:(g + 1) * size] = -math.inf
+        bias[(g + 1) * size - 1] = math.inf
+        want.append((g + 1) * size - 1)
+    for top_groups in range(1, len(want) + 1):
+        for score in ('softmax', 'sigmoid'):
+            _, _, ids = ops.select_experts(logits, top_groups, score=score, bias=bias, groups=groups, top_groups=top_groups)
+            rows = torch.arange(50) != 7
+            assert (ids.cpu()[rows] == torch.tensor(want[:top_groups])).all()
+            assert len(set(ids[7].tolist())) == top_groups
+    bias[0] = math.inf                          # its group's second is finite: worth +inf as well
+    ids = ops.select_experts(logits, 2, bias=bias, groups=groups, top_groups=2)[2]
+    assert (ids.cpu()[rows] == torch.tensor([0, want[0]])).all()
