@@ -237,6 +237,7 @@ __device__ __forceinline__ TeacherFacts teacher_row(const DistillArgs& a, int64_
   const int lane = threadIdx.x & 31;
   const float inv_t = 1.f / a.temperature;
   float top = -INFINITY;
+  bool any = false;            // NaN is a value too, and shows in the loss
   for (int i0 = lane; i0 < padded_slots(a.top); i0 += 128) {      // 128 slots in flight
     int64_t id[4];
     float value[4];
@@ -259,10 +260,11 @@ __device__ __forceinline__ TeacherFacts teacher_row(const DistillArgs& a, int64_
       t.column[i] = used ? int(id[u]) : -1;
       t.p[i] = used ? value[u] : -INFINITY;
       top = fmaxf(top, t.p[i]);
+      any |= t.p[i] != -INFINITY;
     }
   }
   top = warp_max(top);
-  const bool live = top > -INFINITY;
+  const bool live = __any_sync(0xffffffffu, any);
   float sum = 0.f;
   for (int i = lane; i < a.top; i += 32) sum += live ? exp2_approx((t.p[i] - top) * kLog2e) : 0.f;
   sum = warp_sum(sum);
@@ -343,12 +345,13 @@ __device__ __forceinline__ void with_parts(const RowGrad& g, F&& body) {
   else body(std::integral_constant<Parts, kBoth>{});
 }
 
-__device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, bool live, bool has_target, float scale, float max,
-                                            float sum_soft, float sum_hard, const Powers& w) {
+__device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, const TeacherFacts& f, bool has_target, float scale,
+                                            float max, float sum_soft, float sum_hard, const Powers& w) {
   RowGrad g;
   g.w = w;
   g.max = max;
-  g.soft = live ? a.temperature * scale / sum_soft : 0.f;
+  g.soft = f.live ? a.temperature * scale / sum_soft : 0.f;
+  if (f.entropy != f.entropy) g.soft = NAN;       // the teacher's probabilities are NaN, and so is their sum
   g.hard = has_target ? a.hard_weight * scale / sum_hard : 0.f;
   if (w.squares == 0) {                           // one probability serves both parts
     g.soft += g.hard;
@@ -597,7 +600,7 @@ distill_rows_kernel(const DistillArgs a, int row_bytes, int chunk, float* __rest
       if (target >= 0) l += a.hard_weight * (kLn2 * __log2f(sum_hard) + (top - z_target));
       *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(ok ? l : NAN, top, sum_soft, sum_hard);
     }
-    const RowGrad g = row_grad(a, f.live != 0, target >= 0, a.scale, top, sum_soft, sum_hard, w);
+    const RowGrad g = row_grad(a, f, target >= 0, a.scale, top, sum_soft, sum_hard, w);
     T* out = grad + row * a.vocab;
     if (mine >= 0) out[mine] = from_float<T>(gradient(g, edge));
     T* block0 = out + cut.head - first * VEC;      // where block 0 would lie
@@ -699,7 +702,7 @@ distill_fwd_kernel(const DistillArgs a, float* __restrict__ stats, T* grad) {
   }
   if (grad == nullptr) return;
   T* out = grad + row * a.vocab;
-  const RowGrad g = row_grad(a, live, target >= 0, a.scale, sums.m, sums.soft, sums.hard, w);
+  const RowGrad g = row_grad(a, f, target >= 0, a.scale, sums.m, sums.soft, sums.hard, w);
   write_gradient(in, cut, out, a.vocab, g);
   __syncthreads();
   write_named(a, out, g, a.temperature * a.scale, a.hard_weight * a.scale, t, f, target, z_target, blockDim.x);
@@ -726,7 +729,7 @@ distill_bwd_kernel(const DistillArgs a, const float* __restrict__ stats, const f
   const float z_target = target >= 0 ? to_float(in[target]) : 0.f;
   const float scale = a.scale * *grad_out;
   const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
-  const RowGrad g = row_grad(a, facts.live != 0, target >= 0, scale, st.y, st.z, st.w, powers(a));
+  const RowGrad g = row_grad(a, facts, target >= 0, scale, st.y, st.z, st.w, powers(a));
   T* out = grad + row * a.vocab;
   write_gradient(in, cut, out, a.vocab, g);
   __syncthreads();

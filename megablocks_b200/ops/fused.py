@@ -148,7 +148,8 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     over the columns that ``teacher_ids[rows, top]`` (int32 or int64) names: the teacher's kept logits, taken as
     its whole distribution.  Ids outside the vocabulary mark unused slots, a column named twice counts twice;
     a row without a used slot has no such term, one whose target lies outside the vocabulary no cross
-    entropy, and a row with neither has a gradient of zero, whatever its logits.  Every row counts in the mean.
+    entropy, and a row with neither has a gradient of zero, whatever its logits.  Every row counts in the mean.  A
+    used slot of NaN makes the loss and the row's gradient NaN.
     The teacher gets no gradient; the logits stay as they are."""
     if logits.is_cuda and logits.dtype in _DISTILL_DTYPES and teacher_logits.dtype != torch.float64:
         return ext().distillation_loss(logits, teacher_logits, teacher_ids, targets, temperature, hard_weight)

@@ -302,3 +302,29 @@ def test_differentiable_once(dtype):
     again, = torch.autograd.grad(fused.linear_distillation_loss(hidden, weight, values, ids), hidden, create_graph=True)
     with pytest.raises(RuntimeError):
         again.sum().backward()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('vocab', [90, 131072])
+@pytest.mark.parametrize('value_dtype', [BF16, FP32])
+def test_a_teacher_of_nan_shows(device, dtype, vocab, value_dtype):
+    """One, some or all values of a row: the loss is NaN, and the row's gradient, and no other row's."""
+    logits, values, ids, _ = batch(6, vocab, 3, dtype, device, value_dtype)
+    ids[:] = torch.arange(18, device=device).view(6, 3)
+    ids[5] = -1
+    values[1] = math.nan
+    values[2, 1] = math.nan
+    values[3] = math.nan
+    values[5] = math.nan                            # unused
+    ids[3, 1:] = -1                                 # a single slot
+    for hard, targets in ((0.0, None), (0.5, torch.full((6,), 5, device=device))):
+        logits = logits.detach().requires_grad_(True)
+        loss = fused.distillation_loss(logits, values, ids, 2.0, targets, hard)
+        assert loss.isnan()
+        got, = torch.autograd.grad(loss, logits)
+        assert got[1:4].isnan().all() and torch.isfinite(got[[0, 4, 5]]).all()
+        with torch.no_grad():
+            assert fused.distillation_loss(logits, values, ids, 2.0, targets, hard).isnan()
+    one, _, _, _ = batch(1, vocab, 1, dtype, device)
+    assert fused.distillation_loss(one, values[1:2, :1], ids[1:2, :1]).isnan()
