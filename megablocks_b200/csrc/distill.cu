@@ -249,7 +249,7 @@ __device__ __forceinline__ TeacherFacts teacher_row(const DistillArgs& a, int64_
       value[u] = -INFINITY;
       if (i < a.top) {
         id[u] = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
-        value[u] = load_value(a.values, a.value_type, at) * inv_t;
+        value[u] = load_value(a.values, a.value_type, at);
       }
     }
 #pragma unroll
@@ -266,12 +266,13 @@ __device__ __forceinline__ TeacherFacts teacher_row(const DistillArgs& a, int64_
   top = warp_max(top);
   const bool live = __any_sync(0xffffffffu, any);
   float sum = 0.f;
-  for (int i = lane; i < a.top; i += 32) sum += live ? exp2_approx((t.p[i] - top) * kLog2e) : 0.f;
+  // Differences first: the ends of the type, divided by a small temperature, would be infinite.
+  for (int i = lane; i < a.top; i += 32) sum += live ? exp2_approx((t.p[i] - top) * inv_t * kLog2e) : 0.f;
   sum = warp_sum(sum);
   const float log_sum = kLn2 * __log2f(sum), inv = 1.f / sum;
   float ent = 0.f;
   for (int i = lane; i < a.top; i += 32) {
-    const float x = t.p[i] - top;
+    const float x = (t.p[i] - top) * inv_t;
     const float w = live ? exp2_approx(x * kLog2e) * inv : 0.f;
     if (w != 0.f) ent += w * (x - log_sum);
     t.p[i] = w;

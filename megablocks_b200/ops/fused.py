@@ -181,7 +181,7 @@ def _composed_distillation(logits, teacher_logits, teacher_ids, temperature, tar
         hard = (targets >= 0) & (targets < vocab)
     z = z.masked_fill(~(live | hard).unsqueeze(1), 0.0)
     logq = shifted(z).log_softmax(dim=-1).gather(1, ids.masked_fill(~used, 0))
-    loss = temperature**2 * torch.where(used & live.unsqueeze(1), p * (logp - logq), 0.0).sum()
+    loss = temperature**2 * torch.where(p != 0, p * (logp - logq), 0.0).sum()         # p log p is 0 there
     if targets is not None and hard_weight:
         ce = -z.log_softmax(dim=-1).gather(1, targets.masked_fill(~hard, 0).unsqueeze(1)).squeeze(1)
         loss = loss + hard_weight * torch.where(hard, ce, 0.0).sum()

@@ -328,3 +328,18 @@ def test_a_teacher_of_nan_shows(device, dtype, vocab, value_dtype):
             assert fused.distillation_loss(logits, values, ids, 2.0, targets, hard).isnan()
     one, _, _, _ = batch(1, vocab, 1, dtype, device)
     assert fused.distillation_loss(one, values[1:2, :1], ids[1:2, :1]).isnan()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('value_dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('temperature', [0.25, 0.5, 1.0, 3.0])
+def test_teacher_values_at_the_ends_of_their_type(device, value_dtype, temperature):
+    """Slots that are masked by the lowest value, all of a row's too, and a row of the largest."""
+    logits, values, ids, _ = batch(6, 200, 4, BF16, device, value_dtype)
+    ids[:] = torch.arange(24, device=device).view(6, 4)
+    values[0] = torch.finfo(value_dtype).min
+    values[1, 1:] = torch.finfo(value_dtype).min
+    values[2] = torch.finfo(value_dtype).max
+    values[3, 2] = torch.finfo(value_dtype).max
+    got = check(logits, values, ids, temperature, None, 0.0)
+    assert torch.isfinite(got).all()
