@@ -10,6 +10,9 @@ fallback path by accident.  CPU tensors never touch the extension.
 import importlib
 import threading
 
+import torch
+from torch.autograd import forward_ad
+
 _lock = threading.Lock()
 _module = None
 _error = None
@@ -43,3 +46,11 @@ def ext():
 
 def available() -> bool:
     return try_ext() is not None
+
+
+def transformed(*tensors) -> bool:
+    """Whether a call is under a functional transform or a tensor carries a forward-mode tangent, neither of which the
+    kernels see: they would answer as if there were none."""
+    if torch._C._functorch.peek_interpreter_stack() is not None:
+        return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)

@@ -9,8 +9,8 @@ causal attention.  Queries may share keys (``heads`` a multiple of ``kv_heads``:
 
 On CUDA, 16-bit tensors with head sizes up to 128 (multiples of 8) run on the tensor cores
 (``csrc/window_attention*.cu``): nothing of the size ``seq x seq`` is stored, keys outside the window are not
-read, and the gradients are the same in every run.  Everything else is composed of PyTorch ops, which do store
-the scores.
+read, and the gradients are the same in every run.  Everything else, calls with forward-mode tangents or under
+functional transforms among it, is composed of PyTorch ops, which do store the scores.
 """
 
 import math
@@ -18,7 +18,7 @@ from typing import Optional
 
 import torch
 
-from megablocks_b200._ext import ext
+from megablocks_b200._ext import ext, transformed
 
 _KERNEL_DTYPES = (torch.bfloat16, torch.float16)
 
@@ -61,7 +61,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     scale = q.shape[-1]**-0.5 if scale is None else float(scale)
     _check(q, k, v, window, sinks, lengths, scale, q.shape[0])
     window = max(q.shape[1], 1) if window is None else int(window)
-    if not _kernel_dim(q) or q.numel() == 0:
+    if not _kernel_dim(q) or q.numel() == 0 or transformed(q, k, v):
         return _composed(q, k, v, window, int(sinks), lengths, scale)
     return ext().window_attention(q, k, v, window, int(sinks), lengths, scale)
 
@@ -113,7 +113,8 @@ def window_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise ValueError('window_attention_decode is not differentiable: call it without gradients')
     window = max(k.shape[1], 1) if window is None else int(window)
-    if _kernel_dim(q) and q.numel() and k.numel() and all(ext().window_attention_in_place(t) for t in (k, v)):
+    if (_kernel_dim(q) and q.numel() and k.numel() and not transformed(q, k, v)
+            and all(ext().window_attention_in_place(t) for t in (k, v))):
         q = q.contiguous()
         return ext().window_attention_decode(q if q.data_ptr() % 4 == 0 else q.clone(), k, v, lengths, window,
                                              int(sinks), scale)

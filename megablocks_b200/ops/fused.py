@@ -32,7 +32,7 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from megablocks_b200._ext import ext
+from megablocks_b200._ext import ext, transformed
 
 
 class _CrossEntropy(torch.autograd.Function):
@@ -151,7 +151,8 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     entropy, and a row with neither has a gradient of zero, whatever its logits.  Every row counts in the mean.  A
     used slot of NaN makes the loss and the row's gradient NaN.
     The teacher gets no gradient; the logits stay as they are."""
-    if logits.is_cuda and logits.dtype in _DISTILL_DTYPES and teacher_logits.dtype != torch.float64:
+    if (logits.is_cuda and logits.dtype in _DISTILL_DTYPES and teacher_logits.dtype != torch.float64
+            and not transformed(logits)):
         return ext().distillation_loss(logits, teacher_logits, teacher_ids, targets, temperature, hard_weight)
     if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] < 1:
         raise ValueError('distillation expects floating-point logits[rows, vocab]')
@@ -194,7 +195,7 @@ def linear_distillation_loss(hidden: torch.Tensor, weight: torch.Tensor, teacher
     """:func:`distillation_loss` of ``hidden[rows, h] @ weight[vocab, h]^T``: the language-model head and its loss.
     On CUDA the logits are written once, and once overwritten with their gradient."""
     if (hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float32) and hidden.dim() == 2
-            and weight.dtype == hidden.dtype and teacher_logits.dtype != torch.float64
+            and weight.dtype == hidden.dtype and teacher_logits.dtype != torch.float64 and not transformed(hidden, weight)
             and not torch.is_autocast_enabled() and os.environ.get('MB200_FUSED_LM_LOSS', '1') != '0'):
         if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
             return _LinearDistillation.apply(hidden.contiguous(), weight, teacher_logits, teacher_ids, targets,

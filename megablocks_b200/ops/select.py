@@ -20,7 +20,8 @@ worth +inf, and one with a single expert that is not taken out -inf.
 A token whose logits hold NaN (softmax: or +inf) gets distinct valid ids and NaN weights.  An expert with
 a logit of -inf has score 0; where every chosen score is 0, so are the weights.
 
-On CUDA the forward and the backward pass are one kernel each (``csrc/select_experts.cu``).
+On CUDA the forward and the backward pass are one kernel each (``csrc/select_experts.cu``); forward-mode tangents
+and functional transforms take PyTorch ops.
 """
 
 import math
@@ -28,7 +29,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from megablocks_b200._ext import ext
+from megablocks_b200._ext import ext, transformed
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 32, 32
 _SCORES = ('softmax', 'sigmoid')
@@ -65,7 +66,7 @@ def select_experts(logits: torch.Tensor, top_k: int, *, score: str = 'softmax', 
     if norm_p not in (None, 0, 1, 2):
         raise ValueError(f'norm_p must be None, 1 or 2, got {norm_p!r}')
     norm_p = int(norm_p or 0)
-    if logits.is_cuda and logits.dtype in _KERNEL_DTYPES:
+    if logits.is_cuda and logits.dtype in _KERNEL_DTYPES and not transformed(logits):
         return tuple(ext().select_experts(logits, top_k, score == 'sigmoid', bias, groups, top_groups, norm_p, scale))
     _check(logits, top_k, bias, groups, top_groups)
     return _composed(logits, top_k, score, None if bias is None else bias.detach(), groups, top_groups, norm_p, scale)

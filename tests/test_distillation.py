@@ -6,6 +6,7 @@ import pytest
 import torch
 from conftest import DEVICES
 from oracle import assert_rounded
+from torch.autograd import forward_ad
 
 from megablocks_b200.ops import fused
 
@@ -343,3 +344,27 @@ def test_teacher_values_at_the_ends_of_their_type(device, value_dtype, temperatu
     values[3, 2] = torch.finfo(value_dtype).max
     got = check(logits, values, ids, temperature, None, 0.0)
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('requires_grad', [False, True])
+def test_forward_mode_tangents(device, requires_grad):
+    logits, values, ids, targets = batch(6, 50, 4, FP32, device)
+    way = torch.randn_like(logits)
+    eps = 1e-6
+    ends = [plain(logits.double().cpu() + sign * eps * way.double().cpu(), values.cpu(), ids.cpu(), 2.0, targets.cpu(), 0.5)
+            for sign in (1, -1)]
+    want = (ends[0] - ends[1]) / (2 * eps)
+    with forward_ad.dual_level():
+        loss = fused.distillation_loss(forward_ad.make_dual(logits.requires_grad_(requires_grad), way), values, ids, 2.0,
+                                       targets, 0.5)
+        # A mean over six rows of at most (T + hard) 2 max|way|, in fp32.
+        torch.testing.assert_close(forward_ad.unpack_dual(loss).tangent.double().cpu(), want, rtol=0, atol=2.0**-16)
+    hidden, weight = torch.randn(6, 8, device=device), torch.randn(50, 8, device=device)
+    way = torch.randn_like(weight)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(weight.requires_grad_(requires_grad), way)
+        got = forward_ad.unpack_dual(fused.linear_distillation_loss(hidden, dual, values, ids, 2.0)).tangent
+        logits = forward_ad.make_dual(hidden @ weight.detach().t(), hidden @ way.t())
+        want = forward_ad.unpack_dual(fused.distillation_loss(logits, values, ids, 2.0)).tangent
+        torch.testing.assert_close(got, want)

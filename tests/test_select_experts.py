@@ -6,6 +6,7 @@ import pytest
 import torch
 from conftest import DEVICES
 from oracle import assert_rounded
+from torch.autograd import forward_ad
 
 from megablocks_b200 import ops
 from megablocks_b200.ops import select
@@ -416,3 +417,23 @@ def test_a_preferred_expert_among_banned_ones(device, experts, groups):
     bias[0] = math.inf                          # its group's second is finite: worth +inf as well
     ids = ops.select_experts(logits, 2, bias=bias, groups=groups, top_groups=2)[2]
     assert (ids.cpu()[rows] == torch.tensor([0, want[0]])).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('requires_grad', [False, True])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+def test_forward_mode_tangents(device, requires_grad, score):
+    logits = torch.randn(7, 16, device=device)
+    way = torch.randn_like(logits)
+    how = dict(top_k=3, score=score, norm_p=1, scale=2.0, bias=torch.randn(16, device=device) * 0.1)
+    wide = logits.double()
+    eps = 1e-6
+    ends = [plain(wide + sign * eps * way, **how) for sign in (1, -1)]
+    with forward_ad.dual_level():
+        got = ops.select_experts(forward_ad.make_dual(logits.requires_grad_(requires_grad), way), **how)
+        for i in range(2):
+            tangent = forward_ad.unpack_dual(got[i]).tangent
+            # Truncation and cancellation of the differences below 1e-9, sums of fp32 terms below 2.
+            torch.testing.assert_close(tangent.double(), (ends[0][i] - ends[1][i]) / (2 * eps), rtol=0, atol=2.0**-18)
+    got, tangents = torch.func.jvp(lambda x: ops.select_experts(x, **how)[1], (logits.detach(),), (way,))
+    torch.testing.assert_close(tangents.double(), (ends[0][1] - ends[1][1]) / (2 * eps), rtol=0, atol=2.0**-18)

@@ -9,6 +9,7 @@ import pytest
 import torch
 from conftest import DEVICES
 from oracle import assert_rounded
+from torch.autograd import forward_ad
 
 from megablocks_b200 import ops
 
@@ -528,3 +529,27 @@ def test_every_far_query_has_a_share_in_the_first_tokens(seq, hk, d, window, rat
         for got, want, mag in zip(grads, exact[1:], mags[1:]):
             assert_rounded(got, want, 0.0, mag * (2 * half + 2.0**-15))
             assert got[0, :4].any(-1).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('requires_grad', [False, True])
+def test_forward_mode_tangents(device, requires_grad):
+    q, k, v = inputs(2, 30, 4, 2, 64, BF16, device, fused=False)
+    ways = [torch.randn_like(t) for t in (q, k, v)]
+    lengths = torch.tensor([30, 11], dtype=torch.int32, device=device)
+    eps = 1e-6
+    ends = [plain(*(t.double() + sign * eps * w.double() for t, w in zip((q, k, v), ways)), 9, 2, lengths)[0]
+            for sign in (1, -1)]
+    want = (ends[0] - ends[1]) / (2 * eps)
+    with forward_ad.dual_level():
+        duals = [forward_ad.make_dual(t.requires_grad_(requires_grad), w) for t, w in zip((q, k, v), ways)]
+        tangent = forward_ad.unpack_dual(ops.window_attention(*duals, 9, 2, lengths)).tangent
+        # fp32 throughout, rounded once; terms of up to 30 x 8 x 6 sum to 2^-12 at most.
+        assert_rounded(tangent, want, 0.0, torch.full((), 2.0**-12, dtype=torch.float64, device=device))
+    with forward_ad.dual_level(), torch.no_grad():
+        last = [t.detach() for t in (q, k, v)]
+        q1, w1 = last[0][:, 10].contiguous(), ways[0][:, 10].contiguous()
+        only = torch.full((2,), 11, dtype=torch.int32, device=device)
+        one = ops.window_attention_decode(forward_ad.make_dual(q1, w1), last[1], last[2], only, 9, 2)
+        tangent = forward_ad.unpack_dual(one).tangent
+        assert tangent is not None and tangent.any()
