@@ -127,10 +127,11 @@ class LearnedRouter(torch.nn.Module):
                          or args.moe_router_scale != 1.0)
 
     def _apply(self, fn, *args, **kwargs):
+        bias = self.expert_bias
         super()._apply(fn, *args, **kwargs)
-        # The bias moves in steps that 16 bits would swallow: it keeps 32 when the module is cast.
-        if self.expert_bias is not None and self.expert_bias.dtype != torch.float32:
-            self.expert_bias = self.expert_bias.float()
+        # The bias moves in steps that 16 bits would swallow: it keeps its 32 when the module is cast.
+        if bias is not None and self.expert_bias.dtype != bias.dtype:
+            self.expert_bias = bias.to(self.expert_bias.device)
         return self
 
     def count_load(self, tokens_per_expert: torch.Tensor) -> None:

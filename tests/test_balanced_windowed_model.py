@@ -328,3 +328,16 @@ def test_command_line():
                        '--router-groups', '2', '--router-top-groups', '1', '--router-bias-rate', '0.01',
                        '--loss-weight', '0', '--attention-window', '16', '--attention-sinks', '2'])
     assert torch.isfinite(loss)
+
+
+@pytest.mark.parametrize('cast', [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(),
+                                  lambda m: m.to(torch.bfloat16).float(), lambda m: torch.nn.Sequential(m).bfloat16()[0]])
+def test_a_cast_leaves_the_bias_as_it_was(cast):
+    args = Arguments(hidden_size=64, moe_num_experts=4, moe_top_k=2, fp16=False, device=torch.device('cpu'),
+                     moe_router_bias=True)
+    router = router_lib.LearnedRouter(args)
+    bias = torch.tensor([0.1234567, 1.001, -0.3333, 2.0005])
+    router.expert_bias.copy_(bias)
+    router = cast(router)
+    assert router.expert_bias.dtype == torch.float32 and torch.equal(router.expert_bias, bias)
+    assert torch.equal(router.state_dict()['expert_bias'], bias)
