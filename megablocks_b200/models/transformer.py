@@ -304,15 +304,21 @@ class MoETransformer(nn.Module):
             if cfg.flavour == 'mixtral' or not self.is_first_stage:
                 self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False, **kw)
                 nn.init.normal_(self.lm_head.weight, std=cfg.init_std)
-        self._rope = None
+        self._ropes = {}             # device -> rotary tables, each at least twice as long as the one before
 
     def _rope_for(self, seq: int, device):
+        """Rotary tables of at least ``seq`` positions, cut to them.  Tables that are replaced stay alive: a recorded
+        step or decode call reads them where they are."""
         if self.cfg.flavour != 'mixtral':
             return None
-        if self._rope is None or self._rope[0].shape[0] < seq or self._rope[0].device != device:
-            head_dim = self.cfg.hidden_size // self.cfg.num_heads
-            self._rope = _rope_tables(max(seq, self.cfg.max_seq_len), head_dim, self.cfg.rope_theta, device)
-        return self._rope[0][:seq], self._rope[1][:seq]
+        kept = self._ropes.setdefault(torch.empty(0, device=device).device, [])
+        if not kept or kept[-1][0].shape[0] < seq:
+            size = max(seq, self.cfg.max_seq_len, 2 * kept[-1][0].shape[0] if kept else 0)
+            tables = _rope_tables(size, self.cfg.hidden_size // self.cfg.num_heads, self.cfg.rope_theta, device)
+            if tables[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                return tables[0][:seq], tables[1][:seq]         # filled by the replays only: not for others
+            kept.append(tables)
+        return kept[-1][0][:seq], kept[-1][1][:seq]
 
     def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
         x = self.wte(tokens)
@@ -423,6 +429,7 @@ class MoETransformer(nn.Module):
         if self.wpe is not None and capacity > cfg.max_seq_len:
             raise ValueError(f'the model has {cfg.max_seq_len} positions, a cache of {capacity} does not fit')
         weight = self.wte.weight
+        self._rope_for(capacity, weight.device)         # before a call is recorded
         shape = (batch, capacity, cfg.kv_heads, cfg.hidden_size // cfg.num_heads)
         buffers = [[torch.zeros(shape, dtype=weight.dtype, device=weight.device) for _ in self.blocks]
                    for _ in range(2)]

@@ -4,6 +4,7 @@ import math
 import os
 import subprocess
 import sys
+import weakref
 
 import pytest
 import torch
@@ -341,3 +342,67 @@ def test_a_cast_leaves_the_bias_as_it_was(cast):
     router = cast(router)
     assert router.expert_bias.dtype == torch.float32 and torch.equal(router.expert_bias, bias)
     assert torch.equal(router.state_dict()['expert_bias'], bias)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_rotary_tables_stay_where_they_are(device):
+    """Longer sequences and caches bring longer tables; those that a recording may read are not freed or moved."""
+    model = build(device, 'tiny-mixtral').eval()
+    tokens = torch.randint(0, 512, (1, 300), device=device)
+    whole = build(device, 'tiny-mixtral').eval()(tokens)
+    want = model(tokens[:, :64])
+    first = model._rope_for(64, tokens.device)
+    places = [(t.data_ptr(), weakref.ref(t.untyped_storage())) for t in first]
+    kept = [t.clone() for t in first]
+    del first
+    model.new_cache(1, 200)
+    ready = sum(map(len, model._ropes.values()))
+    for n in (65, 100, 200):                    # what a cache needs is there before the first call on it
+        model._rope_for(n, tokens.device)
+    assert sum(map(len, model._ropes.values())) == ready
+    assert torch.equal(model(tokens), whole)
+    for n in range(201, 1200):
+        model._rope_for(n, tokens.device)
+    assert sum(map(len, model._ropes.values())) <= 6        # they at least double
+    storages = [t.untyped_storage() for tables in model._ropes.values() for pair in tables for t in pair]
+    for (place, storage), table in zip(places, kept):
+        assert storage() is not None and place in [s.data_ptr() for s in storages]
+        assert any(torch.equal(t[:64], table) and t.data_ptr() == place
+                   for tables in model._ropes.values() for pair in tables for t in pair)
+    assert torch.equal(model(tokens[:, :64]), want)
+
+
+@pytest.mark.gpu
+def test_recorded_calls_and_longer_tables():
+    """A recorded pass and a recorded decode call give the same after the tables grew and memory was used again; a pass
+    whose tables are made while it is recorded leaves none that are not filled."""
+    model = build('cuda', 'tiny-mixtral', attention_window=None, attention_sinks=0).eval()
+    fixed_choice(model)
+    tokens = torch.randint(0, 512, (1, 300), device='cuda')
+    cache, spare = model.new_cache(1, 40), model.new_cache(1, 40)
+    with torch.no_grad():
+        model.prefill(tokens[:, :30], cache)
+        model.prefill(tokens[:, :30], spare)
+        model.decode(tokens[:, 30], spare)                      # warm
+        want = model.decode(tokens[:, 31], spare)
+        whole = model(tokens[:, :64])
+        decode, forward, late = (torch.cuda.CUDAGraph() for _ in range(3))
+        static = tokens[:, 30].clone()
+        with torch.cuda.graph(decode):
+            out = model.decode(static, cache)
+        with torch.cuda.graph(forward):
+            logits = model(tokens[:, :64])
+        with torch.cuda.graph(late):
+            long = model(tokens)                                # longer than any table so far
+        assert all(len(pairs) == 1 for pairs in model._ropes.values())
+        eager = model(tokens)
+        model.new_cache(1, 2000)
+        junk = [torch.full((n,), float('nan'), device='cuda') for n in (1024, 4096, 8192, 65536) for _ in range(32)]
+        del junk
+        decode.replay()
+        static.copy_(tokens[:, 31])
+        decode.replay()
+        forward.replay()
+        late.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(logits, whole) and torch.equal(long, eager)
