@@ -314,7 +314,8 @@ class MoETransformer(nn.Module):
         kept = self._ropes.setdefault(torch.empty(0, device=device).device, [])
         if not kept or kept[-1][0].shape[0] < seq:
             size = max(seq, self.cfg.max_seq_len, 2 * kept[-1][0].shape[0] if kept else 0)
-            tables = _rope_tables(size, self.cfg.hidden_size // self.cfg.num_heads, self.cfg.rope_theta, device)
+            with torch.inference_mode(False):                   # training may use them next
+                tables = _rope_tables(size, self.cfg.hidden_size // self.cfg.num_heads, self.cfg.rope_theta, device)
             if tables[0].is_cuda and torch.cuda.is_current_stream_capturing():
                 return tables[0][:seq], tables[1][:seq]         # filled by the replays only: not for others
             kept.append(tables)
@@ -431,9 +432,10 @@ class MoETransformer(nn.Module):
         weight = self.wte.weight
         self._rope_for(capacity, weight.device)         # before a call is recorded
         shape = (batch, capacity, cfg.kv_heads, cfg.hidden_size // cfg.num_heads)
-        buffers = [[torch.zeros(shape, dtype=weight.dtype, device=weight.device) for _ in self.blocks]
-                   for _ in range(2)]
-        return KVCache(*buffers, torch.zeros(batch, dtype=torch.int32, device=weight.device))
+        with torch.inference_mode(False):               # a cache may be written in any mode
+            buffers = [[torch.zeros(shape, dtype=weight.dtype, device=weight.device) for _ in self.blocks]
+                       for _ in range(2)]
+            return KVCache(*buffers, torch.zeros(batch, dtype=torch.int32, device=weight.device))
 
     @contextlib.contextmanager
     def _answering(self):

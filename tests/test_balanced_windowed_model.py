@@ -406,3 +406,20 @@ def test_recorded_calls_and_longer_tables():
         late.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(logits, whole) and torch.equal(long, eager)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('name', ['tiny', 'tiny-mixtral'])
+def test_answers_in_inference_mode_and_training_behind_them(device, name):
+    model = build(device, name)
+    tokens = torch.randint(0, 512, (2, 8), device=device)
+    want = model.generate(tokens, 4)
+    model = build(device, name)                 # without tables
+    with torch.inference_mode():
+        assert torch.equal(model.generate(tokens, 4), want)
+        cache = model.new_cache(2, 12)
+        first = model.prefill(tokens, cache).argmax(dim=-1)
+    assert torch.equal(model.decode(first.clone(), cache).argmax(dim=-1), want[:, 1])
+    total, _ = model.train().loss(tokens, tokens.roll(-1, 1))
+    total.backward()
+    assert all(torch.isfinite(p.grad).all() for p in model.parameters() if p.grad is not None)
