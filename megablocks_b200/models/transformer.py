@@ -515,7 +515,7 @@ class MoETransformer(nn.Module):
         """``steps`` most likely tokens behind each prompt: ``[batch, steps]``."""
         if steps < 1:
             raise ValueError('generate takes at least one step')
-        cache = self.new_cache(tokens.shape[0], tokens.shape[1] + steps)
+        cache = self.new_cache(tokens.shape[0], tokens.shape[1] + steps - 1)           # the last token is not fed back
         out = [self.prefill(tokens, cache, lengths).argmax(dim=-1)]
         for _ in range(steps - 1):
             out.append(self.decode(out[-1], cache).argmax(dim=-1))

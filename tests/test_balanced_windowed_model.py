@@ -423,3 +423,16 @@ def test_answers_in_inference_mode_and_training_behind_them(device, name):
     total, _ = model.train().loss(tokens, tokens.roll(-1, 1))
     total.backward()
     assert all(torch.isfinite(p.grad).all() for p in model.parameters() if p.grad is not None)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_answers_that_fill_the_positions(device):
+    """The last token is not fed back: a prompt and all answers but one need a place."""
+    model = build(device, 'tiny').eval()                    # 64 positions
+    tokens = torch.randint(0, 512, (2, 60), device=device)
+    assert model.generate(tokens, 5).shape == (2, 5)
+    assert torch.equal(model.generate(tokens, 5)[:, :3], model.generate(tokens, 3))
+    with pytest.raises(ValueError):
+        model.generate(tokens, 6)
+    full = torch.randint(0, 512, (2, 64), device=device)
+    assert model.generate(full, 1).shape == (2, 1)
