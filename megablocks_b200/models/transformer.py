@@ -218,7 +218,7 @@ class Attention(nn.Module):
                lengths: torch.Tensor) -> torch.Tensor:
         """One token per sequence (``x[1, batch, hidden]``, the batch in the place of the positions, as the
         rotary tables have it) at position ``at[batch]`` of the caches, ``lengths`` with it."""
-        q, k, v = (t.squeeze(0) for t in self._project(x, rope))
+        q, k, v = (t.squeeze(0).to(keys.dtype) for t in self._project(x, rope))        # autocast may differ
         rows = torch.arange(at.shape[0], device=at.device)
         keys[rows, at] = k
         values[rows, at] = v

@@ -436,3 +436,22 @@ def test_answers_that_fill_the_positions(device):
         model.generate(tokens, 6)
     full = torch.randint(0, 512, (2, 64), device=device)
     assert model.generate(full, 1).shape == (2, 1)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('name', ['tiny', 'tiny-mixtral'])
+@pytest.mark.parametrize('window', [9, None])
+def test_answering_under_autocast(device, name, window):
+    """A model of 32 bits fills its cache from keys of 16 and goes on from it."""
+    torch.manual_seed(7)
+    model = MoETransformer(preset(name, device=torch.device(device), dtype=torch.float32, mlp_impl='sparse',
+                                  **{**OPTIONS, 'attention_window': window}))
+    fixed_choice(model)
+    tokens = torch.randint(0, 512, (2, 12), device=device)
+    with torch.autocast(device, torch.bfloat16):
+        cache = model.new_cache(2, 12)
+        got = [model.prefill(tokens[:, :8], cache)]
+        got += [model.decode(tokens[:, i], cache) for i in range(8, 12)]
+        whole = model.eval()(tokens).float()
+    for i, logits in enumerate(got):
+        assert (logits.float() - whole[:, 7 + i]).abs().max() <= whole.abs().max() * 40 * 2.0**-8
