@@ -82,7 +82,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     # Not for fp16: there the loss scale has to reach the logit gradient before it is rounded (the
     # unscaled (softmax - onehot) / rows underflows), and the scale is only known in backward.
     if (hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float32) and hidden.dim() == 2
-            and weight.dtype == hidden.dtype and os.environ.get('MB200_FUSED_LM_LOSS', '1') != '0'):
+            and weight.dtype == hidden.dtype and not torch.is_autocast_enabled()
+            and os.environ.get('MB200_FUSED_LM_LOSS', '1') != '0'):
         return _LinearCrossEntropy.apply(hidden.contiguous(), weight, targets.contiguous())
     return cross_entropy(F.linear(hidden, weight), targets)
 

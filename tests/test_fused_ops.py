@@ -260,3 +260,23 @@ def test_linear_cross_entropy_matches_the_unfused_head_and_loss(device, rows, hi
     torch.testing.assert_close(h.grad.float().cpu(), hr.grad, **tol)
     wtol = dict(rtol=3e-2, atol=3e-2 * float(wr.grad.abs().max())) if dtype == torch.bfloat16 else tol
     torch.testing.assert_close(w.grad.float().cpu(), wr.grad, **wtol)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('loss', ['cross_entropy', 'distillation'])
+def test_head_and_loss_under_autocast(device, loss):
+    """As the head and the loss one after the other: the head's product in 16 bits, gradients in the weights' type."""
+    hidden, weight = (torch.randn(n, 32, device=device, requires_grad=True) for n in (24, 200))
+    targets = torch.randint(0, 200, (24,), device=device)
+    values, ids = torch.randn(24, 4, device=device), torch.randint(0, 200, (24, 4), device=device)
+    with torch.autocast(device, torch.bfloat16):
+        logits = F.linear(hidden, weight)
+        if loss == 'cross_entropy':
+            got, want = fused.linear_cross_entropy(hidden, weight, targets), fused.cross_entropy(logits.clone(), targets)
+        else:
+            got = fused.linear_distillation_loss(hidden, weight, values, ids)
+            want = fused.distillation_loss(logits, values, ids)
+    assert torch.equal(got, want)
+    for a, b, like in zip(torch.autograd.grad(got, (hidden, weight)), torch.autograd.grad(want, (hidden, weight)),
+                          (hidden, weight)):
+        assert a.dtype == like.dtype and torch.equal(a, b)
