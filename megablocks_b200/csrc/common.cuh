@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -62,5 +63,17 @@ __device__ __forceinline__ int upper_bound_i32(const int* __restrict__ ends, int
     case kI64: { using T = int64_t; __VA_ARGS__; break; }                    \
     default: return cudaErrorInvalidValue;                                   \
   }
+
+// Opts a kernel in to more shared memory than the default, once per device: `done` is the kernel's own record.
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool> (&done)[64]) {
+  int device = 0;
+  cudaError_t rc = cudaGetDevice(&device);
+  if (rc != cudaSuccess) return rc;
+  if (done[device & 63].load(std::memory_order_acquire)) return cudaSuccess;
+  rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (rc == cudaSuccess) done[device & 63].store(true, std::memory_order_release);
+  return rc;
+}
 
 }  // namespace mb

@@ -792,10 +792,10 @@ cudaError_t distill_fwd(DType type, const DistillArgs& a, float* stats, void* gr
     const int64_t row_bytes = (bytes + 15) / 16 * 16 + 16, shared = row_bytes + 3 * int64_t(slots);
     if (grad != nullptr && shared <= kSharedBytes) {
       auto kernel = distill_rows_kernel<T>;
-      if (shared > 48 * 1024) {
-        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
-        if (rc != cudaSuccess) return rc;
-      }
+      // The most that any row takes, once: the limit is the kernel's, and another thread may set and launch too.
+      static std::atomic<bool> allowed[64];
+      const cudaError_t rc = allow_shared(kernel, kSharedBytes, allowed);
+      if (rc != cudaSuccess) return rc;
       // As many CTAs as fit an SM, 24 warps between them, but no more than leave each thread four blocks.
       const int resident = max(1, int(min(int64_t(16), kSharedBytes / (shared + 1024))));
       const int threads = max(32, min(kRowThreads / resident, int((bytes + 63) / 64)) / 32 * 32);

@@ -1,8 +1,6 @@
 // Pieces that the windowed-attention kernels share.
 #pragma once
 
-#include <atomic>
-
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -130,18 +128,6 @@ __device__ __forceinline__ void settle(const volatile int* abort_flag) {
   if (*abort_flag == 0) return;
   const uint64_t t0 = globaltimer_ns();
   while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
-}
-
-// Opts a kernel in to more shared memory than the default, once per device: `done` is the kernel's own record.
-template <typename K>
-cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool> (&done)[64]) {
-  int device = 0;
-  cudaError_t rc = cudaGetDevice(&device);
-  if (rc != cudaSuccess) return rc;
-  if (done[device & 63].load(std::memory_order_acquire)) return cudaSuccess;
-  rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (rc == cudaSuccess) done[device & 63].store(true, std::memory_order_release);
-  return rc;
 }
 
 }  // namespace attn

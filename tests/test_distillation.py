@@ -1,6 +1,7 @@
 """Distillation from a teacher's top logits against its definition in 64 bits."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -368,3 +369,46 @@ def test_forward_mode_tangents(device, requires_grad):
         logits = forward_ad.make_dual(hidden @ weight.detach().t(), hidden @ way.t())
         want = forward_ad.unpack_dual(fused.distillation_loss(logits, values, ids, 2.0)).tangent
         torch.testing.assert_close(got, want)
+
+
+@pytest.mark.gpu
+def test_long_and_short_rows_in_one_recording_and_in_two_threads():
+    """A call with shorter rows, or with fewer slots, leaves the shared memory that one with longer rows has asked for."""
+    sizes = [(7, 100000, 40), (7, 30000, 8), (7, 60000, 64), (7, 500, 4)]
+    calls = [batch(rows, vocab, top, BF16, 'cuda') for rows, vocab, top in sizes]
+
+    def one(call):
+        logits, values, ids, targets = call
+        logits = logits.detach().requires_grad_(True)
+        loss = fused.distillation_loss(logits, values, ids, 2.0, targets, 0.5)
+        return loss.detach(), torch.autograd.grad(loss, logits)[0]
+
+    want = [one(c) for c in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = [one(c) for c in calls]
+    one(calls[3])
+    graph.replay()
+    torch.cuda.synchronize()
+    for got, exact in zip(recorded, want):
+        assert all(torch.equal(a, b) for a, b in zip(got, exact))
+
+    wrong = []
+
+    def loop(call, exact):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got = one(call)
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(n for n, (a, b) in enumerate(zip(got, exact)) if not torch.equal(a, b))
+        except RuntimeError as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=loop, args=x) for x in zip(calls, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
