@@ -88,20 +88,8 @@ class Arguments:
     moe_zloss_weight: float = 0
     moe_zloss_in_fp32: bool = False
 
-    # Extensions of this library (absent from the reference): how experts are selected
-    # (``ops.select_experts``).  ``moe_router_score``: 'softmax' or 'sigmoid' scores; ``moe_router_groups``
-    # groups of experts of which the best ``moe_router_top_groups`` stay (``None``: all); the weights are
-    # multiplied by ``moe_router_scale``.  ``moe_router_bias``: a bias per expert that takes part in the
-    # choice only, kept as a buffer of the router and moved against the load by
-    # ``layers.router.balance_routers`` (the trainer does, see ``TrainerConfig.router_bias_rate``), so that
-    # ``moe_loss_weight`` can be 0.
-    moe_router_score: str = 'softmax'
-    moe_router_bias: bool = False
-    moe_router_groups: int = 1
-    moe_router_top_groups: Optional[int] = None
-    moe_router_scale: float = 1.0
-
-    # Route the expert-parallel exchange through the fused peer-memory kernels instead of
+    # Extension of this library (absent from the reference): route the
+    # expert-parallel exchange through the fused peer-memory kernels instead of
     # NCCL all-to-all.  ``None`` picks the fused path whenever a symmetric
     # workspace can be created for ``expert_parallel_group``.
     ep_fused_comm: Optional[bool] = None
@@ -115,6 +103,18 @@ class Arguments:
     ep_max_copies: Optional[int] = None
     ep_capacity_rows: Optional[int] = None
     ep_inflight_microbatches: int = 1
+
+    # Another extension: how experts are selected (``ops.select_experts``).  ``moe_router_score``: 'softmax' or
+    # 'sigmoid' scores; ``moe_router_groups`` groups of experts of which the best ``moe_router_top_groups`` stay
+    # (``None``: all); the weights are multiplied by ``moe_router_scale``.  ``moe_router_bias``: a bias per
+    # expert that takes part in the choice only, kept as a buffer of the router and moved against the load by
+    # ``layers.router.balance_routers`` (the trainer does, see ``TrainerConfig.router_bias_rate``), so that
+    # ``moe_loss_weight`` can be 0.
+    moe_router_score: str = 'softmax'
+    moe_router_bias: bool = False
+    moe_router_groups: int = 1
+    moe_router_top_groups: Optional[int] = None
+    moe_router_scale: float = 1.0
 
     def __post_init__(self):
         if self.mlp_type not in _MLP_TYPES:

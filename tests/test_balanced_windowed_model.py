@@ -1,5 +1,6 @@
 """Expert selection, windowed attention, distillation and decoding as a model uses them together."""
 
+import dataclasses
 import math
 import os
 import subprocess
@@ -455,3 +456,15 @@ def test_answering_under_autocast(device, name, window):
         whole = model.eval()(tokens).float()
     for i, logits in enumerate(got):
         assert (logits.float() - whole[:, 7 + i]).abs().max() <= whole.abs().max() * 40 * 2.0**-8
+
+
+def test_positional_arguments_keep_their_places():
+    """What stood before the selection's options is given in the same places as without them."""
+    names = [f.name for f in dataclasses.fields(Arguments)]
+    old = [n for n in names if not n.startswith('moe_router_')]
+    assert names[:len(old)] == old
+    values = [getattr(Arguments(moe_num_experts=4), n) for n in old]
+    values[old.index('ep_fused_comm')] = False
+    values[old.index('ep_inflight_microbatches')] = 3
+    args = Arguments(*values)
+    assert args.ep_fused_comm is False and args.ep_inflight_microbatches == 3 and args.moe_router_score == 'softmax'
