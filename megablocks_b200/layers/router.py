@@ -123,8 +123,12 @@ class LearnedRouter(torch.nn.Module):
 
         self.register_buffer('expert_bias', vector(torch.float32))
         self.register_buffer('expert_load', vector(torch.int64), persistent=False)
-        self._selects = (args.moe_router_bias or args.moe_router_score != 'softmax' or args.moe_router_groups > 1
-                         or args.moe_router_scale != 1.0)
+
+    @property
+    def _selects(self) -> bool:
+        args = self.args
+        return (self.expert_bias is not None or args.moe_router_score != 'softmax' or args.moe_router_groups > 1
+                or args.moe_router_scale != 1.0)
 
     def _apply(self, fn, *args, **kwargs):
         bias = self.expert_bias

@@ -468,3 +468,21 @@ def test_positional_arguments_keep_their_places():
     values[old.index('ep_inflight_microbatches')] = 3
     args = Arguments(*values)
     assert args.ep_fused_comm is False and args.ep_inflight_microbatches == 3 and args.moe_router_score == 'softmax'
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('change', [dict(moe_router_scale=3.0), dict(moe_router_score='sigmoid'),
+                                    dict(moe_router_groups=4, moe_router_top_groups=1)])
+def test_options_replaced_on_a_router_are_used(device, change):
+    how = dict(hidden_size=64, moe_num_experts=16, moe_top_k=2, fp16=False, device=torch.device(device))
+    router = router_lib.LearnedRouter(Arguments(**how))
+    x = torch.randn(9, 64, device=device)
+    plain = router(x)[1]
+    router.args = Arguments(**how, **change)
+    logits = router.layer(x)
+    want = select_experts(logits, 2, score=router.args.moe_router_score, groups=router.args.moe_router_groups,
+                          top_groups=router.args.moe_router_top_groups, scale=router.args.moe_router_scale)
+    got = router(x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not torch.equal(got[1], plain)
+    router.args = Arguments(**how)
+    assert torch.equal(router(x)[1], plain)
