@@ -14,7 +14,8 @@ attention where ``attention_window`` or ``attention_sinks`` is set and wherever 
 everything MoE runs this library's kernels.  Inputs are ``[batch, seq]`` token ids.
 
 Beside training (``loss``, ``distillation_loss``) a model answers: ``prefill`` fills a :class:`KVCache` from a
-batch of prompts, ``decode`` takes one token per sequence further, ``generate`` does both greedily.
+batch of prompts, ``decode`` takes one token per sequence further, ``generate`` does both greedily.  No token is
+dropped in an answer, whatever the model's capacity factor.
 """
 
 import contextlib
@@ -438,23 +439,28 @@ class MoETransformer(nn.Module):
             return KVCache(*buffers, torch.zeros(batch, dtype=torch.int32, device=weight.device))
 
     @contextlib.contextmanager
-    def _answering(self):
+    def _answering(self, capacity_factor: float):
         """Without gradients and, whatever mode the model is in, without what only training does: the layers'
-        loss accumulators and load counts, jitter."""
+        loss accumulators and load counts, jitter, and tokens that are dropped, which would make an answer depend on
+        the padding and on the other sequences."""
         training = [m for m in self.modules() if m.training] if self.training else []
         for m in training:
             m.training = False
+        factor = self.moe_args.moe_capacity_factor
+        if not self.cfg.dropless:
+            self.moe_args.moe_capacity_factor = capacity_factor
         try:
             with torch.no_grad():
                 yield
         finally:
+            self.moe_args.moe_capacity_factor = factor
             for m in training:
                 m.training = True
 
     def prefill(self, tokens: torch.Tensor, cache: KVCache, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Fill the cache from prompts ``tokens[batch, seq]`` (``lengths[batch]`` valid tokens each, at least one;
         ``None``: all); returns the logits ``[batch, vocab]`` behind each prompt's last token."""
-        with self._answering():
+        with self._answering(0):            # as many places as the fullest expert needs
             return self._prefill(tokens, cache, lengths)
 
     def _prefill(self, tokens, cache, lengths):
@@ -485,7 +491,9 @@ class MoETransformer(nn.Module):
 
         A recorded call may be replayed: lengths advance on the device, and a token for which a sequence has no
         room takes the place of its last one."""
-        with self._answering():
+        # A place for every token with every expert, which takes no look at the counts and so can be recorded (2^-20:
+        # whatever the products round to, no place less).
+        with self._answering(self.cfg.moe_num_experts / self.cfg.moe_top_k * (1 + 2.0**-20)):
             return self._decode(tokens, cache)
 
     def _decode(self, tokens, cache):

@@ -486,3 +486,52 @@ def test_options_replaced_on_a_router_are_used(device, change):
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and not torch.equal(got[1], plain)
     router.args = Arguments(**how)
     assert torch.equal(router(x)[1], plain)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('name,top_k', [('tiny', 1), ('tiny-mixtral', 3)])
+@pytest.mark.parametrize('training', [False, True])
+def test_answers_of_models_that_drop_tokens(device, name, top_k, training):
+    """Nothing is dropped in an answer: it does not depend on padding or on other sequences, and agrees with a pass
+    over the whole sequence that drops nothing.  Training drops as before."""
+    model = build(device, name, dropless=False, moe_capacity_factor=1, moe_top_k=top_k, moe_router_groups=1,
+                  moe_router_top_groups=None).train(training)
+    fixed_choice(model)                         # all tokens to the same experts: most would be dropped
+    tokens = torch.randint(0, 512, (3, 20), device=device)
+    lengths = torch.tensor([12, 5, 1], dtype=torch.int32, device=device)
+    cache = model.new_cache(3, 16)
+    got = [model.prefill(tokens[:, :12], cache, lengths)]
+    for i in range(3):
+        got.append(model.decode(tokens[torch.arange(3), (lengths + i).long()], cache))
+    assert model.moe_args.moe_capacity_factor == 1 and model.training == training
+    with pytest.raises(ValueError):
+        model.prefill(tokens, cache)
+    assert model.moe_args.moe_capacity_factor == 1
+    model.eval()
+    dropped = model(tokens[:1, :12])[0, -1].float()
+    model.moe_args.moe_capacity_factor = 0
+    with torch.no_grad():
+        for b, n in enumerate(lengths.tolist()):
+            whole = model(tokens[b:b + 1, :n + 3])[0].float()
+            size = whole.abs().max()
+            for i in range(4):
+                bound = size * (2.0**-12 if device == 'cpu' else 40 * 2.0**-8)
+                assert (got[i][b].float() - whole[n - 1 + i]).abs().max() <= bound
+    assert (got[0][0].float() - dropped).abs().max() > 0
+
+
+@pytest.mark.gpu
+def test_recorded_decoding_of_a_model_that_drops_tokens():
+    model = build('cuda', 'tiny', dropless=False, moe_capacity_factor=1).eval()
+    tokens = torch.randint(0, 512, (3, 6), device='cuda')
+    eager, cache = model.new_cache(3, 10), model.new_cache(3, 10)
+    for c in (eager, cache):
+        model.prefill(tokens, c)
+    want = [model.decode(tokens[:, i], eager) for i in range(3)]
+    static, graph = tokens[:, 0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = model.decode(static, cache)
+    for i in range(3):
+        static.copy_(tokens[:, i])
+        graph.replay()
+        assert torch.equal(out, want[i])
