@@ -130,10 +130,12 @@ std::vector<at::Tensor> window_backward(const at::Tensor& dout, const at::Tensor
                   lse.numel() == int64_t(p.batch) * p.heads * p.seq_pad, "window_attention: bad log-sum-exp");
   const bool bf16 = q.scalar_type() == at::kBFloat16;
   const int rows = attn::streamed_rows(p.dim);
-  // In a short sequence most rows see a few keys, whose dS nearly cancel, and there are few rows to average over:
-  // with P and dS rounded once, gradients were off by up to 1.56 times their own rounding, as two numbers each by
-  // 1.06 (64 tokens) to 1.4 (2 tokens).  It costs 1.4 us of 11 there (4 x 64 tokens, 4 heads of 32), and 15 to 25 %
-  // of a long sequence's backward pass, whose gradients are off by 1.41 to 1.5 without.
+  // P and dS, rounded once, leave dq and dk off by 1.43 to 1.53 times what their own rounding does, at every length;
+  // as two numbers each by 1.02 (512 tokens) to 1.15 (2 tokens).  Few terms scatter, though: 1 in 20 sequences is off by
+  // more than 2.3 times at 2 tokens, 1.6 at 15, 1.5 at 64, 1.45 at 512; as two numbers 1.7, 1.13, 1.07 and 1.03.  The
+  // price is 7 to 10 % of the backward pass while a sequence is one streamed tile (512 x 64 tokens, 12 heads of 64: 265
+  // and 285 us), 14 % at 8 x 1024 and 25 % at 4096 tokens of heads of 128.  So sequences of one tile take it, by
+  // their padded length: the host does not know the others.
   p.split = p.seq <= 64;
   at::Tensor dq, dk, dv, far;
   at::Tensor delta = at::empty_like(lse);
