@@ -32,7 +32,6 @@ at::Tensor scatter_wgrad_op(const at::Tensor& x, const at::Tensor& grad, const a
 at::Tensor binned_scatter_wgrad(const at::Tensor& x, const at::Tensor& grad, const at::Tensor& indices,
                                 const at::Tensor& bins, int64_t top_k);
 at::Tensor column_sum_op(const at::Tensor& x);
-// The device's status word, which kernels that give up a wait write, and the count of launched kernels.
 // Gradients of a pass that has no gradient itself: where one is asked for (create_graph), taking it is an error
 // rather than zero.
 inline torch::autograd::variable_list once_differentiable(torch::autograd::variable_list grads, const char* name) {
@@ -53,6 +52,7 @@ inline torch::autograd::variable_list once_differentiable(torch::autograd::varia
   return grads;
 }
 
+// The device's status word, which kernels that give up a wait write, and the count of launched kernels.
 int* device_status(const at::Device& device);
 void count_launches(int64_t n);
 // Tensor map of a 16-bit tensor (innermost dimension dense, `strides` in bytes of the others), 128-byte swizzle.

@@ -260,9 +260,10 @@ class Block(nn.Module):
         self.moe = (dMoE if cfg.dropless else MoE)(moe_args)
 
     def forward(self, x: torch.Tensor, delta, delta_bias, rope, attend=None):
-        """``attend`` (optional) takes the place of the attention layer's forward pass.  The residual stream arrives as ``x + delta + delta_bias`` (``delta`` may be ``None``;
+        """The residual stream arrives as ``x + delta + delta_bias`` (``delta`` may be ``None``;
         ``delta_bias`` is the previous MoE layer's output bias, one value per column, or ``None``)
-        and leaves the same way, so every residual add rides in the following norm's kernels."""
+        and leaves the same way, so every residual add rides in the following norm's kernels.
+        ``attend`` (optional) takes the place of the attention layer's forward pass."""
         x, normed = _add_norm(self.ln1, x, delta, delta_bias)
         x, normed = _add_norm(self.ln2, x, self.attn(normed, rope) if attend is None else attend(self.attn, normed))
         # The MoE layer is token-wise: it flattens every leading dimension, so the
