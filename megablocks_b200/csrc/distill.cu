@@ -14,8 +14,10 @@
 // L2.  The few columns that the teacher or the target names are written again, with their whole value and one
 // rounding, after the row.
 //
-// 8192 rows of 51200 bf16 logits, 64 of the teacher: 332 us (1.68 GB, 0.78 of the copy bandwidth), 347 with the mean
-// and the backward pass's factor; half of the exponentials' rate, half of the issue slots.
+// 8192 rows of 51200 bf16 logits, 64 of the teacher: 333 us at 1965 MHz (1.68 GB, 0.77 of the copy bandwidth); pass
+// after pass, at the 1880 MHz that the power limit leaves, 343, and 351 with the mean and the backward pass's factor.
+// Neither the exponential unit (0.56 of its rate) nor the issue slots (0.51) nor memory is full: the barriers
+// between a row's passes leave each of them idle in turn.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 

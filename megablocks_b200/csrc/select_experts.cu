@@ -18,8 +18,10 @@
 // short, as the last token's latency is the launch's: with all of the choice redone a launch of 37 us ended 13 us
 // later for five tokens with close groups.
 //
-// 32768 x 256 bf16 in 8 groups, sigmoid and bias: 40 us (36 MB, 0.14 of the copy bandwidth), bound by
-// instructions, 874 a token at 3.1 a cycle and SM; backward 12 us at 0.6 of it.
+// 32768 x 256 bf16 in 8 groups, sigmoid and bias: 39 us (36 MB, 0.14 of the copy bandwidth), bound by
+// instructions, 900 a token, of which 0.84 a cycle and scheduler are issued.  Backward from the weights alone 12 us:
+// the chosen logits' sectors, ids, gradients and the rows written are 28 MB, 0.37 of the copy bandwidth; its loads
+// wait for the ids (11 of 17 cycles between a warp's instructions).
 #include "common.cuh"
 
 namespace mb {

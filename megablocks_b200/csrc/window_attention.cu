@@ -15,12 +15,13 @@
 // on the first half of a tile's probabilities while the second half is taken.
 //
 // Time, and rate of the visible pairs' products (4 dim operations each):
-//   1 x 16384 tokens, 32 query heads over 8 key heads of 128, window 4096: 0.94 ms, 1020 TFLOP/s, 0.63 of cuBLAS's;
-//     the products' operands from shared memory and the 128 x 128 exponentials of a tile take about as long
-//   1 x 8191, the same heads, window 1024: 205 us, 620 TFLOP/s; prologue and epilogue are a quarter of a CTA
+//   1 x 16384 tokens, 32 query heads over 8 key heads of 128, window 4096: 0.97 ms at 1965 MHz, 990 TFLOP/s, 0.61 of
+//     cuBLAS's burst (pass after pass 0.99 ms, at the 1665 MHz that the power limit leaves); tensor cores busy 0.51 of the
+//     time, exponential unit 0.53: the products' operands from shared memory take about as long
+//   1 x 8191, the same heads, window 1024: 208 us, 620 TFLOP/s; prologue and epilogue are a quarter of a CTA
 //   6 x up to 1999, 16 over 4 heads of 96, window 512: 94 us
-//   8 x 1024, 12 heads of 64, window 256: 38 us, 150 TFLOP/s, 1.7 TB/s; three or four tiles a CTA, half of them
-//     edges, so that prologue, epilogue and hidden pairs are most of it
+//   8 x 1024, 12 heads of 64, window 256: 37 us, 155 TFLOP/s, 1.7 TB/s; three or four tiles a CTA, half of them
+//     edges, so that prologue, epilogue and hidden pairs are most of it (tensor cores busy 0.16 of the time)
 // CTAs that start in the order of their lengths ended 8 % sooner than in the order of memory on the last three.
 #include "window_attention.cuh"
 

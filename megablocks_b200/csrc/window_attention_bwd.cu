@@ -19,9 +19,10 @@
 // with 64, reading the resident operand from shared memory again for half the columns set the pace.
 //
 // Time of the keys' and the queries' kernel, and rate of the visible pairs' products (8 and 6 dim operations each):
-//   1 x 16384 tokens, 32 query heads over 8 key heads of 128, window 4096: 1.65 and 1.27 ms, 1160 and 1130 TFLOP/s,
-//     0.7 of cuBLAS's, bound by the MMAs and their operands; row sums 68 us (5.9 TB/s)
-//   6 x up to 1999, 16 over 4 heads of 96, window 512: 99 and 97 us, row sums 18
+//   1 x 16384 tokens, 32 query heads over 8 key heads of 128, window 4096: 1.69 and 1.32 ms at 1965 MHz, 1140 and 1100
+//     TFLOP/s, 0.70 and 0.67 of cuBLAS's burst (pass after pass 1.72 and 1.34 ms, at the 1665 MHz that the power limit
+//     leaves); tensor cores busy 0.59 and 0.56 of the time, the MMAs and their operands; row sums 68 us (5.9 TB/s)
+//   6 x up to 1999, 16 over 4 heads of 96, window 512: 98 and 96 us, row sums 18
 //   8 x 1024, 12 heads of 64, window 256: 44 and 30 us, row sums 7.5, far queries' sums 2.8; short streams
 // Row sums taken by the queries' kernel, while its first tiles arrive, cost it more than theirs does (97 -> 143 us in
 // the second case): nothing hides the loads at the start of a CTA.

@@ -10,8 +10,8 @@
 // run on warp-level MMAs: 16 rows would leave the 128-row tensor-memory ones seven eighths empty, and the
 // memory sets the pace.
 //
-// 64 sequences of up to 8192 keys, 32 over 8 heads of 128, window 4096: 167 us, 5.5 TB/s of visible keys and values, 0.84
-// of the copy bandwidth; sequences of different lengths end at different times.  One sequence: 12 us for 16.8 MB, of
+// 64 sequences of up to 8192 keys, 32 over 8 heads of 128, window 4096: 170 us, 5.4 TB/s of visible keys and values, 0.82
+// of the copy bandwidth; sequences of different lengths end at different times.  One sequence: 12.4 us for 16.8 MB, of
 // which the launch of a cluster and the join are 6 and the rest a chain of 16-key steps.
 #include <cstdint>
 

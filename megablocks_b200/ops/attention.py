@@ -11,6 +11,10 @@ On CUDA, 16-bit tensors with head sizes up to 128 (multiples of 8) run on the te
 (``csrc/window_attention*.cu``): nothing of the size ``seq x seq`` is stored, keys outside the window are not
 read, and the gradients are the same in every run.  Everything else, calls with forward-mode tangents or under
 functional transforms among it, is composed of PyTorch ops, which do store the scores.
+
+Products are taken over whole tiles, with probabilities of zero for pairs that are hidden by the window: NaN or an
+infinity in ``v`` (in any input, for the gradients) may reach other tokens of the sequence than those that see it.
+Behind a sequence's end, and out of sight of a decoded token, anything may stand.
 """
 
 import math
