@@ -139,7 +139,8 @@ class LearnedRouter(torch.nn.Module):
         return self
 
     def count_load(self, tokens_per_expert: torch.Tensor) -> None:
-        """Add one forward pass's tokens per expert to the load that :func:`balance_routers` goes by."""
+        """Add one forward pass's tokens per expert to the load that :func:`balance_routers` goes by.  A pass that
+        activation checkpointing runs again may count again, for all experts alike, which moves no bias differently."""
         if self.expert_load is not None:
             self.expert_load.add_(tokens_per_expert.detach())
 
