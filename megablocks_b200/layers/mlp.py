@@ -140,7 +140,11 @@ class MLP(_ExpertWeights):
     def _uniform_bins(self, experts: int, capacity: int, device) -> torch.Tensor:
         key = (experts, capacity, str(device))
         if key not in self._bins_cache:
-            self._bins_cache[key] = (torch.arange(1, experts + 1, dtype=torch.int32, device=device) * capacity)
+            with torch.inference_mode(False):                   # training may use them next
+                bins = torch.arange(1, experts + 1, dtype=torch.int32, device=device) * capacity
+            if bins.is_cuda and torch.cuda.is_current_stream_capturing():
+                return bins                                     # filled by the replays only: not for others
+            self._bins_cache[key] = bins
         return self._bins_cache[key]
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

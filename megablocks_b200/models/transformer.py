@@ -313,7 +313,7 @@ class MoETransformer(nn.Module):
         step or decode call reads them where they are."""
         if self.cfg.flavour != 'mixtral':
             return None
-        kept = self._ropes.setdefault(torch.empty(0, device=device).device, [])
+        kept = self._ropes.setdefault(device, [])
         if not kept or kept[-1][0].shape[0] < seq:
             size = max(seq, self.cfg.max_seq_len, 2 * kept[-1][0].shape[0] if kept else 0)
             with torch.inference_mode(False):                   # training may use them next

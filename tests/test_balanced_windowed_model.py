@@ -535,3 +535,39 @@ def test_recorded_decoding_of_a_model_that_drops_tokens():
         static.copy_(tokens[:, i])
         graph.replay()
         assert torch.equal(out, want[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('training', [False, True])
+def test_bins_made_during_a_recording_are_its_own(training):
+    """The first call with a number of tokens may be recorded: calls that follow, before a replay, take bins that are
+    filled."""
+    model = build('cuda', 'tiny', dropless=False, moe_capacity_factor=1).train(training)
+    tokens = torch.randint(0, 512, (3, 6), device='cuda')
+    cache, spare = model.new_cache(3, 10), model.new_cache(3, 10)
+    for c in (cache, spare):
+        model.prefill(tokens, c)
+    want = build('cuda', 'tiny', dropless=False, moe_capacity_factor=1).eval()
+    exact = want.new_cache(3, 10)
+    want.prefill(tokens, exact)
+    want = want.decode(tokens[:, 0], exact)
+    graph = torch.cuda.CUDAGraph()
+    known = [set(b.moe.experts.mlp._bins_cache) for b in model.blocks]
+    with torch.cuda.graph(graph):
+        out = model.decode(tokens[:, 0], cache)
+    assert [set(b.moe.experts.mlp._bins_cache) for b in model.blocks] == known
+    assert torch.equal(model.decode(tokens[:, 0], spare), want)
+    graph.replay()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_training_behind_answers_in_inference_mode_of_a_model_that_drops_tokens(device):
+    model = build(device, 'tiny', dropless=False, moe_capacity_factor=1)
+    tokens = torch.randint(0, 512, (1, 8), device=device)
+    with torch.inference_mode():
+        model.eval()(tokens)                    # as many tokens as the training step has
+        model.generate(tokens, 3)
+    total, _ = model.train().loss(tokens, tokens.roll(-1, 1))
+    total.backward()
+    assert all(torch.isfinite(p.grad).all() for p in model.parameters() if p.grad is not None)
