@@ -2,6 +2,7 @@
 // TMA tensor maps and calls into the torch-free kernel launchers of kernels.h.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -581,7 +582,8 @@ at::Tensor& status_word(const at::Device& device) {
   const int idx = device.index();
   if (!(*words)[idx].defined()) {
     // On a stream of its own: were the first use inside a recording, zeroing it would be recorded, and repeated by
-    // every replay, instead of done.
+    // every replay, instead of done.  And not in inference mode, outside of which it could not be cleared.
+    c10::InferenceMode writable(false);
     c10::cuda::CUDAGuard guard(device);
     c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
     const auto side = c10::cuda::getStreamFromPool(false, idx);

@@ -12,6 +12,7 @@ import os
 import shutil
 import socket
 import subprocess
+import sys
 import time
 
 import pytest
@@ -177,3 +178,31 @@ def test_extension_shares_the_cpp_runtime_of_torch():
         pytest.skip('needs the built extension and nm')
     symbols = subprocess.run(['nm', '-D', '--defined-only', _ext.ext().__file__], capture_output=True, text=True, check=True)
     assert '_ZNSo9_M_insert' not in symbols.stdout       # std::ostream << number, defined in libstdc++ alone
+
+
+_IN_INFERENCE_MODE = """
+import sys, torch
+sys.path.insert(0, {root!r})
+from megablocks_b200 import ops
+from megablocks_b200._ext import ext
+from megablocks_b200.utils import status
+x = torch.randn(1, 40, 2, 64, device='cuda').bfloat16()
+with torch.inference_mode():
+    ops.window_attention(x, x, x, 8, 2)                         # the process's first use of the status word
+ext().ep_wait_flags(torch.zeros(8, dtype=torch.int32, device='cuda'), 2, 5, 19, None)
+for clear in (True, False):
+    try:
+        status.check()
+    except status.DeviceWaitTimeout:
+        assert clear
+    else:
+        assert not clear
+"""
+
+
+@pytest.mark.gpu
+def test_status_of_a_process_that_begins_in_inference_mode():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, '-c', _IN_INFERENCE_MODE.format(root=root)], capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
